@@ -58,12 +58,18 @@ extern "C" {
 #define UA_TILE 128        /* rows and columns of one kernel tile */
 #define UA_HEAD_DIM 128    /* the only supported head dimension */
 #define UA_MAX_PARTS 16    /* most partial outputs one ua_merge call combines */
+#define UA_ROPE_MAX_DIM 512 /* largest head_dim of the rotary entry points */
 #define UA_NOALLOC_MAX_LINES 65532   /* most query tiles + key tiles of ua_tilelist_build_device_noalloc */
+
+/* Element types of the entry points that take more than bf16. */
+#define UA_BF16 0
+#define UA_FP16 1
+#define UA_FP32 2
 
 /* 100 * major + minor.  102: `nnz` argument of the attention entry points, ua_merge_update, the
  * no-allocation builder, `work` of ua_tilelist_build_device grown to n_qtiles + n_ktiles + 7.  104: ua_bsa_bwd.
- * 105: ua_tilelist_build_device_scratch.  106: ua_copy_in.  */
-#define UA_VERSION 106
+ * 105: ua_tilelist_build_device_scratch.  106: ua_copy_in.  107: ua_rope, ua_rope_append.  */
+#define UA_VERSION 107
 int ua_version(void);
 const char *ua_strerror(int rc);
 
@@ -297,6 +303,35 @@ int ua_cols_scatter(const void *src, void *dst, int n_chunks, int batch, int64_t
  * device can address, or from device memory, to the device, by a kernel on `stream`; both 16-byte aligned.  For what
  * is made on the host for one call: a tile list, a block mask.  The host memory has to stay until the kernel is through. */
 int ua_copy_in(void *dst, const void *src, int64_t bytes, void *stream);
+
+/* ---- rotary positions --------------------------------------------------------------------------
+ * No counterpart in the reference, whose executors are given Q and K with their positions in them.
+ * Pair i of the first rotary_dim (even, <= head_dim <= UA_ROPE_MAX_DIM) entries of every head is turned by the angle
+ * position * freqs[i]:  (a, b) -> scale * (a cos - b sin, b cos + a sin).  The pairs are (x[i], x[i + rotary_dim / 2]), or with
+ * `interleaved` (x[2i], x[2i + 1]); the rest of the head passes through unchanged.  inverse != 0 turns back, which, with
+ * the same scale, is the gradient: dx = ua_rope(dy, inverse).
+ * x [batch, seqlen, heads, head_dim] of `dtype` (UA_BF16, UA_FP16, UA_FP32) with (batch, token, head) element strides, any
+ * of them; wide strides and pointers (16 bytes) make wide accesses.  q and k are turned in one launch; n_kv_heads = 0 (or n_heads = 0) leaves one
+ * out.  Outputs may be exactly the inputs (same pointer and strides) or not overlap them.
+ * freqs: DEVICE array of rotary_dim / 2 doubles, radians per position.  The angle is reduced in twice 64 bits: far positions lose
+ * nothing.  positions: DEVICE array of int32 (positions_64 = 0) or int64, read at b * position_stride_b + s * position_stride_s; NULL:
+ * token s is at start + s. */
+int ua_rope(const void *q, const void *k, void *q_out, void *k_out, const double *freqs,
+            const void *positions, int positions_64, int64_t position_stride_b, int64_t position_stride_s, int64_t start,
+            int batch, int seqlen, int n_heads, int n_kv_heads, int head_dim, int rotary_dim,
+            int dtype, int interleaved, int inverse, float scale,
+            const int64_t *q_strides, const int64_t *k_strides, const int64_t *q_out_strides, const int64_t *k_out_strides,
+            void *stream);
+
+/* The new tokens of a serving step: token t (of n_new) of sequence b is at position lens[b] - n_new + t, where lens (DEVICE,
+ * int32 [batch]) are the lengths WITH the new tokens.  q is turned into q_out; k, turned, and v are written to row
+ * `position` of k_cache and v_cache [batch, room, n_kv_heads, head_dim].  Rows outside [0, room) are not written (a sequence shorter than
+ * n_new, a full cache), no other row of the caches is touched.  q_out may be q; the caches must not overlap the inputs. */
+int ua_rope_append(const void *q, const void *k, const void *v, void *q_out, void *k_cache, void *v_cache, const double *freqs,
+                   const int32_t *lens, int batch, int n_new, int n_heads, int n_kv_heads, int room, int head_dim, int rotary_dim,
+                   int dtype, int interleaved, float scale,
+                   const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides,
+                   const int64_t *q_out_strides, const int64_t *k_cache_strides, const int64_t *v_cache_strides, void *stream);
 
 #ifdef __cplusplus
 }

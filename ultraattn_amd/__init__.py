@@ -10,6 +10,9 @@ def __getattr__(name):
     if name in ("bsa_fwd", "bsa_bwd", "merge_partials", "softmax_delta", "update_out_and_lse", "grad_accumulate", "grad_sum"):
         from . import ops
         return getattr(ops, name)
+    if name in ("rope_freqs", "rope_fwd", "rope_bwd", "rope_append"):
+        from . import rope
+        return getattr(rope, name)
     if name in ("BlockSparseExecutor", "mask_from_comp_kernels", "comp_kernels_from_schedule"):
         from . import executor
         return getattr(executor, name)

@@ -38,6 +38,8 @@ SIGNATURES = {
     "ua_grad_sum": (c_int, [POINTER(c_void_p), c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, _i64p, c_float, c_void_p]),
     "ua_cols_gather": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p]),
     "ua_cols_scatter": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p]),
+    "ua_rope": (c_int, [c_void_p] * 6 + [c_int] + [c_int64] * 3 + [c_int] * 9 + [c_float] + [_i64p] * 4 + [c_void_p]),
+    "ua_rope_append": (c_int, [c_void_p] * 8 + [c_int] * 9 + [c_float] + [_i64p] * 6 + [c_void_p]),
     "ua_copy_in": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }
 

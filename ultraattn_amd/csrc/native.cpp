@@ -21,6 +21,7 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <vector>
 #include "../../include/ultraattn.h"
 
 namespace {
@@ -639,6 +640,148 @@ PyObject* permute_cols(PyObject* const* a) {
   return out.wrap();
 }
 
+// ---- rotary positions, sliding windows: what these operators check ------------------------------------------------
+int dtype_code(const char* name, const at::Tensor& t, bool fp32) {
+  const at::ScalarType dt = t.scalar_type();
+  if (dt == at::kBFloat16) return UA_BF16;
+  if (dt == at::kHalf) return UA_FP16;
+  if (dt == at::kFloat && fp32) return UA_FP32;
+  fail(PyExc_TypeError, std::string(name) + " must be bfloat16" + (fp32 ? ", float16 or float32" : " or float16") + ", got " + c10::toString(dt));
+}
+// A row tensor [B, S, H, D] of a type and device, head_dim contiguous.
+void check_rows4(const char* name, const at::Tensor& t, const at::Tensor& ref) {
+  if (!t.is_cuda()) fail(PyExc_ValueError, std::string(name) + " must be a CUDA (HIP) tensor");
+  if (t.device() != ref.device()) fail(PyExc_ValueError, std::string(name) + " is on another device than the first tensor");
+  if (t.scalar_type() != ref.scalar_type())
+    fail(PyExc_TypeError, std::string(name) + " must be " + c10::toString(ref.scalar_type()) + ", got " + c10::toString(t.scalar_type()));
+  if (t.dim() != 4) fail(PyExc_ValueError, std::string(name) + " must be [B, S, H, D], got " + shape_str(t.sizes()));
+  if (t.stride(3) != 1 && t.size(3) != 1) fail(PyExc_ValueError, std::string(name) + ": head_dim axis must be contiguous");
+  for (int i = 0; i < 4; ++i)
+    if (t.size(i) > INT32_MAX) fail(PyExc_ValueError, std::string(name) + " is too long: " + shape_str(t.sizes()));
+}
+void check_shape(const char* name, const at::Tensor& t, at::IntArrayRef want) {
+  if (!t.sizes().equals(want)) fail(PyExc_ValueError, std::string(name) + " has shape " + shape_str(t.sizes()) + ", expected " + shape_str(want));
+}
+// A result tensor: no element at the address of another (an expanded view would be written by several at once).
+void check_written(const char* name, const at::Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> d;
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) == 0) return;
+    if (t.size(i) > 1) d.emplace_back(t.stride(i), t.size(i));
+  }
+  std::sort(d.begin(), d.end());
+  int64_t extent = 1;
+  for (const auto& [stride, size] : d) {
+    if (stride < extent) fail(PyExc_ValueError, std::string(name) + " is written to: its elements must not overlap (strides " + shape_str(t.strides()) + ")");
+    extent += stride * (size - 1);
+  }
+}
+at::Tensor result(Slot& s, const char* name, const at::Tensor& ref) {
+  if (!s.given) return s.t = like(ref);
+  s.t = tensor(s.given, name);
+  check_rows4(name, s.t, ref);
+  check_shape(name, s.t, ref.sizes());
+  check_written(name, s.t);
+  return s.t;
+}
+const double* frequencies(const at::Tensor& f, const at::Tensor& x, int64_t& rotary) {
+  if (f.scalar_type() != at::kDouble || f.dim() != 1 || !f.is_contiguous() || f.device() != x.device())
+    fail(PyExc_ValueError, "freqs must be a contiguous float64 vector on the tensors' device");
+  rotary = 2 * f.numel();
+  if (rotary < 2 || rotary > x.size(3))
+    fail(PyExc_ValueError, "freqs holds " + std::to_string(f.numel()) + " pairs, a head of " + std::to_string(x.size(3)) + " has room for 1 to " +
+                               std::to_string(x.size(3) / 2));
+  return (const double*)f.data_ptr();
+}
+const int32_t* lengths(const at::Tensor& l, const at::Tensor& x) {
+  if (l.scalar_type() != at::kInt || l.dim() != 1 || l.size(0) != x.size(0) || !l.is_contiguous() || l.device() != x.device())
+    fail(PyExc_ValueError, "lens must be a contiguous int32 vector of one length per sequence on the tensors' device");
+  return (const int32_t*)l.data_ptr();
+}
+float positive(PyObject* o, const char* name) {
+  const float x = (float)number(o);
+  if (!(x > 0.f) || std::isinf(x)) fail(PyExc_ValueError, std::string(name) + " must be a positive number");
+  return x;
+}
+
+// rope(q, k, freqs, positions, start, interleaved, inverse, scale, q_out, k_out) -> (q_out, k_out)
+PyObject* rope(PyObject* const* a) {
+  const at::Tensor& q = tensor(a[0], "q");
+  const int dt = dtype_code("q", q, true);
+  check_rows4("q", q, q);
+  const bool has_k = a[1] != Py_None;
+  const at::Tensor& k = has_k ? tensor(a[1], "k") : q;
+  if (has_k) {
+    check_rows4("k", k, q);
+    check_shape("k", k, {q.size(0), q.size(1), k.size(2), q.size(3)});
+  }
+  int64_t rotary;
+  const double* f = frequencies(tensor(a[2], "freqs"), q, rotary);
+  const void* pos = nullptr;
+  int pos64 = 0;
+  int64_t pos_b = 0, pos_s = 0;
+  if (a[3] != Py_None) {
+    const at::Tensor& t = tensor(a[3], "positions");
+    if (t.device() != q.device() || (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) || t.dim() < 1 || t.dim() > 2 ||
+        t.size(t.dim() - 1) != q.size(1) || (t.dim() == 2 && t.size(0) != q.size(0)))
+      fail(PyExc_ValueError, "positions must be an int32 or int64 tensor [S] or [B, S] on the tensors' device, got " + shape_str(t.sizes()));
+    pos = t.data_ptr();
+    pos64 = t.scalar_type() == at::kLong;
+    pos_s = t.stride(t.dim() - 1);
+    pos_b = t.dim() == 2 ? t.stride(0) : 0;
+  }
+  const int64_t start = integer(a[4]);
+  const bool interleaved = truth(a[5]), inverse = truth(a[6]);
+  const float scale = positive(a[7], "scale");
+  Slot qo(a[8]), ko(a[9]);
+  if (!has_k && ko.given) fail(PyExc_ValueError, "k_out without k");
+  result(qo, "q_out", q);
+  if (has_k) result(ko, "k_out", k);
+  const On on(q);
+  call("ua_rope", [&] {
+    return ua_rope(q.data_ptr(), has_k ? k.data_ptr() : nullptr, qo.t.data_ptr(), has_k ? ko.t.data_ptr() : nullptr, f, pos, pos64, pos_b, pos_s, start,
+                   (int)q.size(0), (int)q.size(1), (int)q.size(2), has_k ? (int)k.size(2) : 0, (int)q.size(3), (int)rotary, dt, interleaved, inverse,
+                   scale, Strides(q), Strides(k), Strides(qo.t), Strides(has_k ? ko.t : qo.t), on.stream);
+  });
+  if (has_k) return tuple_of(qo, ko);
+  PyObject* r = PyTuple_New(2);
+  PyTuple_SET_ITEM(r, 0, qo.wrap());
+  Py_INCREF(Py_None);
+  PyTuple_SET_ITEM(r, 1, Py_None);
+  return r;
+}
+
+// rope_append(q, k, v, k_cache, v_cache, lens, freqs, interleaved, scale, q_out) -> q_out
+PyObject* rope_append(PyObject* const* a) {
+  const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &kc = tensor(a[3], "k_cache"), &vc = tensor(a[4], "v_cache");
+  const int dt = dtype_code("q", q, true);
+  check_rows4("q", q, q);
+  check_rows4("k", k, q);
+  check_rows4("v", v, q);
+  check_rows4("k_cache", kc, q);
+  check_rows4("v_cache", vc, q);
+  check_shape("k", k, {q.size(0), q.size(1), k.size(2), q.size(3)});
+  check_shape("v", v, k.sizes());
+  check_shape("k_cache", kc, {k.size(0), kc.size(1), k.size(2), k.size(3)});
+  check_shape("v_cache", vc, kc.sizes());
+  check_written("k_cache", kc);
+  check_written("v_cache", vc);
+  const int32_t* lens = lengths(tensor(a[5], "lens"), q);
+  int64_t rotary;
+  const double* f = frequencies(tensor(a[6], "freqs"), q, rotary);
+  const bool interleaved = truth(a[7]);
+  const float scale = positive(a[8], "scale");
+  Slot qo(a[9]);
+  result(qo, "q_out", q);
+  const On on(q);
+  call("ua_rope_append", [&] {
+    return ua_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), qo.t.data_ptr(), kc.data_ptr(), vc.data_ptr(), f, lens, (int)q.size(0),
+                          (int)q.size(1), (int)q.size(2), (int)k.size(2), (int)kc.size(1), (int)q.size(3), (int)rotary, dt, interleaved, scale, Strides(q),
+                          Strides(k), Strides(v), Strides(qo.t), Strides(kc), Strides(vc), on.stream);
+  });
+  return qo.wrap();
+}
+
 // ---- module ---------------------------------------------------------------------------------------------
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -664,7 +807,7 @@ PyMethodDef methods[] = {
     UA_METHOD(dense_forward, 8), UA_METHOD(dense_backward, 14), UA_METHOD(bsa_forward, 10), UA_METHOD(bsa_backward, 15),
     UA_METHOD(delta, 3), UA_METHOD(grad_accumulate, 4), UA_METHOD(merge, 4), UA_METHOD(grad_sum, 3),
     UA_METHOD(merge_update, 5), UA_METHOD(permute_cols, 6), UA_METHOD(lists_from_mask, 5),
-    UA_METHOD(build_lists_device, 3), {nullptr, nullptr, 0, nullptr}};
+    UA_METHOD(build_lists_device, 3), UA_METHOD(rope, 10), UA_METHOD(rope_append, 10), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "Native host side of the attention operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,295 @@
+// Rotary positions: pair i of the first `rotary_dim` entries of every head is turned by the angle position * freqs[i],
+//   (a, b) -> scale * (a cos - b sin, b cos + a sin),
+// with pairs (x[i], x[i + rotary_dim / 2]) or, interleaved, (x[2i], x[2i + 1]); the rest of the head passes through.  The
+// gradient is the turn by the negative angle with the same scale.  The appending form also sends K, rotated, and V to
+// their places in a cache.
+//
+// Bound: HBM, each row in and out once.  The angles are not read from a table: a workgroup makes the cosines and sines of its tokens once, in
+// LDS, and all heads of a token, of Q and of K, use them.
+#include <algorithm>
+#include "ua_common.h"
+
+namespace ua {
+
+typedef _Float16 fp16;
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeAngles = 512;           // pairs of all of a workgroup's tokens (a head of 256 has up to 128)
+constexpr int kRopeMaxTokens = 16;
+constexpr int kRopeAhead = 4;              // items of a thread whose loads are in flight together
+
+// One of the tensors that a call goes through: x [batch, tokens, heads, head_dim] to y, turned or (kRotate = 0) as it is.  An item is
+// one or two vectors of a head: a pair of them that is turned, or two neighbours that pass through.
+struct RopeTensor {
+  const void* x; void* y;
+  Strides3 xs, ys;
+  int rotate, cached;        // cached: y's row is the token's position, [0, room), not its index
+  int items;                 // of a token, all heads
+  Div by_head, by_token;     // items of a head, of a token
+};
+struct RopeParams {
+  RopeTensor t[3];
+  const double* freqs;
+  const int32_t* pos32; const int64_t* pos64; const int32_t* lens;       // at most one of them
+  int64_t pos_b, pos_s, start;
+  int n_tokens, seqlen, tokens_per_group, n_half, head_vecs, room;
+  float scale, sign;         // of the angle: -1 turns back
+  Div by_seq;
+};
+
+__device__ __forceinline__ int64_t rope_position(const RopeParams& p, int b, int s) {
+  if (p.pos64) return p.pos64[b * p.pos_b + s * p.pos_s];
+  if (p.pos32) return p.pos32[b * p.pos_b + s * p.pos_s];
+  if (p.lens) return (int64_t)p.lens[b] - p.seqlen + s;
+  return p.start + s;
+}
+
+// cos and sin of position * freq.  The angle in turns is a product in twice 64 bits, of which only the part behind the point is
+// used: far positions lose nothing (position 2^31 with one rounding in 64 bits is 5e-7 off, as much as a cosine in 32 bits has).
+__device__ __forceinline__ void rope_angle(int64_t pos, double freq, float& c, float& s) {
+#pragma clang fp contract(off)         // (turns - rint(turns) as one fma would count `rest` twice)
+  constexpr double kHi = 0.15915494309189535, kLo = -9.839338337591e-18;       // 1 / (2 pi) = kHi + kLo
+  const double f = freq * kHi, f_lo = fma(freq, kHi, -f) + freq * kLo;
+  const double p = (double)pos, turns = p * f, rest = fma(p, f, -turns) + p * f_lo;
+  const float half_turns = 2.f * (float)((turns - rint(turns)) + rest);
+  sincospif(half_turns, &s, &c);
+}
+
+template <class T, int kV> __device__ __forceinline__ void rope_load(T (&d)[kV], const T* p) {
+  typedef __attribute__((ext_vector_type(kV))) T vec;
+  if constexpr (kV == 1) d[0] = *p;
+  else {
+    const vec x = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int j = 0; j < kV; ++j) d[j] = x[j];
+  }
+}
+template <class T, int kV> __device__ __forceinline__ void rope_store(T* p, const T (&d)[kV]) {
+  typedef __attribute__((ext_vector_type(kV))) T vec;
+  if constexpr (kV == 1) *p = d[0];
+  else {
+    vec x;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) x[j] = d[j];
+    *reinterpret_cast<vec*>(p) = x;
+  }
+}
+
+// kV elements a vector: the most that sizes, strides and pointers allow, up to 16 bytes.  A workgroup goes through the tensors one after the
+// other, or, where there are few tokens, takes one of them (blockIdx.y): which one is then a scalar either way.
+template <class T, int kV, bool kInterleaved>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) {
+  __shared__ __attribute__((aligned(16))) float cosine[kRopeAngles], sine[kRopeAngles];
+  __shared__ int64_t position[kRopeMaxTokens];
+  const int first = blockIdx.x * p.tokens_per_group, n_here = min(p.tokens_per_group, p.n_tokens - first);
+  const int begin = gridDim.y > 1 ? blockIdx.y : 0, end = gridDim.y > 1 ? begin + 1 : 3;
+  bool made = false;
+  for (int which = begin; which < end; ++which) {
+    const RopeTensor& x = p.t[which];
+    const int n = n_here * x.items, n_turned = x.rotate ? p.n_half / kV : 0;
+    for (int i0 = 0; i0 < n; i0 += kRopeThreads * kRopeAhead) {
+      T a[kRopeAhead][kV], b2[kRopeAhead][kV];
+      T* to[kRopeAhead];
+      int token[kRopeAhead], angle[kRopeAhead], second[kRopeAhead];    // first angle, -1: passes through; elements to the second vector, 0: none
+#pragma unroll
+      for (int u = 0; u < kRopeAhead; ++u) {
+        const int i = i0 + u * kRopeThreads + threadIdx.x;
+        to[u] = nullptr;
+        if (i >= n) continue;
+        const int t = quotient(i, x.by_token), r = i - t * x.items, h = quotient(r, x.by_head), item = r - h * x.by_head.d;
+        const int b = quotient(first + t, p.by_seq), s = first + t - b * p.seqlen;
+        int at;                                           // the first vector, in vectors
+        if (item < n_turned) {
+          angle[u] = t * p.n_half + item * kV;
+          at = kInterleaved ? 2 * item : item;
+          second[u] = kInterleaved ? kV : p.n_half;
+        } else {
+          angle[u] = -1;
+          at = 2 * item;                                  // (2 * n_turned vectors are turned)
+          second[u] = at + 1 < p.head_vecs ? kV : 0;
+        }
+        token[u] = t;
+        const T* from = static_cast<const T*>(x.x) + b * x.xs.b + s * x.xs.s + h * x.xs.h + at * kV;
+        to[u] = static_cast<T*>(x.y) + b * x.ys.b + (x.cached ? 0 : s * x.ys.s) + h * x.ys.h + at * kV;
+        rope_load<T, kV>(a[u], from);
+        if (second[u]) rope_load<T, kV>(b2[u], from + second[u]);
+      }
+      if (!made) {                                        // workgroup-uniform; the first loads are on their way meanwhile
+        made = true;
+        for (int i = threadIdx.x; i < n_here * p.n_half; i += kRopeThreads) {
+          const int t = i / p.n_half, b = quotient(first + t, p.by_seq), s = first + t - b * p.seqlen;
+          float c, sn;
+          rope_angle(rope_position(p, b, s), p.freqs[i - t * p.n_half], c, sn);
+          cosine[i] = c * p.scale;
+          sine[i] = sn * p.scale * p.sign;
+        }
+        if (threadIdx.x < n_here) {
+          const int b = quotient(first + threadIdx.x, p.by_seq);
+          position[threadIdx.x] = rope_position(p, b, first + threadIdx.x - b * p.seqlen);
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int u = 0; u < kRopeAhead; ++u) {
+        if (!to[u]) continue;
+        if (x.cached) {
+          const int64_t row = position[token[u]];
+          if (row < 0 || row >= p.room) continue;
+          to[u] += row * x.ys.s;
+        }
+        if (angle[u] >= 0) {
+          // entries 0 .. 2 kV - 1 of the two vectors; pair j is (j, kV + j), or (2j, 2j + 1)
+          float f[2 * kV];
+#pragma unroll
+          for (int j = 0; j < kV; ++j) { f[j] = (float)a[u][j]; f[kV + j] = (float)b2[u][j]; }
+#pragma unroll
+          for (int j = 0; j < kV; ++j) {
+            const int lo = kInterleaved ? 2 * j : j, hi = kInterleaved ? 2 * j + 1 : kV + j;
+            const float c = cosine[angle[u] + j], s = sine[angle[u] + j], g = f[lo], e = f[hi];
+            f[lo] = g * c - e * s;
+            f[hi] = e * c + g * s;
+          }
+#pragma unroll
+          for (int j = 0; j < kV; ++j) { a[u][j] = (T)f[j]; b2[u][j] = (T)f[kV + j]; }
+        }
+        rope_store<T, kV>(to[u], a[u]);
+        if (second[u]) rope_store<T, kV>(to[u] + second[u], b2[u]);
+      }
+    }
+  }
+}
+
+template <class T, int kV>
+static void rope_launch(const RopeParams& p, bool interleaved, dim3 groups, hipStream_t st) {
+  if (interleaved) rope_kernel<T, kV, true><<<groups, kRopeThreads, 0, st>>>(p);
+  else             rope_kernel<T, kV, false><<<groups, kRopeThreads, 0, st>>>(p);
+}
+
+struct RopeShape { int batch, seqlen, head_dim, rotary_dim, dtype; };
+
+// The widest vector (in elements) that the layout allows.
+static int rope_vector(const RopeShape& s, const RopeTensor* t, const int* heads, int n) {
+  const int size = s.dtype == UA_FP32 ? 4 : 2;
+  for (int v = 16 / size; v > 1; v /= 2) {
+    bool ok = s.rotary_dim / 2 % v == 0 && s.head_dim % v == 0;
+    for (int i = 0; i < n && ok; ++i) {
+      if (!heads[i]) continue;
+      const int64_t all[6] = {t[i].xs.b, t[i].xs.s, t[i].xs.h, t[i].ys.b, t[i].ys.s, t[i].ys.h};
+      for (const int64_t x : all) ok = ok && x % v == 0;
+      ok = ok && reinterpret_cast<uintptr_t>(t[i].x) % (v * size) == 0 && reinterpret_cast<uintptr_t>(t[i].y) % (v * size) == 0;
+    }
+    if (ok) return v;
+  }
+  return 1;
+}
+
+static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_tensors, int interleaved, hipStream_t st) {
+  const int v = rope_vector(s, p.t, heads, n_tensors);
+  p.n_half = s.rotary_dim / 2;
+  p.head_vecs = s.head_dim / v;
+  p.seqlen = s.seqlen;
+  int64_t n_items = 0;
+  for (int i = 0; i < 3; ++i) {
+    RopeTensor& t = p.t[i];
+    if (i >= n_tensors || !heads[i]) { t.items = 0; t.by_head = t.by_token = make_div(1); continue; }
+    const int turned = t.rotate ? p.n_half / v : 0, rest = p.head_vecs - 2 * turned;
+    const bool in_place = t.rotate && !t.cached && t.x == t.y && t.xs.b == t.ys.b && t.xs.s == t.ys.s && t.xs.h == t.ys.h;   // what passes through is there already
+    const int per_head = turned + (in_place ? 0 : (rest + 1) / 2);
+    if ((int64_t)per_head * heads[i] * kRopeMaxTokens > INT32_MAX) return UA_ERR_SHAPE;
+    t.items = per_head * heads[i];
+    t.by_head = make_div(per_head);
+    t.by_token = make_div(t.items);
+    n_items += t.items;
+  }
+  if ((int64_t)s.batch * s.seqlen > INT32_MAX) return UA_ERR_SHAPE;
+  p.n_tokens = s.batch * s.seqlen;
+  if (p.n_tokens == 0 || n_items == 0) return UA_OK;
+  p.by_seq = make_div(s.seqlen);
+  // Tokens of a workgroup: as many as give each thread an angle, while that leaves four workgroups a CU.
+  p.tokens_per_group = std::max(1, std::min({kRopeAngles / p.n_half, kRopeMaxTokens, (kRopeThreads + p.n_half - 1) / p.n_half, p.n_tokens / (4 * kCus)}));
+  const int lines = (p.n_tokens + p.tokens_per_group - 1) / p.tokens_per_group;
+  const dim3 groups(lines, lines <= 4 * kCus ? n_tensors : 1);
+  const int rc = check_device();
+  if (rc != UA_OK) return rc;
+  if (s.dtype == UA_FP32) {
+    if (v == 4) rope_launch<float, 4>(p, interleaved, groups, st);
+    else if (v == 2) rope_launch<float, 2>(p, interleaved, groups, st);
+    else rope_launch<float, 1>(p, interleaved, groups, st);
+  } else if (s.dtype == UA_FP16) {
+    if (v == 8) rope_launch<fp16, 8>(p, interleaved, groups, st);
+    else if (v == 4) rope_launch<fp16, 4>(p, interleaved, groups, st);
+    else if (v == 2) rope_launch<fp16, 2>(p, interleaved, groups, st);
+    else rope_launch<fp16, 1>(p, interleaved, groups, st);
+  } else {
+    if (v == 8) rope_launch<bf16, 8>(p, interleaved, groups, st);
+    else if (v == 4) rope_launch<bf16, 4>(p, interleaved, groups, st);
+    else if (v == 2) rope_launch<bf16, 2>(p, interleaved, groups, st);
+    else rope_launch<bf16, 1>(p, interleaved, groups, st);
+  }
+  return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
+}
+
+static int rope_check(const RopeShape& s, int n_heads, int n_kv_heads, float scale) {
+  if (s.batch < 0 || s.seqlen < 0 || n_heads < 0 || n_kv_heads < 0 || s.head_dim <= 0) return UA_ERR_SHAPE;
+  if (s.rotary_dim <= 0 || s.rotary_dim % 2 || s.rotary_dim > s.head_dim) return UA_ERR_SHAPE;
+  if (s.head_dim > UA_ROPE_MAX_DIM || s.dtype < UA_BF16 || s.dtype > UA_FP32 || !(scale > 0.f)) return UA_ERR_UNSUPPORTED;
+  return UA_OK;
+}
+static_assert(UA_ROPE_MAX_DIM / 2 <= kRopeAngles, "the angles of one token fit");
+static Strides3 strides_of(const int64_t* s) { return {s[0], s[1], s[2]}; }
+
+}  // namespace ua
+
+extern "C" int ua_rope(const void* q, const void* k, void* q_out, void* k_out, const double* freqs, const void* positions, int positions_64,
+                       int64_t position_stride_b, int64_t position_stride_s, int64_t start, int batch, int seqlen, int n_heads, int n_kv_heads,
+                       int head_dim, int rotary_dim, int dtype, int interleaved, int inverse, float scale, const int64_t* q_strides,
+                       const int64_t* k_strides, const int64_t* q_out_strides, const int64_t* k_out_strides, void* stream) {
+  using namespace ua;
+  const RopeShape s{batch, seqlen, head_dim, rotary_dim, dtype};
+  const int rc = rope_check(s, n_heads, n_kv_heads, scale);
+  if (rc != UA_OK) return rc;
+  if ((int64_t)batch * seqlen == 0) return UA_OK;
+  if (!freqs || (n_heads && (!q || !q_out || !q_strides || !q_out_strides)) || (n_kv_heads && (!k || !k_out || !k_strides || !k_out_strides)))
+    return UA_ERR_NULL;
+  RopeParams p{};
+  const int heads[2] = {n_heads, n_kv_heads};
+  if (n_heads) { p.t[0] = {q, q_out, strides_of(q_strides), strides_of(q_out_strides), 1, 0, 0, {}, {}}; }
+  if (n_kv_heads) { p.t[1] = {k, k_out, strides_of(k_strides), strides_of(k_out_strides), 1, 0, 0, {}, {}}; }
+  p.freqs = freqs;
+  p.pos64 = positions_64 ? (const int64_t*)positions : nullptr;
+  p.pos32 = positions_64 ? nullptr : (const int32_t*)positions;
+  p.pos_b = position_stride_b; p.pos_s = position_stride_s;
+  p.start = start;
+  p.scale = scale;
+  p.sign = inverse ? -1.f : 1.f;
+  return rope_run(p, s, heads, 2, interleaved, (hipStream_t)stream);
+}
+
+extern "C" int ua_rope_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void* v_cache, const double* freqs,
+                              const int32_t* lens, int batch, int n_new, int n_heads, int n_kv_heads, int room, int head_dim, int rotary_dim,
+                              int dtype, int interleaved, float scale, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                              const int64_t* q_out_strides, const int64_t* k_cache_strides, const int64_t* v_cache_strides, void* stream) {
+  using namespace ua;
+  const RopeShape s{batch, n_new, head_dim, rotary_dim, dtype};
+  const int rc = rope_check(s, n_heads, n_kv_heads, scale);
+  if (rc != UA_OK) return rc;
+  if (room < 0) return UA_ERR_SHAPE;
+  if ((int64_t)batch * n_new == 0) return UA_OK;
+  if (room == 0) n_kv_heads = 0;                     // (no row to write: the cache may be NULL)
+  if (!freqs || !lens || (n_heads && (!q || !q_out || !q_strides || !q_out_strides)) ||
+      (n_kv_heads && (!k || !v || !k_cache || !v_cache || !k_strides || !v_strides || !k_cache_strides || !v_cache_strides)))
+    return UA_ERR_NULL;
+  RopeParams p{};
+  const int heads[3] = {n_heads, n_kv_heads, n_kv_heads};
+  if (n_heads) p.t[0] = {q, q_out, strides_of(q_strides), strides_of(q_out_strides), 1, 0, 0, {}, {}};
+  if (n_kv_heads) {
+    p.t[1] = {k, k_cache, strides_of(k_strides), strides_of(k_cache_strides), 1, 1, 0, {}, {}};
+    p.t[2] = {v, v_cache, strides_of(v_strides), strides_of(v_cache_strides), 0, 1, 0, {}, {}};
+  }
+  p.freqs = freqs;
+  p.lens = lens;
+  p.room = room;
+  p.scale = scale;
+  p.sign = 1.f;
+  return rope_run(p, s, heads, 3, interleaved, (hipStream_t)stream);
+}
