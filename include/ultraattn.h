@@ -68,8 +68,8 @@ extern "C" {
 
 /* 100 * major + minor.  102: `nnz` argument of the attention entry points, ua_merge_update, the
  * no-allocation builder, `work` of ua_tilelist_build_device grown to n_qtiles + n_ktiles + 7.  104: ua_bsa_bwd.
- * 105: ua_tilelist_build_device_scratch.  106: ua_copy_in.  107: ua_rope, ua_rope_append.  */
-#define UA_VERSION 107
+ * 105: ua_tilelist_build_device_scratch.  106: ua_copy_in.  107: ua_rope, ua_rope_append.  108: ua_swa_*.  */
+#define UA_VERSION 108
 int ua_version(void);
 const char *ua_strerror(int rc);
 
@@ -332,6 +332,28 @@ int ua_rope_append(const void *q, const void *k, const void *v, void *q_out, voi
                    int dtype, int interleaved, float scale,
                    const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides,
                    const int64_t *q_out_strides, const int64_t *k_cache_strides, const int64_t *v_cache_strides, void *stream);
+
+/* ---- sliding-window attention with sinks -----------------------------------------------------------
+ * No counterpart in the reference, whose tile kernel is called with window_size = (-1, -1) (search_algo/benchmark.py:365-366).
+ * Query i is at position q_start + i, key j at k_start + j.  The query sees the key iff
+ *     (right < 0  or  k_start + j <= q_start + i + right)  and  (left < 0  or  k_start + j >= q_start + i - left  or  k_start + j < sinks):
+ * a window of `left` keys before and `right` behind its own position, and the sequence's first `sinks` keys.  Both starts place
+ * shards: the chunk of keys that another rank holds, or queries that follow a cached prefix (q_start = k_start + seqlen_k - seqlen_q).
+ * q, o [batch, seqlen_q, n_heads, head_dim]; k, v [batch, seqlen_k, n_kv_heads, head_dim]: key head h serves query heads
+ * h * n_heads / n_kv_heads ...  Any lengths (0 too, up to 2^28), head_dim 64 or 128, dtype UA_BF16 or UA_FP16; pointers 16-byte
+ * aligned, element strides multiples of 8 (inputs may have strides of 0: broadcast).  lse [batch, n_heads, seqlen_q] fp32, contiguous, natural log: rows
+ * that see no key get o = 0, lse = -inf, and ua_merge / ua_merge_update join shards.  Scores, statistics and sums are 32 bits; P is rounded
+ * to dtype for its product with V, as it is in ua_bsa_fwd.
+ * Few long walks are cut into parts, whose fp32 results are merged in a second launch, if `workspace` (16-byte aligned,
+ * overwritten) holds ua_swa_workspace_bytes(); calls that overlap in time need one each.  With less nothing is cut.
+ * A key's or value's NaN or infinity reaches rows that see it, and may reach rows whose tile of 128 sees it. */
+int64_t ua_swa_workspace_bytes(int batch, int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim,
+                               int64_t q_start, int64_t k_start, int64_t left, int64_t right, int64_t sinks);
+int ua_swa_fwd(const void *q, const void *k, const void *v, void *o, float *lse,
+               int batch, int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim, int dtype,
+               const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides, const int64_t *o_strides,
+               int64_t q_start, int64_t k_start, int64_t left, int64_t right, int64_t sinks, float softmax_scale,
+               void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

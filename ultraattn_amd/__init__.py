@@ -10,6 +10,9 @@ def __getattr__(name):
     if name in ("bsa_fwd", "bsa_bwd", "merge_partials", "softmax_delta", "update_out_and_lse", "grad_accumulate", "grad_sum"):
         from . import ops
         return getattr(ops, name)
+    if name in ("swa_fwd", "swa_bwd", "swa_decode"):
+        from . import window
+        return getattr(window, name)
     if name in ("rope_freqs", "rope_fwd", "rope_bwd", "rope_append"):
         from . import rope
         return getattr(rope, name)

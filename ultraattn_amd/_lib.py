@@ -40,6 +40,8 @@ SIGNATURES = {
     "ua_cols_scatter": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p]),
     "ua_rope": (c_int, [c_void_p] * 6 + [c_int] + [c_int64] * 3 + [c_int] * 9 + [c_float] + [_i64p] * 4 + [c_void_p]),
     "ua_rope_append": (c_int, [c_void_p] * 8 + [c_int] * 9 + [c_float] + [_i64p] * 6 + [c_void_p]),
+    "ua_swa_workspace_bytes": (c_int64, [c_int] * 6 + [c_int64] * 5),
+    "ua_swa_fwd": (c_int, [c_void_p] * 5 + [c_int] * 7 + [_i64p] * 4 + [c_int64] * 5 + [c_float, c_void_p, c_int64, c_void_p]),
     "ua_copy_in": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }
 

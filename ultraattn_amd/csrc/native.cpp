@@ -782,6 +782,65 @@ PyObject* rope_append(PyObject* const* a) {
   return qo.wrap();
 }
 
+// ---- sliding-window attention ---------------------------------------------------------------------------------
+// Strides of a tensor some of whose axes have one element or none (torch leaves any stride there).
+Strides used_strides(const at::Tensor& t) {
+  auto of = [&](int i) { return t.size(i) > 1 ? t.stride(i) : kDim; };
+  return Strides(of(0), of(1), of(2));
+}
+void check_swa(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const char* k_name, const char* v_name) {
+  dtype_code("q", q, false);
+  check_rows4("q", q, q);
+  check_rows4(k_name, k, q);
+  check_rows4(v_name, v, q);
+  if (q.size(3) != 64 && q.size(3) != 128) fail(PyExc_ValueError, "head_dim must be 64 or 128, got " + std::to_string(q.size(3)));
+  check_shape(k_name, k, {q.size(0), k.size(1), k.size(2), q.size(3)});
+  check_shape(v_name, v, k.sizes());
+  if (q.size(2) < 1 || k.size(2) < 1 || q.size(2) % k.size(2))
+    fail(PyExc_ValueError, std::to_string(q.size(2)) + " query heads cannot share " + std::to_string(k.size(2)) + " key heads evenly");
+}
+void check_lse(const char* name, const at::Tensor& t, const at::Tensor& rows) {
+  check_stat(name, t, rows);
+  if (t.device() != rows.device()) fail(PyExc_ValueError, std::string(name) + " is on another device than the first tensor");
+}
+// What a call says of positions: window left and right, sinks, q_start (None: the last query is at the last key) and k_start.
+struct Window {
+  int64_t left, right, sinks, q_start, k_start;
+  Window(PyObject* const* a, int64_t seq_q, int64_t seq_k) : left(integer(a[0])), right(integer(a[1])), sinks(integer(a[2])), k_start(integer(a[4])) {
+    constexpr int64_t kMost = int64_t(1) << 60;
+    if (left < -1 || right < -1 || left > kMost || right > kMost) fail(PyExc_ValueError, "window sizes must be -1 (no bound) or a number of keys");
+    if (sinks < 0 || sinks > kMost) fail(PyExc_ValueError, "sinks must be a number of keys");
+    q_start = a[3] == Py_None ? k_start + seq_k - seq_q : integer(a[3]);
+    if (q_start > kMost || q_start < -kMost || k_start > kMost || k_start < -kMost) fail(PyExc_ValueError, "q_start and k_start must be positions");
+  }
+};
+float swa_scale(PyObject* o, int64_t dim) { return o == Py_None ? (float)(1.0 / std::sqrt((double)dim)) : positive(o, "softmax_scale"); }
+at::Tensor scratch(int64_t bytes, const at::Tensor& like) { return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor(); }
+
+// swa_forward(q, k, v, left, right, sinks, q_start, k_start, softmax_scale, out, lse) -> (out, lse)
+// (The workspace of a cut call is its own: taken from the allocator in stream order, so that calls on other streams and captured graphs
+// never share one.)
+PyObject* swa_forward(PyObject* const* a) {
+  const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v");
+  check_swa(q, k, v, "k", "v");
+  const Window w(a + 3, q.size(1), k.size(1));
+  const float scale = swa_scale(a[8], q.size(3));
+  const int dt = dtype_code("q", q, false);
+  Slot out(a[9]), lse(a[10]);
+  result(out, "out", q);
+  if (lse.given) check_lse("lse", lse.t = tensor(lse.given, "lse"), q);
+  else lse.t = stat_of(q);
+  const On on(q);
+  const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), sq = (int)q.size(1), sk = (int)k.size(1), D = (int)q.size(3);
+  const at::Tensor ws = scratch(ua_swa_workspace_bytes(B, H, Hk, sq, sk, D, w.q_start, w.k_start, w.left, w.right, w.sinks), q);
+  call("ua_swa_fwd", [&] {
+    return ua_swa_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.t.data_ptr(), (float*)lse.t.data_ptr(), B, H, Hk, sq, sk, D, dt,
+                      used_strides(q), used_strides(k), used_strides(v), used_strides(out.t), w.q_start, w.k_start, w.left, w.right, w.sinks, scale,
+                      ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, on.stream);
+  });
+  return tuple_of(out, lse);
+}
+
 // ---- module ---------------------------------------------------------------------------------------------
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -807,7 +866,7 @@ PyMethodDef methods[] = {
     UA_METHOD(dense_forward, 8), UA_METHOD(dense_backward, 14), UA_METHOD(bsa_forward, 10), UA_METHOD(bsa_backward, 15),
     UA_METHOD(delta, 3), UA_METHOD(grad_accumulate, 4), UA_METHOD(merge, 4), UA_METHOD(grad_sum, 3),
     UA_METHOD(merge_update, 5), UA_METHOD(permute_cols, 6), UA_METHOD(lists_from_mask, 5),
-    UA_METHOD(build_lists_device, 3), UA_METHOD(rope, 10), UA_METHOD(rope_append, 10), {nullptr, nullptr, 0, nullptr}};
+    UA_METHOD(build_lists_device, 3), UA_METHOD(rope, 10), UA_METHOD(rope_append, 10), UA_METHOD(swa_forward, 11), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "Native host side of the attention operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,329 @@
+// Sliding-window attention with sinks, forward.
+//
+// One workgroup (4 waves of 32 query rows) per (128 rows, head) walks the 64-key blocks that its rows see (SwaWalk): the sinks' blocks, then the
+// window's.  Transposed products, as in the block-sparse forward: S^T = K Q^T, O^T += V^T P^T, so that a lane holds one query's column and
+// exp2(S^T), rounded, is the next product's B operand.  Only blocks at the window's edges compare positions; blocks that a wave's 32 rows do not see
+// are skipped by it.  K and V come in through two LDS stages, the next block's copies between this one's matrix instructions.
+//
+// The running maximum is raised only where a block's sums show a score far above it, or where a row has not seen a key yet.
+#include <algorithm>
+#include "swa.h"
+
+namespace ua {
+
+// Sums of a lane's 32 exponentials from which the reference is raised.  fp16 holds P up to 65504.
+template <class T> struct SwaRaise;
+template <> struct SwaRaise<bf16> { static constexpr float kSum = 16777216.f; };
+template <> struct SwaRaise<fp16> { static constexpr float kSum = 1024.f; };
+
+template <class T, int kD>
+__global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
+  using H = SwaHead<kD>;
+  using V = SwaVec<T>;
+  typedef typename V::x8 x8;
+  __shared__ __attribute__((aligned(1024))) unsigned char stage_a[2 * H::kTile];
+  __shared__ __attribute__((aligned(1024))) unsigned char stage_b[2 * H::kTile];
+  const uint32_t lds[2] = {(uint32_t)(uintptr_t)(lds_byte*)stage_a, (uint32_t)(uintptr_t)(lds_byte*)stage_b};
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int pos, bh;
+  map_block(blockIdx.x, p.map, pos, bh);
+  const int line = quotient(pos, p.by_parts), part = pos - line * p.n_parts;
+  const int qt = p.n_qtiles - 1 - line;                   // (the longest walks of a causal window first)
+  const int b = quotient(bh, p.by_heads), h = bh - b * p.n_heads, hk = quotient(h, p.by_group);
+  const int r0 = qt * kSwaRows, row0 = r0 + 32 * wave, n_rows = p.seq_q - row0;      // rows of this wave that exist (may be <= 0)
+
+  const SwaWalk walk(r0, min(r0 + kSwaRows, p.seq_q) - 1, p.hi, p.lo, p.sinks, p.seq_k);
+  const int part_len = (walk.n + p.n_parts - 1) / p.n_parts, i0 = min(part * part_len, walk.n), i1 = min(i0 + part_len, walk.n);
+  SwaStream<kD, false, true> in((const T*)p.k + b * p.ks.b + hk * p.ks.h, p.ks.s, (const T*)p.v + b * p.vs.b + hk * p.vs.h, p.vs.s, wave, lane);
+  if (i0 < i1) {
+    in.block(walk.at(i0) * kSwaBlock, p.seq_k, true);
+#pragma unroll
+    for (int n = 0; n < in.kPieces; ++n) in.copy(n, lds[0]);
+  }
+  x8 qf[H::kSteps];
+  {
+    u32x4 raw[H::kSteps];
+    const int first = min(row0, p.seq_q - 1);
+    swa_load_rows<kD>(raw, (const T*)p.q + b * p.qs.b + first * p.qs.s + h * p.qs.h, p.qs.s, p.seq_q - first);
+    const uint32_t turn = lds[1] + wave * 32 * H::kRow;   // the stage that the first step fills
+    swa_put_rows<kD>(raw, turn);
+    swa_frags<T, kD>(qf, turn);
+#pragma unroll
+    for (int i = 0; i < H::kSteps; ++i) asm volatile("" : "+v"(qf[i]));      // read before the walk
+  }
+  f32x16 o[H::kBlocks];
+#pragma unroll
+  for (int m = 0; m < H::kBlocks; ++m) o[m] = f32x16{0};
+  float m_run = -INFINITY, m_use = 0.f, l_run = 0.f;
+  uint32_t nat[H::kSteps], tr[H::kBlocks];
+#pragma unroll
+  for (int i = 0; i < H::kSteps; ++i) nat[i] = H::at_n(lane & 31, 2 * i + (lane >> 5));
+#pragma unroll
+  for (int m = 0; m < H::kBlocks; ++m) tr[m] = H::kTile + H::tr_offset(lane, m);
+
+  auto step = [&](int i, auto stage_tag) {
+    constexpr int kStage = decltype(stage_tag)::value;
+    const uint32_t here = lds[kStage], other = lds[kStage ^ 1];
+    const int key0 = walk.at(i) * kSwaBlock;
+    in.block(walk.at(i + 1) * kSwaBlock, p.seq_k, i + 1 < i1);
+    wait_vmem_all();
+    __syncthreads();                        // this block has landed, and everyone has left the other stage
+    const bool hidden = key0 > row0 + 31 + p.hi || (key0 + kSwaBlock <= row0 + p.lo && key0 >= p.sinks);
+    if (hidden) {
+#pragma unroll
+      for (int n = 0; n < in.kPieces; ++n) in.copy(n, other);
+      return;
+    }
+    // S^T: two blocks of 32 keys in turn
+    f32x16 s[2] = {f32x16{0}, f32x16{0}};
+    {
+      constexpr int kAhead = 4, kAll = 2 * H::kSteps;
+      x8 kf[kAll];
+      auto rd = [&](int n) { return lds_get<x8>(here + nat[n >> 1] + 32 * H::kRow * (n & 1)); };
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) kf[n] = rd(n);
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+      for (int n = 0; n < kAll; ++n) {
+        if (n + kAhead < kAll) kf[n + kAhead] = rd(n + kAhead);
+        s[n & 1] = V::mfma(kf[n], qf[n >> 1], s[n & 1]);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (n & 1) in.copy(n >> 1, other);
+      }
+      static_assert(kAll / 2 == SwaStream<kD, false, true>::kPieces, "a copy after every other product");
+    }
+    const bool whole = key0 + kSwaBlock - 1 <= min(row0 + p.hi, p.seq_k - 1) && (key0 >= row0 + 31 + p.lo || key0 + kSwaBlock <= p.sinks);
+    if (!whole) {
+      const int lane_now = fresh_lane(), row = row0 + (lane_now & 31), last = min(row + p.hi, p.seq_k - 1), first = row + p.lo;
+      const uint32_t seen = (uint32_t)max(last - first + 1, 0);
+      const int sinks = min(p.sinks, last + 1), key = key0 + 4 * (lane_now >> 5);
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int k = key + 32 * mb + 8 * (j >> 2) + (j & 3);
+          if ((uint32_t)(k - first) >= seen && k >= sinks) s[mb][j] = -INFINITY;
+        }
+    }
+    constexpr int kVAhead = 3, kVAll = 4 * H::kBlocks;
+    x8 vf[4];
+    auto rd_v = [&](int n) {                // fragment n % kBlocks of 16 keys
+      const uint32_t at = here + tr[n % H::kBlocks] + 16 * H::kRow * (n / H::kBlocks);
+      return lds_tr_pair<T>(at, at + 8 * H::kRow);
+    };
+#pragma unroll
+    for (int n = 0; n < kVAhead; ++n) vf[n] = rd_v(n);
+    float rs = 0.f;
+    x8 pf[4];
+    auto exponentials = [&]() {
+      rs = 0.f;
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float e = fast_exp2(fmaf(s[mb][j], p.scale_log2, -m_use));
+          rs += e;
+          pf[2 * mb + (j >> 3)][j & 7] = (T)e;
+        }
+    };
+    exponentials();
+    if (__builtin_amdgcn_ballot_w64(!(rs < SwaRaise<T>::kSum) || m_run == -INFINITY) != 0) {        // wave-uniform, rare
+      float mx = s[0][0], a, c;
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[mb][j]);
+      swap_lanes<32>(mx, a, c);
+      const float m_new = fmaxf(m_run, fmaxf(a, c) * p.scale_log2);
+      m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = m_new == m_run ? 1.f : fast_exp2(m_run - m_use);      // m_run = -inf -> 0
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int m = 0; m < H::kBlocks; ++m)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[m][j] *= alpha;
+      exponentials();
+    }
+    l_run += rs;
+#pragma unroll
+    for (int n = 0; n < kVAll; ++n) {
+      if (n + kVAhead < kVAll) vf[(n + kVAhead) & 3] = rd_v(n + kVAhead);
+      o[n % H::kBlocks] = V::mfma(vf[n & 3], pf[n / H::kBlocks], o[n % H::kBlocks]);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+  };
+  for (int i = i0; i < i1; i += 2) {
+    step(i, std::integral_constant<int, 0>{});
+    if (i + 1 < i1) step(i + 1, std::integral_constant<int, 1>{});
+  }
+  wait_vmem_all();                          // the last step's copies filled a stage with zeros
+  __syncthreads();
+  if (n_rows <= 0) return;
+  float a, c;
+  swap_lanes<32>(l_run, a, c);
+  const float l = a + c, inv = l > 0.f || l != l ? 1.f / l : 0.f;      // (NaN stays)
+  const float lse = l > 0.f || l != l ? (m_run + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+  const int out_lane = fresh_lane();
+  if (p.n_parts > 1) {
+    const int64_t row = ((int64_t)bh * p.seq_q + row0);
+    swa_store_f32<kD>(p.part_o + part * p.o_part + row * kD, kD, n_rows, o, inv);
+    if (out_lane < min(n_rows, 32)) p.part_lse[part * p.lse_part + row + out_lane] = lse;
+  } else {
+    swa_store_rows<T, kD>((T*)p.o + b * p.os.b + (int64_t)row0 * p.os.s + h * p.os.h, p.os.s, n_rows, o, inv, lds[0] + wave * 32 * H::kRow);
+    if (out_lane < min(n_rows, 32)) p.lse[(int64_t)bh * p.seq_q + row0 + out_lane] = lse;
+  }
+}
+
+// Partial rows of fp32 and their lse, part i of row (b, h, s) at part_o + i * o_part + row * kD:
+//   LSE = log sum_p exp(lse_p),  O = sum_p exp(lse_p - LSE) O_p.
+// Four rows a wave, 16 lanes on a row; bound by the launch and the caches, the partials having just been written.
+template <class T, int kD>
+__global__ __launch_bounds__(256) void merge_rows_kernel(const float* part_o, int64_t o_part, const float* part_lse, int64_t lse_part, int n_parts,
+                                                         T* o, Strides3 os, float* lse, int n_rows, int n_heads, int seq, Div by_seq, Div by_heads) {
+  constexpr int kPer = kD / 16;
+  const int row = blockIdx.x * 16 + (threadIdx.x >> 4), c = threadIdx.x & 15;
+  if (row >= n_rows) return;
+  float top = -INFINITY;
+  for (int i = 0; i < n_parts; ++i) top = fmaxf(top, part_lse[i * lse_part + row]);
+  const float at = top == -INFINITY ? 0.f : top;
+  float total = 0.f, acc[kPer] = {};
+  for (int i = 0; i < n_parts; ++i) {
+    const float l = part_lse[i * lse_part + row];
+    if (l == -INFINITY) continue;                        // (such a part left no row)
+    const float w = fast_exp2((l - at) * kLog2e);
+    total += w;
+    const float* x = part_o + i * o_part + (int64_t)row * kD + c * kPer;
+#pragma unroll
+    for (int j = 0; j < kPer; j += 4) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(x + j);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) acc[j + n] += w * y[n];
+    }
+  }
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  const int bh = quotient(row, by_seq), s = row - bh * seq, b = quotient(bh, by_heads), h = bh - b * n_heads;
+  T* out = o + b * os.b + (int64_t)s * os.s + h * os.h + c * kPer;
+  typedef __attribute__((ext_vector_type(kPer))) T vec;
+  vec w;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) w[j] = (T)(acc[j] * inv);
+  *reinterpret_cast<vec*>(out) = w;
+  if (c == 0) lse[row] = total > 0.f || total != total ? at + __builtin_amdgcn_logf(total) * kLn2 : -INFINITY;
+}
+
+int swa_merge(const float* part_o, int64_t o_part, const float* part_lse, int64_t lse_part, int n_parts, void* o, const Strides3& os, float* lse,
+              int batch, int n_heads, int seq, int head_dim, int dtype, hipStream_t st) {
+  const int n_rows = batch * n_heads * seq, groups = (n_rows + 15) / 16;
+  auto run = [&](auto kernel, auto* out) {
+    kernel<<<groups, 256, 0, st>>>(part_o, o_part, part_lse, lse_part, n_parts, out, os, lse, n_rows, n_heads, seq, make_div(seq), make_div(n_heads));
+  };
+  if (dtype == UA_FP16) head_dim == 64 ? run(merge_rows_kernel<fp16, 64>, (fp16*)o) : run(merge_rows_kernel<fp16, 128>, (fp16*)o);
+  else                  head_dim == 64 ? run(merge_rows_kernel<bf16, 64>, (bf16*)o) : run(merge_rows_kernel<bf16, 128>, (bf16*)o);
+  return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
+}
+
+bool swa_strides_ok(const int64_t* s, bool written) {
+  if (s[0] % 8 || s[1] % 8 || s[2] % 8 || s[0] < 0 || s[1] < 0 || s[2] < 0) return false;
+  return !written || (s[1] > 0 && s[2] > 0);
+}
+
+int swa_fill(SwaParams& p, int batch, int n_heads, int n_kv_heads, int seq_q, int seq_k, int head_dim, int dtype, int64_t q_start, int64_t k_start,
+             int64_t left, int64_t right, int64_t sinks, float softmax_scale) {
+  constexpr int64_t kMost = int64_t(1) << 60;
+  if (batch < 0 || n_heads <= 0 || n_kv_heads <= 0 || seq_q < 0 || seq_k < 0 || n_heads % n_kv_heads) return UA_ERR_SHAPE;
+  if (seq_q > kSwaMaxLen || seq_k > kSwaMaxLen || (int64_t)batch * n_heads * ((seq_q + kSwaRows - 1) / kSwaRows) > INT32_MAX / UA_MAX_PARTS ||
+      (int64_t)batch * n_heads * ((seq_k + kSwaRows - 1) / kSwaRows) > INT32_MAX / UA_MAX_PARTS)
+    return UA_ERR_SHAPE;
+  if (q_start > kMost || q_start < -kMost || k_start > kMost || k_start < -kMost || left < -1 || right < -1 || left > kMost || right > kMost || sinks < 0 ||
+      sinks > kMost)
+    return UA_ERR_SHAPE;
+  if ((head_dim != 64 && head_dim != 128) || (dtype != UA_BF16 && dtype != UA_FP16) || !(softmax_scale > 0.f)) return UA_ERR_UNSUPPORTED;
+  auto clamp = [](int64_t x) { return (int)std::min<int64_t>(std::max<int64_t>(x, -kFar), kFar); };
+  p.batch = batch; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.group = n_heads / n_kv_heads; p.seq_q = seq_q; p.seq_k = seq_k;
+  p.hi = right < 0 ? kFar : clamp(q_start - k_start + right);
+  p.lo = left < 0 ? -kFar : clamp(q_start - k_start - left);
+  p.sinks = left < 0 ? 0 : (int)std::min<int64_t>(std::max<int64_t>(sinks - k_start, 0), seq_k);
+  p.scale = softmax_scale;
+  p.scale_log2 = softmax_scale * kLog2e;
+  p.n_qtiles = (seq_q + kSwaRows - 1) / kSwaRows;
+  p.n_ktiles = (seq_k + kSwaRows - 1) / kSwaRows;
+  p.n_parts = 1;
+  p.by_heads = make_div(n_heads);
+  p.by_kv_heads = make_div(n_kv_heads);
+  p.by_group = make_div(p.group);
+  return UA_OK;
+}
+
+// Blocks of 64 keys that the longest walk of a call has.
+static int64_t longest_walk(const SwaParams& p) {
+  const int64_t blocks = ((int64_t)p.seq_k + kSwaBlock - 1) / kSwaBlock;
+  const int64_t window = p.hi >= kFar || p.lo <= -kFar ? blocks : ((int64_t)p.hi - p.lo + kSwaRows + 2 * kSwaBlock - 1) / kSwaBlock + (p.sinks + kSwaBlock - 1) / kSwaBlock;
+  return std::max<int64_t>(std::min(window, blocks), 0);
+}
+// Parts that a forward's walks are cut into.
+static int fwd_parts(const SwaParams& p) {
+  const int64_t lines = (int64_t)p.batch * p.n_heads * p.n_qtiles, walk = longest_walk(p);
+  if (lines == 0 || lines >= kDenseFullLaunch || walk < 8) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({kDenseTargetGroups / lines, walk / 4, UA_MAX_PARTS}));
+}
+static int64_t part_rows(const SwaParams& p) { return (int64_t)p.batch * p.n_heads * p.seq_q; }
+
+}  // namespace ua
+
+extern "C" int64_t ua_swa_workspace_bytes(int batch, int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim, int64_t q_start,
+                                          int64_t k_start, int64_t left, int64_t right, int64_t sinks) {
+  using namespace ua;
+  SwaParams p{};
+  if (swa_fill(p, batch, n_heads, n_kv_heads, seqlen_q, seqlen_k, head_dim, UA_BF16, q_start, k_start, left, right, sinks, 1.f) != UA_OK) return 0;
+  const int parts = fwd_parts(p);
+  return parts > 1 ? parts * (align256(part_rows(p) * head_dim * 4) + align256(part_rows(p) * 4)) : 0;
+}
+
+extern "C" int ua_swa_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int batch, int n_heads, int n_kv_heads, int seqlen_q,
+                          int seqlen_k, int head_dim, int dtype, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                          const int64_t* o_strides, int64_t q_start, int64_t k_start, int64_t left, int64_t right, int64_t sinks, float softmax_scale,
+                          void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace ua;
+  SwaParams p{};
+  int rc = swa_fill(p, batch, n_heads, n_kv_heads, seqlen_q, seqlen_k, head_dim, dtype, q_start, k_start, left, right, sinks, softmax_scale);
+  if (rc != UA_OK) return rc;
+  if ((int64_t)batch * seqlen_q == 0) return UA_OK;
+  if (!q || !o || !lse || !q_strides || !o_strides || !k_strides || !v_strides || (seqlen_k > 0 && (!k || !v))) return UA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !swa_strides_ok(q_strides, false) || !swa_strides_ok(k_strides, false) ||
+      !swa_strides_ok(v_strides, false) || !swa_strides_ok(o_strides, true))
+    return UA_ERR_ALIGN;
+  if (k_strides[1] > (INT32_MAX >> 9) || v_strides[1] > (INT32_MAX >> 9)) return UA_ERR_SHAPE;
+  rc = check_device();
+  if (rc != UA_OK) return rc;
+  p.q = q; p.k = k; p.v = v; p.o = o; p.lse = lse;
+  p.qs = {q_strides[0], q_strides[1], q_strides[2]};
+  p.ks = {k_strides[0], k_strides[1], k_strides[2]};
+  p.vs = {v_strides[0], v_strides[1], v_strides[2]};
+  p.os = {o_strides[0], o_strides[1], o_strides[2]};
+  const hipStream_t st = (hipStream_t)stream;
+  const int parts = fwd_parts(p);
+  const int64_t o_bytes = align256(part_rows(p) * head_dim * 4), lse_bytes = align256(part_rows(p) * 4);
+  if (parts > 1 && workspace && aligned16(workspace) && workspace_bytes >= parts * (o_bytes + lse_bytes)) {
+    p.n_parts = parts;
+    p.part_o = (float*)workspace;
+    p.o_part = o_bytes / 4;
+    p.part_lse = (float*)((char*)workspace + parts * o_bytes);
+    p.lse_part = lse_bytes / 4;
+  }
+  p.by_parts = make_div(p.n_parts);
+  p.map = block_map(batch * n_heads, p.n_qtiles * p.n_parts);
+  const unsigned n = (unsigned)(batch * n_heads * p.n_qtiles * p.n_parts);
+  if (dtype == UA_FP16) {
+    if (head_dim == 64) swa_fwd_kernel<fp16, 64><<<n, 256, 0, st>>>(p);
+    else                swa_fwd_kernel<fp16, 128><<<n, 256, 0, st>>>(p);
+  } else {
+    if (head_dim == 64) swa_fwd_kernel<bf16, 64><<<n, 256, 0, st>>>(p);
+    else                swa_fwd_kernel<bf16, 128><<<n, 256, 0, st>>>(p);
+  }
+  if (hipGetLastError() != hipSuccess) return UA_ERR_LAUNCH;
+  if (p.n_parts == 1) return UA_OK;
+  return swa_merge(p.part_o, p.o_part, p.part_lse, p.lse_part, p.n_parts, o, p.os, lse, batch, n_heads, seqlen_q, head_dim, dtype, st);
+}

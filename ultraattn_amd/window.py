@@ -1,0 +1,25 @@
+"""Sliding-window attention with sinks on one MI355X: forward, backward, and new tokens against a cache.
+
+Host side of ``ua_swa_*`` in ``include/ultraattn.h``, beside the block-sparse operators of ``ops.py`` and in their manner: row tensors
+``[B, S, H, D]`` with any (batch, token, head) strides, ``lse`` ``[B, H, S]`` fp32 in natural logarithm, results written in place when
+given, everything on the current CUDA(HIP) stream, nothing synchronises.  Types are bf16 and fp16, D is 64 or 128, lengths are arbitrary, and keys
+may have fewer heads than queries (each serves ``Hq / Hk`` consecutive ones).
+
+Query i is at position ``q_start + i`` and key j at ``k_start + j``.  With ``window=(left, right)`` a query at p sees the keys at
+``p - left .. p + right`` (-1: no bound on that side) and, up to ``p + right``, the first ``sinks`` positions of the sequence.
+``q_start=None`` puts the last query at the last key.  A query that sees no key gets ``out = 0``, ``lse = -inf`` and no gradient, so
+results over shards of the keys (``k_start``) are joined by ``merge_partials`` / ``update_out_and_lse``.
+"""
+from typing import Optional, Tuple
+
+import torch
+
+from ._lib import native
+
+
+def swa_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Tuple[int, int] = (-1, 0), sinks: int = 0,
+            softmax_scale: Optional[float] = None, q_start: Optional[int] = None, k_start: int = 0, out: Optional[torch.Tensor] = None,
+            lse: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Forward -> (out, lse).  The default window is causal attention, aligned at the last key; ``softmax_scale`` is 1 / sqrt(D)."""
+    left, right = window
+    return native().swa_forward(q, k, v, left, right, sinks, q_start, k_start, softmax_scale, out, lse)
