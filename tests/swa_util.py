@@ -9,6 +9,7 @@ u is half a step of the type (2^-8 for bf16's 8 bits, 2^-11 for fp16's 11: `eps 
     dV       u |dV| + (u + ep + e n) sum P |dO|
     dS       P (dP - delta) with |d dP| <= (D + 4) e sum |dO| |V| and |d delta| <= sum |dO| |dO_bound| of the forward's result, which the backward is given:
              (u + ep + 4 e) |dS| + P (...); fp16: 2^-25 beside that
+    any      result in fp16 is rounded to a multiple of 2^-24 where it is below 2^-14: 2^-25 more (u |x| is less there)
     dQ, dK   u |dQ| + scale sum_j (dS's bound + n e |dS|) |K|, and alike
 """
 import math
@@ -63,7 +64,7 @@ class Reference:
         big = S.masked_fill(hide, 0).abs().amax(-1, keepdim=True).clamp_min(1) if es.shape[-1] and S.shape[-1] else torch.ones_like(lse)
         ep = 2 * es + 8 * e * big + n * e
         O = mm(P, V)
-        o_bound = u * O.abs() + (u + ep + n * e) * mm(P, V.abs()) + tiny * mm((~hide).double(), V.abs())
+        o_bound = u * O.abs() + tiny + (u + ep + n * e) * mm(P, V.abs()) + tiny * mm((~hide).double(), V.abs())
         self.out, self.out_bound = back(O), back(o_bound) * 1.01
         self.lse = lse.squeeze(-1)
         self.lse_bound = (es + n * e + 8 * e * lse.abs().clamp_min(1)).squeeze(-1)
@@ -80,9 +81,9 @@ class Reference:
         d_err = (DO.abs() * (o_bound * 1.01 + dim * e * O.abs())).sum(-1, keepdim=True) + (dim + 4) * e * mm(DO.abs(), V.abs().transpose(-1, -2))
         ds_bound = (u + ep + 4 * e) * dS.abs() + (1 + u) * P * d_err + tiny * (~hide)
         self.dv, self.dk, self.dq = share(dV), share(mm(dS.transpose(-1, -2), Q) * scale), back(mm(dS, K) * scale)
-        self.dv_bound = (u * self.dv.abs() + share(dv_bound)) * 1.01
-        self.dq_bound = (u * self.dq.abs() + back(mm(ds_bound + n * e * dS.abs(), K.abs()) * scale)) * 1.01
-        self.dk_bound = (u * self.dk.abs() + share(mm((ds_bound + rows * e * dS.abs()).transpose(-1, -2), Q.abs()) * scale)) * 1.01
+        self.dv_bound = (u * self.dv.abs() + tiny + share(dv_bound)) * 1.01
+        self.dq_bound = (u * self.dq.abs() + tiny + back(mm(ds_bound + n * e * dS.abs(), K.abs()) * scale)) * 1.01
+        self.dk_bound = (u * self.dk.abs() + tiny + share(mm((ds_bound + rows * e * dS.abs()).transpose(-1, -2), Q.abs()) * scale)) * 1.01
 
     def check(self, **got):
         for name, x in got.items():

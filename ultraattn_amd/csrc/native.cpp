@@ -841,6 +841,46 @@ PyObject* swa_forward(PyObject* const* a) {
   return tuple_of(out, lse);
 }
 
+// swa_backward(dout, q, k, v, out, lse, dq, dk, dv, softmax_d, left, right, sinks, q_start, k_start, softmax_scale) -> (dq, dk, dv)
+PyObject* swa_backward(PyObject* const* a) {
+  const at::Tensor &dout = tensor(a[0], "dout"), &q = tensor(a[1], "q"), &k = tensor(a[2], "k"), &v = tensor(a[3], "v"), &lse = tensor(a[5], "lse");
+  check_swa(q, k, v, "k", "v");
+  const int dt = dtype_code("q", q, false);
+  check_rows4("dout", dout, q);
+  check_shape("dout", dout, q.sizes());
+  check_lse("lse", lse, q);
+  const Window w(a + 10, q.size(1), k.size(1));
+  const float scale = swa_scale(a[15], q.size(3));
+  Slot dq(a[6]), dk(a[7]), dv(a[8]);
+  result(dq, "dq", q);
+  result(dk, "dk", k);
+  result(dv, "dv", v);
+  const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), sq = (int)q.size(1), sk = (int)k.size(1), D = (int)q.size(3);
+  const On on(q);
+  at::Tensor delta;
+  if (a[9] != Py_None) {
+    delta = tensor(a[9], "softmax_d");
+    check_lse("softmax_d", delta, q);
+  } else {
+    if (a[4] == Py_None) fail(PyExc_ValueError, "either out or softmax_d is required");
+    const at::Tensor& out = tensor(a[4], "out");
+    check_rows4("out", out, q);
+    check_shape("out", out, q.sizes());
+    delta = stat_of(q);
+    call("ua_swa_bwd_delta", [&] {
+      return ua_swa_bwd_delta(out.data_ptr(), dout.data_ptr(), (float*)delta.data_ptr(), B, H, sq, D, dt, used_strides(out), used_strides(dout), on.stream);
+    });
+  }
+  const at::Tensor ws = scratch(ua_swa_bwd_workspace_bytes(B, H, Hk, sq, sk, D, w.q_start, w.k_start, w.left, w.right, w.sinks), q);
+  call("ua_swa_bwd", [&] {
+    return ua_swa_bwd(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), (const float*)lse.data_ptr(), (const float*)delta.data_ptr(),
+                      dq.t.data_ptr(), dk.t.data_ptr(), dv.t.data_ptr(), B, H, Hk, sq, sk, D, dt, used_strides(dout), used_strides(q), used_strides(k),
+                      used_strides(v), used_strides(dq.t), used_strides(dk.t), used_strides(dv.t), w.q_start, w.k_start, w.left, w.right, w.sinks, scale,
+                      ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, on.stream);
+  });
+  return tuple_of(dq, dk, dv);
+}
+
 // ---- module ---------------------------------------------------------------------------------------------
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -866,7 +906,8 @@ PyMethodDef methods[] = {
     UA_METHOD(dense_forward, 8), UA_METHOD(dense_backward, 14), UA_METHOD(bsa_forward, 10), UA_METHOD(bsa_backward, 15),
     UA_METHOD(delta, 3), UA_METHOD(grad_accumulate, 4), UA_METHOD(merge, 4), UA_METHOD(grad_sum, 3),
     UA_METHOD(merge_update, 5), UA_METHOD(permute_cols, 6), UA_METHOD(lists_from_mask, 5),
-    UA_METHOD(build_lists_device, 3), UA_METHOD(rope, 10), UA_METHOD(rope_append, 10), UA_METHOD(swa_forward, 11), {nullptr, nullptr, 0, nullptr}};
+    UA_METHOD(build_lists_device, 3), UA_METHOD(rope, 10), UA_METHOD(rope_append, 10), UA_METHOD(swa_forward, 11), UA_METHOD(swa_backward, 16),
+    {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "Native host side of the attention operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

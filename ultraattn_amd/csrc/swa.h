@@ -43,22 +43,26 @@ struct SwaHead {
   static_assert(kD == 64 || kD == 128, "head sizes");
   static constexpr int kRow = 2 * kD, kChunks = kD / 8, kSteps = kD / 16, kBlocks = kD / 32;
   static constexpr int kCopyRows = 1024 / kRow, kCopies = kSwaBlock / kCopyRows / 4;      // of a wave and a block
-  static constexpr int kTile = kSwaBlock * kRow;
+  static constexpr int kUnits = kSwaBlock / kCopyRows;                                    // of a block
   // rows are read as they are: 16 rows at one chunk
   static __device__ __forceinline__ int slot_n(int r, int c) { return kD == 128 ? c ^ (r & 15) : c ^ (r >> 1 & 7); }
   // rows are read transposed: 4 rows at 4 chunks that start at a multiple of 4
   static __device__ __forceinline__ int slot_t(int r, int c) { return kD == 128 ? c ^ ((r & 3) << 2) : c ^ ((r >> 1 & 1) << 2); }
-  static __device__ __forceinline__ uint32_t at_n(int r, int c) { return r * kRow + (slot_n(r, c) << 4); }
-  // byte offset in memory of what lane `lane` of wave `wave` copies first, from a block's first row on
-  template <bool kTransposed>
-  static __device__ __forceinline__ int copy_offset(int row_stride, int wave, int lane) {
-    const int r = kCopyRows * wave + lane / kChunks, s = lane % kChunks;
-    return (r * row_stride + (kTransposed ? slot_t(r, s) : slot_n(r, s)) * 8) * 2;
+  // both: of 256 bytes as transposed, the fours of rows at a pitch of 1040 bytes, so that 16 rows meet 16 slots; of 128 bytes three bits of the row
+  static __device__ __forceinline__ int slot_b(int r, int c) {
+    return kD == 128 ? slot_t(r, c) : c ^ ((r >> 1 & 1) << 2) ^ ((r >> 2 & 1) << 1) ^ (r >> 3 & 1);
   }
-  // transposing read m (of kBlocks): columns 32 m + lane % 32, rows 4 (lane / 32) .. + 3
+  static constexpr int kPitchB = kD == 128 ? 1040 : 1024, kTile = kUnits * 1024, kTileB = kUnits * kPitchB;
+  static __device__ __forceinline__ uint32_t at_n(int r, int c) { return r * kRow + (slot_n(r, c) << 4); }
+  static __device__ __forceinline__ uint32_t at_b(int r, int c) { return r / kCopyRows * kPitchB + r % kCopyRows * kRow + (slot_b(r, c) << 4); }
+  // transposing read m (of kBlocks): columns 32 m + lane % 32, rows 4 (lane / 32) .. + 3; of the `both` layout, rows + 8 * second
   static __device__ __forceinline__ uint32_t tr_offset(int lane, int m) {
     const int i = lane & 15, r = i >> 2, row = 4 * (lane >> 5) + r;
     return row * kRow + (slot_t(row, 4 * m + 2 * (lane >> 4 & 1) + ((i & 3) >> 1)) << 4) + (i & 1) * 8;
+  }
+  static __device__ __forceinline__ uint32_t tr_offset_b(int lane, int m, int second) {
+    const int i = lane & 15, r = i >> 2, row = 4 * (lane >> 5) + r + 8 * second;
+    return at_b(row, 4 * m + 2 * (lane >> 4 & 1) + ((i & 3) >> 1)) + (i & 1) * 8;
   }
 };
 
@@ -124,21 +128,30 @@ __device__ __forceinline__ void swa_store_f32(float* rows, int64_t row_stride, i
   }
 }
 
-// Two operands of 64 rows, copied asynchronously into a stage of LDS: x at 0, y at kTile.
-template <int kD, bool kXT, bool kYT>
+// Two operands of 64 rows, copied asynchronously into a stage of LDS, x at 0, y behind it.  How either is read there: as it is (kN),
+// transposed (kT), or both.
+enum SwaRead { kN, kT, kB };
+template <int kD, SwaRead kX, SwaRead kY>
 struct SwaStream {
   using H = SwaHead<kD>;
   static constexpr int kPieces = 2 * H::kCopies;
+  static constexpr int kPitchX = kX == kB ? H::kPitchB : 1024, kPitchY = kY == kB ? H::kPitchB : 1024, kSecond = H::kUnits * kPitchX;
+  static constexpr int kBytes = kSecond + H::kUnits * kPitchY;
   const char *x, *y;
   int64_t xs, ys;                                  // bytes of a row
   int xoff, yoff;
   u32x4 rx, ry;
-  uint32_t wave_lds;
-  __device__ __forceinline__ SwaStream(const void* x_, int64_t xs_, const void* y_, int64_t ys_, int wave, int lane)
-      : x((const char*)x_), y((const char*)y_), xs(2 * xs_), ys(2 * ys_), wave_lds(wave * 1024) {
-    xoff = H::template copy_offset<kXT>((int)xs_, wave, lane);
-    yoff = H::template copy_offset<kYT>((int)ys_, wave, lane);
+  uint32_t wave;
+  template <SwaRead kRead>
+  static __device__ __forceinline__ int offset(int row_stride, int wave, int lane) {       // of a copy's lane from the block's first row on
+    const int r = H::kCopyRows * wave + lane / H::kChunks, s = lane % H::kChunks;
+    return (r * row_stride + (kRead == kN ? H::slot_n(r, s) : kRead == kT ? H::slot_t(r, s) : H::slot_b(r, s)) * 8) * 2;
   }
+  __device__ __forceinline__ SwaStream(int64_t xs_, int64_t ys_, int wave_, int lane) : xs(2 * xs_), ys(2 * ys_), wave(wave_) {
+    xoff = offset<kX>((int)xs_, wave_, lane);
+    yoff = offset<kY>((int)ys_, wave_, lane);
+  }
+  __device__ __forceinline__ void of(const void* x_, const void* y_) { x = (const char*)x_; y = (const char*)y_; }
   // Rows row0 .. row0 + 63 of n are next; those from n on read as zeros, and without `more` all of them.
   __device__ __forceinline__ void block(int row0, int n, bool more) {
     const int rows = more ? min(n - row0, kSwaBlock) : 0;
@@ -147,8 +160,8 @@ struct SwaStream {
   }
   __device__ __forceinline__ void copy(int n, uint32_t stage) const {
     const int j = n >> 1, row = 4 * H::kCopyRows * j;
-    if (n & 1) dma16_abs(ry, stage + H::kTile + wave_lds + 4096 * j, yoff, row * (int)ys);
-    else       dma16_abs(rx, stage + wave_lds + 4096 * j, xoff, row * (int)xs);
+    if (n & 1) dma16_abs(ry, stage + kSecond + (4 * j + wave) * kPitchY, yoff, row * (int)ys);
+    else       dma16_abs(rx, stage + (4 * j + wave) * kPitchX, xoff, row * (int)xs);
   }
 };
 
@@ -180,13 +193,14 @@ struct SwaParams {
   Strides3 qs, ks, vs, os, ds, dqs, dks, dvs;
   int batch, n_heads, n_kv_heads, group, seq_q, seq_k, hi, lo, sinks;
   float scale, scale_log2;
-  // Forward: the walks are cut into n_parts, part i leaves fp32 rows and their lse at part_o + i * o_part and part_lse + i * lse_part.
-  int n_parts;
-  float *part_o, *part_lse;
-  int64_t o_part, lse_part;
+  // The rows' walks are cut into n_parts; part i leaves fp32 rows (and, forward, their lse), contiguous [batch, heads, tokens, head_dim], at part_o +
+  // i * o_part and part_lse + i * lse_part.  Backward: the first n_cut columns' walks are cut into col_parts, dK and dV alike.
+  int n_parts, n_cut, col_parts;
+  float *part_o, *part_lse, *part_dk, *part_dv;
+  int64_t o_part, lse_part, col_part;
   BlockMap map, cols;
-  Div by_heads, by_kv_heads, by_group, by_parts;
-  int n_qtiles, n_ktiles, n_col_blocks;
+  Div by_heads, by_kv_heads, by_group, by_parts, by_cols, by_cut;
+  int n_qtiles, n_ktiles, n_cut_blocks, n_col_blocks;
 };
 
 int swa_fill(SwaParams& p, int batch, int n_heads, int n_kv_heads, int seq_q, int seq_k, int head_dim, int dtype, int64_t q_start, int64_t k_start,

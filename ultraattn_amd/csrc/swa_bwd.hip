@@ -1,0 +1,610 @@
+// Sliding-window attention with sinks, backward: P is made again from the rows' LSE, nothing is added atomically.
+//
+//   columns: a workgroup (4 waves of 32 keys) per (128 keys, key head) holds K and V and walks the blocks of 64 query rows that see
+//            it, of all query heads that share it:  S = Q K^T, dP = dO V^T - delta, dV^T += dO^T P, dK^T += Q^T dS;
+//   rows:    a workgroup per (128 queries, head) holds Q and dO and walks the blocks of 64 keys (SwaWalk):
+//            S^T = K Q^T, dP^T = V dO^T - delta, dQ^T += K^T dS^T.
+// P = exp2(scale log2(e) S - log2(e) LSE), dS = P dP; dK and dQ are multiplied by the scale at their end.  In the accumulators a lane holds
+// one key (query), so that P and dS, rounded, are operands of the next products.  Both sides are one launch: neither leaves the device partly
+// empty at its end.
+//
+// A column of the sinks is seen by every later query: its walk is cut into parts of about the others' length, which leave fp32 dK and
+// dV that a last launch adds in their order.  So are all walks where there are few of them.
+#include <algorithm>
+#include "swa.h"
+
+namespace ua {
+
+// P <= 1 in fp16 is below its normal range from 6e-5 on, where long rows are: it is held times 2^14, dV is divided by that.
+template <class T> constexpr float kSwaPScale = 1.f;
+template <> constexpr float kSwaPScale<fp16> = 16384.f;
+
+template <int kD> using BwdStream = SwaStream<kD, kB, kB>;
+template <int kD> struct BwdLds {
+  static constexpr int kStage = BwdStream<kD>::kBytes, kStat = 2 * kStage, kStatBytes = 2 * kSwaBlock * 4, kBytes = kStat + 2 * kStatBytes;
+};
+// Addresses, within a stage, of 128-bit reads of 32 rows and of transposing reads.
+template <class T, int kD>
+struct BwdAddr {
+  using H = SwaHead<kD>;
+  typedef typename SwaVec<T>::x8 x8;
+  static constexpr int kNat = 4, kTr = 4;
+  uint32_t nat[kNat], tr[kTr];
+  __device__ __forceinline__ explicit BwdAddr(uint32_t lds) {
+    const int lane = fresh_lane();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // (of 128 columns the chunks 2 i and 2 i + 1 of 16 lie 32 bytes apart; so do rows 8 apart, at a constant)
+      nat[i] = lds + H::at_b(lane & 31, (kD == 128 ? 4 : 2) * i + (lane >> 5));
+      tr[i] = lds + (kD == 128 ? H::tr_offset_b(lane, i, 0) : H::tr_offset_b(lane, i >> 1, i & 1));
+      asm volatile("" : "+v"(nat[i]), "+v"(tr[i]));
+    }
+  }
+  static constexpr int kRows32 = 32 / H::kCopyRows * H::kPitchB, kRows16 = kRows32 / 2, kRows8 = kRows32 / 4;
+  template <int kOff> __device__ __forceinline__ x8 row(int i) const {                 // columns 16 i ..
+    return lds_get<x8>(kD == 128 ? nat[i >> 1] + (kOff + 32 * (i & 1)) : nat[i] + kOff);
+  }
+  template <int kOff> __device__ __forceinline__ x8 column(int i) const {              // columns 32 (i % kBlocks), 16 rows from 16 (i / kBlocks) on
+    constexpr int kB = H::kBlocks;
+    const int rows = kOff + kRows16 * (i / kB);
+    return kD == 128 ? lds_tr_pair<T>(tr[i % kB] + rows, tr[i % kB] + (rows + kRows8)) : lds_tr_pair<T>(tr[2 * (i % kB)] + rows, tr[2 * (i % kB) + 1] + rows);
+  }
+};
+
+// The kernel's parameters read again from the kernel-argument segment: each walk's behind the branch that leads to it, and its end's behind the
+// walk.  All at once ask for more scalar registers than there are, and live in vector lanes then.
+__device__ __forceinline__ const SwaParams& params_again() {
+  typedef const __attribute__((address_space(4))) SwaParams* Late;
+  Late p = (Late)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const SwaParams*)p;
+}
+
+// ---- columns ------------------------------------------------------------------------------------------------------
+// 32 query rows at kOff of a stage, their statistics at `stat`.  first, seen: the rows row0 + quad that a lane's key is visible to, if `mask`.
+template <class T, int kD, int kOff, int kCopies, class Copy>
+__device__ __forceinline__ void dkdv_rows(const BwdAddr<T, kD>& ad, uint32_t stat, const typename SwaVec<T>::x8 (&kf)[kD / 16],
+                                          const typename SwaVec<T>::x8 (&vf)[kD / 16], f32x16 (&dk)[kD / 32], f32x16 (&dv)[kD / 32], float scale_log2,
+                                          bool mask, int row0, int first, uint32_t seen, Copy copy) {
+  using V = SwaVec<T>;
+  using H = SwaHead<kD>;
+  typedef typename V::x8 x8;
+  constexpr int kY = BwdStream<kD>::kSecond;
+  f32x16 s, dp;
+  const uint32_t mine = stat + 16 * (fresh_lane() >> 5);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 a = lds_get<f32x4>(mine + 32 * g), c = lds_get<f32x4>(mine + kSwaBlock * 4 + 32 * g);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { s[4 * g + j] = a[j]; dp[4 * g + j] = c[j]; }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  {
+    constexpr int kAhead = 2, kAll = 2 * H::kSteps;
+    x8 fr[kAll];
+    auto rd = [&](int i) { return (i & 1) ? ad.template row<kOff + kY>(i >> 1) : ad.template row<kOff>(i >> 1); };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fr[i] = rd(i);
+    __builtin_amdgcn_sched_group_barrier(0x100, 8 + kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < kAll; ++i) {
+      if (i + kAhead < kAll) fr[i + kAhead] = rd(i + kAhead);
+      if (i & 1) dp = V::mfma(fr[i], vf[i >> 1], dp);
+      else       s = V::mfma(fr[i], kf[i >> 1], s);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if ((i + 1) * kCopies / kAll != i * kCopies / kAll) copy(i * kCopies / kAll);
+    }
+  }
+  constexpr int kTAhead = 2, kTAll = 4 * H::kBlocks;
+  auto rd_tr = [&](int i) { return (i & 1) ? ad.template column<kOff>(i >> 1) : ad.template column<kOff + kY>(i >> 1); };
+  x8 ft[kTAll];
+#pragma unroll
+  for (int i = 0; i < kTAhead; ++i) ft[i] = rd_tr(i);
+  if (mask) {
+    const int row = row0 + 4 * (fresh_lane() >> 5) - first;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if ((uint32_t)(row + 8 * (i >> 2) + (i & 3)) >= seen) s[i] = -INFINITY;
+  }
+  x8 pb[2], dsb[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float e = fast_exp2(s[i] * scale_log2);
+    pb[i >> 3][i & 7] = (T)(kSwaPScale<T> == 1.f ? e : e * kSwaPScale<T>);
+    dsb[i >> 3][i & 7] = (T)(e * dp[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kTAll; ++i) {
+    if (i + kTAhead < kTAll) ft[i + kTAhead] = rd_tr(i + kTAhead);
+    const int n = i >> 1, m = n % H::kBlocks, t = n / H::kBlocks;
+    if (i & 1) dk[m] = V::mfma(ft[i], dsb[t], dk[m]);
+    else       dv[m] = V::mfma(ft[i], pb[t], dv[m]);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+  }
+}
+
+template <class T, int kD>
+__device__ __forceinline__ void columns_walk(uint32_t lds, int block) {
+  const SwaParams& p = params_again();
+  using H = SwaHead<kD>;
+  using L = BwdLds<kD>;
+  typedef typename SwaVec<T>::x8 x8;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int kt, bh, part = 0;
+  const bool cut = block < p.n_cut_blocks;
+  if (cut) {                                             // the parts of one column far from each other
+    const int rest = quotient(block, p.by_cols);
+    bh = block - rest * p.by_cols.d;
+    part = quotient(rest, p.by_cut);
+    kt = rest - part * p.n_cut;
+  } else {
+    map_block(block - p.n_cut_blocks, p.cols, kt, bh);
+    kt += p.n_cut;
+  }
+  const int b = quotient(bh, p.by_kv_heads), hk = bh - b * p.n_kv_heads, k0 = kt * kSwaRows;
+  const SwaColumn col(k0, min(k0 + kSwaRows, p.seq_k) - 1, p.hi, p.lo, p.sinks, p.seq_q);
+  const int total = col.n * p.group, part_len = cut ? (total + p.col_parts - 1) / p.col_parts : total;
+  const int i0 = min(part * part_len, total), i1 = min(i0 + part_len, total);
+
+  // a step's place: query head (of the group) and block of 64 rows
+  int g = __builtin_amdgcn_readfirstlane(col.n ? i0 / col.n : 0), at = i0 - g * col.n;
+  BwdStream<kD> in(p.qs.s, p.ds.s, wave, lane);
+  auto base = [&](int head) {
+    const int h = hk * p.group + head;
+    in.of((const T*)p.q + b * p.qs.b + h * p.qs.h, (const T*)p.dout + b * p.ds.b + h * p.ds.h);
+  };
+  // -lse / scale (rows that see nothing, and rows that are not there: -inf, so that P = 0) and -delta, from which S and dP start; two waves bring either
+  auto load_stat = [&](int head, int row0) {
+    const int row = row0 + 32 * (wave & 1) + (fresh_lane() & 31);
+    const float* rows = (wave >= 2 ? p.delta : p.lse) + ((int64_t)b * p.n_heads + hk * p.group + head) * p.seq_q;
+    return row < p.seq_q ? rows[row] : wave >= 2 ? 0.f : -INFINITY;
+  };
+  const float scale_log2 = p.scale_log2;
+  auto put_stat = [&](int stage, float x) {
+    const float y = wave >= 2 ? -x : x == -INFINITY ? x : x * (-kLog2e / scale_log2);
+    lds_put(lds + L::kStat + stage * L::kStatBytes + 128 * wave + 4 * (fresh_lane() & 31), y);
+  };
+  float stat = 0.f;
+  if (i0 < i1) {
+    base(g);
+    in.block((col.first + at) * kSwaBlock, p.seq_q, true);
+#pragma unroll
+    for (int n = 0; n < in.kPieces; ++n) in.copy(n, lds);
+    stat = load_stat(g, (col.first + at) * kSwaBlock);
+  }
+  const int key0 = k0 + 32 * wave, from = min(key0, p.seq_k - 1);
+  x8 kf[H::kSteps], vf[H::kSteps];
+  {
+    u32x4 kraw[H::kSteps], vraw[H::kSteps];
+    swa_load_rows<kD>(kraw, (const T*)p.k + b * p.ks.b + from * p.ks.s + hk * p.ks.h, p.ks.s, p.seq_k - from);
+    swa_load_rows<kD>(vraw, (const T*)p.v + b * p.vs.b + from * p.vs.s + hk * p.vs.h, p.vs.s, p.seq_k - from);
+    const uint32_t turn = lds + L::kStage + wave * 32 * H::kRow;       // the stage that the first step fills
+    swa_put_rows<kD>(kraw, turn);
+    swa_frags<T, kD>(kf, turn);
+    swa_put_rows<kD>(vraw, turn);
+    swa_frags<T, kD>(vf, turn);
+  }
+  f32x16 dk[H::kBlocks], dv[H::kBlocks];
+#pragma unroll
+  for (int m = 0; m < H::kBlocks; ++m) { dk[m] = f32x16{0}; dv[m] = f32x16{0}; }
+  const BwdAddr<T, kD> ad(lds);
+  if (i0 < i1) put_stat(0, stat);
+#pragma unroll
+  for (int i = 0; i < H::kSteps; ++i) asm volatile("" : "+v"(kf[i]), "+v"(vf[i]));      // arrived before the walk
+  // the rows that this lane's key is visible to: first .. first + seen - 1
+  const int key = key0 + (lane & 31);
+  wait_vmem_all();
+  __syncthreads();
+
+  auto step = [&](int i, auto stage_tag) {
+    constexpr int kStage = decltype(stage_tag)::value;
+    const int row0 = (col.first + at) * kSwaBlock;
+    if (++at == col.n) { at = 0; base(++g < p.group ? g : 0); }
+    const int next0 = (col.first + at) * kSwaBlock;
+    in.block(next0, p.seq_q, i + 1 < i1);
+    if (i + 1 < i1) stat = load_stat(g, next0);
+    const uint32_t other = lds + (kStage ^ 1) * L::kStage;
+    auto rows = [&](auto mb_tag) {
+      constexpr int kMb = decltype(mb_tag)::value, kCopies = BwdStream<kD>::kPieces / 2;
+      const int r0 = row0 + 32 * kMb;
+      auto copy = [&](int n) { in.copy(kMb * kCopies + n, other); };
+      // beyond the rows, before what they see, or behind it and no sink
+      int hidden = __builtin_amdgcn_readfirstlane(max(max(r0 - p.seq_q + 1, key0 - r0 - 31 - p.hi), min(r0 + p.lo - key0 - 31, key0 - p.sinks + 1)));
+      if (hidden > 0)
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n) copy(n);
+      asm volatile("" : "+s"(hidden));       // (as two sides of one branch the products do not stay in the same registers)
+      if (hidden > 0) return;
+      const bool whole = key0 + 31 <= r0 + p.hi && (key0 >= r0 + 31 + p.lo || key0 + 31 < p.sinks);
+      int first = 0;
+      uint32_t seen = 0;
+      if (!whole) {
+        first = key - p.hi;
+        const int last = key < p.sinks ? 2 * kFar - 1 : key - p.lo;
+        seen = last >= first ? (uint32_t)last - (uint32_t)first + 1u : 0u;
+      }
+      dkdv_rows<T, kD, kStage * L::kStage + kMb * BwdAddr<T, kD>::kRows32, kCopies>(
+          ad, lds + L::kStat + kStage * L::kStatBytes + kMb * 128, kf, vf, dk, dv, scale_log2, !whole, r0, first, seen, copy);
+    };
+    rows(std::integral_constant<int, 0>{});
+    rows(std::integral_constant<int, 1>{});
+    wait_vmem_all();
+    if (i + 1 < i1) put_stat(kStage ^ 1, stat);
+    __syncthreads();                        // the next block has landed, and everyone has left this one
+  };
+  for (int i = i0; i < i1; i += 2) {
+    step(i, std::integral_constant<int, 0>{});
+    if (i + 1 < i1) step(i + 1, std::integral_constant<int, 1>{});
+  }
+  const SwaParams& e = params_again();
+  const int n_rows = e.seq_k - key0;
+  if (n_rows <= 0) return;
+  if (cut) {
+    const int64_t row = part * e.col_part + ((int64_t)bh * e.n_cut * kSwaRows + key0) * kD;
+    swa_store_f32<kD>(e.part_dk + row, kD, n_rows, dk, e.scale);
+    swa_store_f32<kD>(e.part_dv + row, kD, n_rows, dv, 1.f / kSwaPScale<T>);
+  } else {
+    const uint32_t turn = lds + wave * 32 * H::kRow;
+    swa_store_rows<T, kD>((T*)e.dk + b * e.dks.b + (int64_t)key0 * e.dks.s + hk * e.dks.h, e.dks.s, n_rows, dk, e.scale, turn);
+    swa_store_rows<T, kD>((T*)e.dv + b * e.dvs.b + (int64_t)key0 * e.dvs.s + hk * e.dvs.h, e.dvs.s, n_rows, dv, 1.f / kSwaPScale<T>, turn);
+  }
+}
+
+// ---- rows ---------------------------------------------------------------------------------------------------------
+template <class T, int kD, int kOff, int kCopies, class Copy>
+__device__ __forceinline__ void dq_keys(const BwdAddr<T, kD>& ad, const typename SwaVec<T>::x8 (&qf)[kD / 16], const typename SwaVec<T>::x8 (&dof)[kD / 16],
+                                        const f32x16& neg_delta, f32x16 (&dq)[kD / 32], float scale_log2, float lse2, bool mask, int key0, int first,
+                                        uint32_t seen, int sinks, Copy copy) {
+  using V = SwaVec<T>;
+  using H = SwaHead<kD>;
+  typedef typename V::x8 x8;
+  constexpr int kY = BwdStream<kD>::kSecond;
+  f32x16 s, dp;
+  {
+    constexpr int kAhead = 4, kAll = 2 * H::kSteps;
+    x8 fr[kAll];
+    auto rd = [&](int i) { return (i & 1) ? ad.template row<kOff + kY>(i >> 1) : ad.template row<kOff>(i >> 1); };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fr[i] = rd(i);
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < kAll; ++i) {
+      if (i + kAhead < kAll) fr[i + kAhead] = rd(i + kAhead);
+      if (i & 1) dp = V::mfma(fr[i], dof[i >> 1], i == 1 ? neg_delta : dp);
+      else       s = V::mfma(fr[i], qf[i >> 1], i == 0 ? f32x16{0} : s);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if ((i + 1) * kCopies / kAll != i * kCopies / kAll) copy(i * kCopies / kAll);
+    }
+  }
+  constexpr int kTAhead = 3, kTAll = 2 * H::kBlocks;
+  x8 ft[kTAll];
+#pragma unroll
+  for (int i = 0; i < kTAhead; ++i) ft[i] = ad.template column<kOff>(i);
+  if (mask) {
+    const int key = key0 + 4 * (fresh_lane() >> 5);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int k = key + 8 * (i >> 2) + (i & 3);
+      if ((uint32_t)(k - first) >= seen && k >= sinks) s[i] = -INFINITY;
+    }
+  }
+  x8 dsb[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) dsb[i >> 3][i & 7] = (T)(fast_exp2(fmaf(s[i], scale_log2, -lse2)) * dp[i]);
+#pragma unroll
+  for (int i = 0; i < kTAll; ++i) {
+    if (i + kTAhead < kTAll) ft[i + kTAhead] = ad.template column<kOff>(i + kTAhead);
+    dq[i % H::kBlocks] = V::mfma(ft[i], dsb[i / H::kBlocks], dq[i % H::kBlocks]);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+  }
+}
+
+template <class T, int kD>
+__device__ __forceinline__ void rows_walk(uint32_t lds, int block) {
+  const SwaParams& p = params_again();
+  using H = SwaHead<kD>;
+  using L = BwdLds<kD>;
+  typedef typename SwaVec<T>::x8 x8;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int pos, bh;
+  map_block(block, p.map, pos, bh);
+  const int line = quotient(pos, p.by_parts), part = pos - line * p.n_parts, qt = p.n_qtiles - 1 - line;
+  const int b = quotient(bh, p.by_heads), h = bh - b * p.n_heads, hk = quotient(h, p.by_group);
+  const int r0 = qt * kSwaRows, row0 = r0 + 32 * wave, n_rows = p.seq_q - row0;
+  const SwaWalk walk(r0, min(r0 + kSwaRows, p.seq_q) - 1, p.hi, p.lo, p.sinks, p.seq_k);
+  const int part_len = (walk.n + p.n_parts - 1) / p.n_parts, i0 = min(part * part_len, walk.n), i1 = min(i0 + part_len, walk.n);
+  BwdStream<kD> in(p.ks.s, p.vs.s, wave, lane);
+  in.of((const T*)p.k + b * p.ks.b + hk * p.ks.h, (const T*)p.v + b * p.vs.b + hk * p.vs.h);
+  if (i0 < i1) {
+    in.block(walk.at(i0) * kSwaBlock, p.seq_k, true);
+#pragma unroll
+    for (int n = 0; n < in.kPieces; ++n) in.copy(n, lds);
+  }
+  const int from = min(row0, p.seq_q - 1);
+  x8 qf[H::kSteps], dof[H::kSteps];
+  float lse_raw, neg_delta;
+  {
+    u32x4 qraw[H::kSteps], doraw[H::kSteps];
+    swa_load_rows<kD>(qraw, (const T*)p.q + b * p.qs.b + from * p.qs.s + h * p.qs.h, p.qs.s, p.seq_q - from);
+    swa_load_rows<kD>(doraw, (const T*)p.dout + b * p.ds.b + from * p.ds.s + h * p.ds.h, p.ds.s, p.seq_q - from);
+    const int64_t row = (int64_t)bh * p.seq_q + min(row0 + (lane & 31), p.seq_q - 1);
+    lse_raw = p.lse[row];
+    neg_delta = -p.delta[row];
+    const uint32_t turn = lds + L::kStage + wave * 32 * H::kRow;
+    swa_put_rows<kD>(qraw, turn);
+    swa_frags<T, kD>(qf, turn);
+    swa_put_rows<kD>(doraw, turn);
+    swa_frags<T, kD>(dof, turn);
+  }
+  const float lse2 = lse_raw == -INFINITY ? INFINITY : lse_raw * kLog2e;        // (P = 0 in rows that see nothing)
+  f32x16 nd, dq[H::kBlocks];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) nd[i] = neg_delta;
+  asm volatile("" : "+v"(nd));              // registers, not one value moved into an accumulator again and again
+#pragma unroll
+  for (int m = 0; m < H::kBlocks; ++m) dq[m] = f32x16{0};
+  const BwdAddr<T, kD> ad(lds);
+#pragma unroll
+  for (int i = 0; i < H::kSteps; ++i) asm volatile("" : "+v"(qf[i]), "+v"(dof[i]));
+
+  auto step = [&](int i, auto stage_tag) {
+    constexpr int kStage = decltype(stage_tag)::value;
+    const int block0 = walk.at(i) * kSwaBlock;
+    in.block(walk.at(i + 1) * kSwaBlock, p.seq_k, i + 1 < i1);
+    wait_vmem_all();
+    __syncthreads();                        // this block has landed, and everyone has left the other stage
+    const uint32_t other = lds + (kStage ^ 1) * L::kStage;
+    auto keys = [&](auto mb_tag) {
+      constexpr int kMb = decltype(mb_tag)::value, kCopies = BwdStream<kD>::kPieces / 2;
+      const int key0 = block0 + 32 * kMb;
+      auto copy = [&](int n) { in.copy(kMb * kCopies + n, other); };
+      int hidden = __builtin_amdgcn_readfirstlane(max(max(key0 - p.seq_k + 1, key0 - row0 - 31 - p.hi), min(row0 + p.lo - key0 - 31, key0 - p.sinks + 1)));
+      if (hidden > 0)
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n) copy(n);
+      asm volatile("" : "+s"(hidden));       // (see columns_walk)
+      if (hidden > 0) return;
+      const bool whole = key0 + 31 <= min(row0 + p.hi, p.seq_k - 1) && (key0 >= row0 + 31 + p.lo || key0 + 31 < p.sinks);
+      int first = 0, sinks = 0;
+      uint32_t seen = 0;
+      if (!whole) {
+        const int row = row0 + (fresh_lane() & 31), last = min(row + p.hi, p.seq_k - 1);
+        first = row + p.lo;
+        seen = (uint32_t)max(last - first + 1, 0);
+        sinks = min(p.sinks, last + 1);
+      }
+      dq_keys<T, kD, kStage * L::kStage + kMb * BwdAddr<T, kD>::kRows32, kCopies>(ad, qf, dof, nd, dq, p.scale_log2, lse2, !whole, key0, first, seen, sinks,
+                                                                                  copy);
+    };
+    keys(std::integral_constant<int, 0>{});
+    keys(std::integral_constant<int, 1>{});
+  };
+  for (int i = i0; i < i1; i += 2) {
+    step(i, std::integral_constant<int, 0>{});
+    if (i + 1 < i1) step(i + 1, std::integral_constant<int, 1>{});
+  }
+  wait_vmem_all();                          // the last step's copies filled a stage with zeros
+  __syncthreads();
+  if (n_rows <= 0) return;
+  const SwaParams& e = params_again();
+  if (e.n_parts > 1)
+    swa_store_f32<kD>(e.part_o + part * e.o_part + ((int64_t)bh * e.seq_q + row0) * kD, kD, n_rows, dq, e.scale);
+  else
+    swa_store_rows<T, kD>((T*)e.dq + b * e.dqs.b + (int64_t)row0 * e.dqs.s + h * e.dqs.h, e.dqs.s, n_rows, dq, e.scale, lds + wave * 32 * H::kRow);
+}
+
+template <class T, int kD>
+__global__ __launch_bounds__(256, 2) void swa_bwd_kernel(const SwaParams p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[BwdLds<kD>::kBytes];
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)smem;
+  if ((int)blockIdx.x < p.n_col_blocks) columns_walk<T, kD>(lds, blockIdx.x);
+  else                                  rows_walk<T, kD>(lds, blockIdx.x - p.n_col_blocks);
+}
+
+// delta = rowsum(dO * O).  16 tokens of 4 heads a workgroup: memory sees rows of 4 heads, and 64 bytes of each head's result.
+template <class T, int kD>
+__global__ __launch_bounds__(256) void swa_delta_kernel(const T* o, const T* dout, float* delta, Strides3 os, Strides3 ds, int n_heads, int seq, Div by_tokens,
+                                                        Div by_heads) {
+  constexpr int kLanes = kD / 8, kRows = 256 / kLanes;
+  typedef typename SwaVec<T>::x8 x8;
+  __shared__ float sums[16][4];
+  const int th = quotient(blockIdx.x, by_heads), hb = blockIdx.x - th * by_heads.d, b = quotient(th, by_tokens), t0 = (th - b * by_tokens.d) * 16, h0 = 4 * hb;
+  const int lane = threadIdx.x % kLanes;
+#pragma unroll
+  for (int i = 0; i < 64 / kRows; ++i) {
+    const int r = i * kRows + threadIdx.x / kLanes, t = min(t0 + r / 4, seq - 1), h = min(h0 + r % 4, n_heads - 1);
+    const x8 x = *reinterpret_cast<const x8*>(o + b * os.b + t * os.s + h * os.h + 8 * lane);
+    const x8 y = *reinterpret_cast<const x8*>(dout + b * ds.b + t * ds.s + h * ds.h + 8 * lane);
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fmaf((float)x[j], (float)y[j], sum);
+#pragma unroll
+    for (int d = kLanes / 2; d; d /= 2) sum += __shfl_xor(sum, d);
+    if (lane == 0) sums[r / 4][r % 4] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int t = t0 + threadIdx.x % 16, h = h0 + threadIdx.x / 16;
+    if (t < seq && h < n_heads) delta[((int64_t)b * n_heads + h) * seq + t] = sums[threadIdx.x % 16][threadIdx.x / 16];
+  }
+}
+
+// Sums of fp32 parts, part i at parts + i * part, contiguous [batch * heads, tokens, kD], into the first `tokens` rows of a strided result.
+struct SwaSum {
+  const float* parts; void* out;
+  int64_t part;
+  Strides3 os;
+  int n_parts, tokens, part_tokens, heads, n_rows, n_groups;     // part_tokens: rows of a head in the parts
+  Div by_tokens, by_heads;
+};
+struct SwaSums { SwaSum s[3]; };
+template <class T, int kD>
+__global__ __launch_bounds__(256) void swa_sum_kernel(const SwaSums all) {
+  int block = blockIdx.x, which = 0;
+  if (block >= all.s[0].n_groups) { block -= all.s[0].n_groups; which = 1; }
+  if (which == 1 && block >= all.s[1].n_groups) { block -= all.s[1].n_groups; which = 2; }
+  const SwaSum& x = all.s[which];
+  constexpr int kPer = kD / 16;
+  const int row = block * 16 + (threadIdx.x >> 4), c = threadIdx.x & 15;
+  if (row >= x.n_rows) return;
+  const int bh = quotient(row, x.by_tokens), t = row - bh * x.tokens, b = quotient(bh, x.by_heads), h = bh - b * x.heads;
+  const float* from = x.parts + ((int64_t)bh * x.part_tokens + t) * kD + c * kPer;
+  float acc[kPer] = {};
+  for (int i = 0; i < x.n_parts; ++i)
+#pragma unroll
+    for (int j = 0; j < kPer; j += 4) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(from + i * x.part + j);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) acc[j + n] += y[n];
+    }
+  typedef __attribute__((ext_vector_type(kPer))) T vec;
+  vec w;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) w[j] = (T)acc[j];
+  *reinterpret_cast<vec*>((T*)x.out + b * x.os.b + t * x.os.s + h * x.os.h + c * kPer) = w;
+}
+
+// How a backward is cut, and where its parts lie in the workspace (bytes).
+struct BwdCut {
+  int row_parts, n_cut, col_parts;
+  int64_t dq_bytes, col_bytes, total;             // of a part; of a part's dK
+};
+static BwdCut bwd_cut(const SwaParams& p, int head_dim) {
+  // Steps of 64 rows: of a row tile, of a column, of a column of the sinks (the longest); a column's has four products and a row's three.
+  const int64_t q_blocks = (p.seq_q + kSwaBlock - 1) / kSwaBlock, k_blocks = (p.seq_k + kSwaBlock - 1) / kSwaBlock;
+  const int64_t window = p.hi >= kFar || p.lo <= -kFar ? INT32_MAX : std::max<int64_t>(((int64_t)p.hi - p.lo + kSwaRows + 2 * kSwaBlock - 1) / kSwaBlock, 1);
+  const int64_t col = std::min(window, q_blocks) * p.group, sink_col = q_blocks * p.group, row = std::min(window + (p.sinks + kSwaBlock - 1) / kSwaBlock, k_blocks);
+  const int64_t cols = (int64_t)p.batch * p.n_kv_heads * p.n_ktiles, rows = (int64_t)p.batch * p.n_heads * p.n_qtiles;
+  const int64_t sink_tiles = p.sinks ? (p.sinks + kSwaRows - 1) / kSwaRows : 0;
+  BwdCut c{1, 0, 1, 0, 0, 0};
+  if (cols == 0 || rows == 0) return c;
+  const int64_t work = 4 * cols * col + 3 * rows * row;
+  const int64_t each = std::max<int64_t>(work / kDenseTargetGroups, 32);       // products of a workgroup, where there are few
+  auto parts = [&](int64_t steps) { return (int)std::min<int64_t>((steps + each - 1) / each, UA_MAX_PARTS); };
+  if (cols + rows < kDenseFullLaunch) {
+    c.row_parts = parts(3 * row);
+    c.col_parts = parts(4 * col);
+    if (c.col_parts > 1) c.n_cut = p.n_ktiles;
+  }
+  // the sinks' columns: parts of the other columns' length
+  if (sink_tiles && c.n_cut == 0 && sink_col > 2 * col) {
+    c.n_cut = (int)std::min<int64_t>(sink_tiles, p.n_ktiles);
+    c.col_parts = (int)std::min<int64_t>((sink_col + col - 1) / col, UA_MAX_PARTS);
+  }
+  if (c.row_parts > 1) c.dq_bytes = align256((int64_t)p.batch * p.n_heads * p.seq_q * head_dim * 4);
+  if (c.n_cut) c.col_bytes = align256((int64_t)p.batch * p.n_kv_heads * c.n_cut * kSwaRows * head_dim * 4);
+  c.total = (c.row_parts > 1 ? c.row_parts * c.dq_bytes : 0) + 2 * c.col_parts * c.col_bytes;
+  return c;
+}
+
+template <class T, int kD>
+static int bwd_run(const SwaParams& p, unsigned n, const SwaSums& sums, hipStream_t st) {
+  if (n) swa_bwd_kernel<T, kD><<<n, 256, 0, st>>>(p);
+  if (hipGetLastError() != hipSuccess) return UA_ERR_LAUNCH;
+  const int groups = sums.s[0].n_groups + sums.s[1].n_groups + sums.s[2].n_groups;
+  if (groups) swa_sum_kernel<T, kD><<<groups, 256, 0, st>>>(sums);
+  return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
+}
+template <class T, int kD>
+static int delta_run(const void* o, const void* dout, float* delta, const int64_t* os, const int64_t* ds, int batch, int n_heads, int seq, hipStream_t st) {
+  const int tokens = (seq + 15) / 16, heads = (n_heads + 3) / 4;
+  swa_delta_kernel<T, kD><<<batch * tokens * heads, 256, 0, st>>>((const T*)o, (const T*)dout, delta, {os[0], os[1], os[2]}, {ds[0], ds[1], ds[2]}, n_heads, seq,
+                                                                   make_div(tokens), make_div(heads));
+  return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
+}
+
+}  // namespace ua
+
+extern "C" int ua_swa_bwd_delta(const void* o, const void* dout, float* delta, int batch, int n_heads, int seqlen_q, int head_dim, int dtype,
+                                const int64_t* o_strides, const int64_t* do_strides, void* stream) {
+  using namespace ua;
+  if (batch < 0 || n_heads <= 0 || seqlen_q < 0 || (int64_t)batch * ((seqlen_q + 15) / 16) * ((n_heads + 3) / 4) > INT32_MAX) return UA_ERR_SHAPE;
+  if ((head_dim != 64 && head_dim != 128) || (dtype != UA_BF16 && dtype != UA_FP16)) return UA_ERR_UNSUPPORTED;
+  if ((int64_t)batch * seqlen_q == 0) return UA_OK;
+  if (!o || !dout || !delta || !o_strides || !do_strides) return UA_ERR_NULL;
+  if (!aligned16(o) || !aligned16(dout) || !swa_strides_ok(o_strides, false) || !swa_strides_ok(do_strides, false)) return UA_ERR_ALIGN;
+  const int rc = check_device();
+  if (rc != UA_OK) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == UA_FP16) return head_dim == 64 ? delta_run<fp16, 64>(o, dout, delta, o_strides, do_strides, batch, n_heads, seqlen_q, st)
+                                              : delta_run<fp16, 128>(o, dout, delta, o_strides, do_strides, batch, n_heads, seqlen_q, st);
+  return head_dim == 64 ? delta_run<bf16, 64>(o, dout, delta, o_strides, do_strides, batch, n_heads, seqlen_q, st)
+                        : delta_run<bf16, 128>(o, dout, delta, o_strides, do_strides, batch, n_heads, seqlen_q, st);
+}
+
+extern "C" int64_t ua_swa_bwd_workspace_bytes(int batch, int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim, int64_t q_start,
+                                              int64_t k_start, int64_t left, int64_t right, int64_t sinks) {
+  using namespace ua;
+  SwaParams p{};
+  if (swa_fill(p, batch, n_heads, n_kv_heads, seqlen_q, seqlen_k, head_dim, UA_BF16, q_start, k_start, left, right, sinks, 1.f) != UA_OK) return 0;
+  return bwd_cut(p, head_dim).total;
+}
+
+extern "C" int ua_swa_bwd(const void* dout, const void* q, const void* k, const void* v, const float* lse, const float* delta, void* dq, void* dk, void* dv,
+                          int batch, int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim, int dtype, const int64_t* do_strides,
+                          const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* dq_strides,
+                          const int64_t* dk_strides, const int64_t* dv_strides, int64_t q_start, int64_t k_start, int64_t left, int64_t right, int64_t sinks,
+                          float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace ua;
+  SwaParams p{};
+  int rc = swa_fill(p, batch, n_heads, n_kv_heads, seqlen_q, seqlen_k, head_dim, dtype, q_start, k_start, left, right, sinks, softmax_scale);
+  if (rc != UA_OK) return rc;
+  const bool some_q = (int64_t)batch * seqlen_q > 0, some_k = (int64_t)batch * seqlen_k > 0;
+  if (!some_q && !some_k) return UA_OK;
+  for (const int64_t* s : {do_strides, q_strides, k_strides, v_strides, dq_strides, dk_strides, dv_strides})
+    if (!s) return UA_ERR_NULL;
+  if ((some_q && (!dout || !q || !lse || !delta || !dq)) || (some_k && (!k || !v || !dk || !dv))) return UA_ERR_NULL;
+  for (const void* x : {dout, q, k, v, (const void*)dq, (const void*)dk, (const void*)dv})
+    if (!aligned16(x)) return UA_ERR_ALIGN;
+  for (const int64_t* s : {do_strides, q_strides, k_strides, v_strides})
+    if (!swa_strides_ok(s, false)) return UA_ERR_ALIGN;
+  for (const int64_t* s : {dq_strides, dk_strides, dv_strides})
+    if (!swa_strides_ok(s, true)) return UA_ERR_ALIGN;
+  for (const int64_t* s : {do_strides, q_strides, k_strides, v_strides})
+    if (s[1] > (INT32_MAX >> 9)) return UA_ERR_SHAPE;
+  rc = check_device();
+  if (rc != UA_OK) return rc;
+  auto three = [](const int64_t* s) { return Strides3{s[0], s[1], s[2]}; };
+  p.dout = dout; p.q = q; p.k = k; p.v = v; p.lse = const_cast<float*>(lse); p.delta = const_cast<float*>(delta);
+  p.dq = dq; p.dk = dk; p.dv = dv;
+  p.ds = three(do_strides); p.qs = three(q_strides); p.ks = three(k_strides); p.vs = three(v_strides);
+  p.dqs = three(dq_strides); p.dks = three(dk_strides); p.dvs = three(dv_strides);
+  BwdCut cut = bwd_cut(p, head_dim);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < cut.total) cut = BwdCut{1, 0, 1, 0, 0, 0};
+  p.n_parts = cut.row_parts;
+  p.n_cut = cut.n_cut;
+  p.col_parts = cut.col_parts;
+  char* at = (char*)workspace;
+  p.part_dk = (float*)at;
+  p.part_dv = (float*)(at + cut.col_parts * cut.col_bytes);
+  p.col_part = cut.col_bytes / 4;
+  p.part_o = (float*)(at + 2 * cut.col_parts * cut.col_bytes);
+  p.o_part = cut.dq_bytes / 4;
+  const int col_heads = batch * n_kv_heads;
+  p.by_parts = make_div(p.n_parts);
+  p.by_cols = make_div(std::max(col_heads, 1));
+  p.by_cut = make_div(std::max(p.n_cut, 1));
+  p.n_cut_blocks = col_heads * p.n_cut * p.col_parts;
+  p.n_col_blocks = p.n_cut_blocks + col_heads * (p.n_ktiles - p.n_cut);
+  p.cols = block_map(std::max(col_heads, 1), std::max(p.n_ktiles - p.n_cut, 1));
+  p.map = block_map(batch * n_heads, std::max(p.n_qtiles * p.n_parts, 1));
+  const unsigned n = (unsigned)(p.n_col_blocks + batch * n_heads * p.n_qtiles * p.n_parts);
+  SwaSums sums{};
+  auto sum = [&](int i, const float* parts, int64_t part, int n_parts, void* out, const Strides3& os, int tokens, int part_tokens, int heads) {
+    const int rows = batch * heads * tokens;
+    sums.s[i] = {parts, out, part, os, n_parts, tokens, part_tokens, heads, rows, (rows + 15) / 16, make_div(std::max(tokens, 1)), make_div(heads)};
+  };
+  if (p.n_cut) {
+    const int tokens = std::min(p.n_cut * kSwaRows, seqlen_k);
+    sum(0, p.part_dk, p.col_part, p.col_parts, dk, p.dks, tokens, p.n_cut * kSwaRows, n_kv_heads);
+    sum(1, p.part_dv, p.col_part, p.col_parts, dv, p.dvs, tokens, p.n_cut * kSwaRows, n_kv_heads);
+  }
+  if (p.n_parts > 1) sum(2, p.part_o, p.o_part, p.n_parts, dq, p.dqs, seqlen_q, seqlen_q, n_heads);
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == UA_FP16) return head_dim == 64 ? bwd_run<fp16, 64>(p, n, sums, st) : bwd_run<fp16, 128>(p, n, sums, st);
+  return head_dim == 64 ? bwd_run<bf16, 64>(p, n, sums, st) : bwd_run<bf16, 128>(p, n, sums, st);
+}

@@ -34,7 +34,9 @@ __global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
 
   const SwaWalk walk(r0, min(r0 + kSwaRows, p.seq_q) - 1, p.hi, p.lo, p.sinks, p.seq_k);
   const int part_len = (walk.n + p.n_parts - 1) / p.n_parts, i0 = min(part * part_len, walk.n), i1 = min(i0 + part_len, walk.n);
-  SwaStream<kD, false, true> in((const T*)p.k + b * p.ks.b + hk * p.ks.h, p.ks.s, (const T*)p.v + b * p.vs.b + hk * p.vs.h, p.vs.s, wave, lane);
+  typedef SwaStream<kD, kN, kT> Stream;
+  Stream in(p.ks.s, p.vs.s, wave, lane);
+  in.of((const T*)p.k + b * p.ks.b + hk * p.ks.h, (const T*)p.v + b * p.vs.b + hk * p.vs.h);
   if (i0 < i1) {
     in.block(walk.at(i0) * kSwaBlock, p.seq_k, true);
 #pragma unroll
@@ -59,7 +61,7 @@ __global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
 #pragma unroll
   for (int i = 0; i < H::kSteps; ++i) nat[i] = H::at_n(lane & 31, 2 * i + (lane >> 5));
 #pragma unroll
-  for (int m = 0; m < H::kBlocks; ++m) tr[m] = H::kTile + H::tr_offset(lane, m);
+  for (int m = 0; m < H::kBlocks; ++m) tr[m] = Stream::kSecond + H::tr_offset(lane, m);
 
   auto step = [&](int i, auto stage_tag) {
     constexpr int kStage = decltype(stage_tag)::value;
@@ -91,7 +93,7 @@ __global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         if (n & 1) in.copy(n >> 1, other);
       }
-      static_assert(kAll / 2 == SwaStream<kD, false, true>::kPieces, "a copy after every other product");
+      static_assert(kAll / 2 == Stream::kPieces, "a copy after every other product");
     }
     const bool whole = key0 + kSwaBlock - 1 <= min(row0 + p.hi, p.seq_k - 1) && (key0 >= row0 + 31 + p.lo || key0 + kSwaBlock <= p.sinks);
     if (!whole) {

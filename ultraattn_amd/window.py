@@ -23,3 +23,13 @@ def swa_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Tuple[int
     """Forward -> (out, lse).  The default window is causal attention, aligned at the last key; ``softmax_scale`` is 1 / sqrt(D)."""
     left, right = window
     return native().swa_forward(q, k, v, left, right, sinks, q_start, k_start, softmax_scale, out, lse)
+
+
+def swa_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[torch.Tensor], lse: torch.Tensor,
+            window: Tuple[int, int] = (-1, 0), sinks: int = 0, softmax_scale: Optional[float] = None, q_start: Optional[int] = None, k_start: int = 0,
+            dq: Optional[torch.Tensor] = None, dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None,
+            softmax_d: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Backward -> (dq, dk, dv), with the arguments of the forward.  ``lse`` and ``softmax_d`` (rowsum(dout * out), as ``bsa_bwd`` takes it; then
+    ``out`` is ignored) are the rows' global statistics; dk and dv are summed over the query heads of a key head.  The same call gives the same bits."""
+    left, right = window
+    return native().swa_backward(dout, q, k, v, out, lse, dq, dk, dv, softmax_d, left, right, sinks, q_start, k_start, softmax_scale)
