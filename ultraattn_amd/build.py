@@ -4,6 +4,7 @@ and the Python binding ``csrc/native.cpp`` into ``_native.so`` next to this file
 import os
 import subprocess
 import sys
+import time
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
@@ -51,16 +52,17 @@ def build_library(verbose: bool = False, jobs: int = 4) -> str:
         cmd = [hipcc_path(), *HIPCC_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
-        procs.append((src, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
-        while sum(p.poll() is None for _, _, p in procs) >= jobs:
-            for _, _, p in procs:
-                if p.poll() is None:
-                    p.wait()
-                    break
+        # (a file, not a pipe: a compiler whose warnings fill a pipe that nobody reads yet would wait for ever)
+        log = open(obj + ".log", "w+")
+        procs.append((src, obj, log, subprocess.Popen(cmd, stdout=log, stderr=subprocess.STDOUT, text=True)))
+        while sum(p.poll() is None for *_, p in procs) >= jobs:
+            time.sleep(0.05)
     objs = []
-    for src, obj, p in procs:
-        out, _ = p.communicate()
-        out = "\n".join(l for l in out.splitlines() if "packed-fp32-ops" not in l)
+    for src, obj, log, p in procs:
+        p.wait()
+        with log:
+            log.seek(0)
+            out = "\n".join(l for l in log.read().splitlines() if "packed-fp32-ops" not in l)
         if p.returncode != 0:
             raise RuntimeError(f"hipcc failed on {src}:\n{out}")
         if verbose and out.strip():
