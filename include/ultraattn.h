@@ -373,6 +373,19 @@ int ua_swa_bwd(const void *dout, const void *q, const void *k, const void *v, co
                int64_t q_start, int64_t k_start, int64_t left, int64_t right, int64_t sinks, float softmax_scale,
                void *workspace, int64_t workspace_bytes, void *stream);
 
+/* A few new tokens of every sequence against its cache: q, o [batch, n_tokens, n_heads, head_dim]; caches [batch, room, n_kv_heads, head_dim] that hold
+ * the new tokens' keys and values already (ua_rope_append); lens DEVICE int32 [batch], the lengths WITH the new tokens, up to 2^29 (shorter
+ * than 0 is 0; of a length beyond `room` the keys that the cache has count).  Token t of sequence b is at position lens[b] - n_tokens + t and sees
+ * the keys up to its own position, with left >= 0 those at most `left` behind it and the first `sinks`; a token before
+ * position 0 sees none (o = 0, lse = -inf).  Nothing behind lens[b] is read.  lse [batch, n_heads, n_tokens].  Types, strides and alignment as above.
+ * Long caches are cut into parts of workgroups of their own if `workspace` holds ua_swa_decode_workspace_bytes(), which does not depend on
+ * lens: a captured call serves all lengths. */
+int64_t ua_swa_decode_workspace_bytes(int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int head_dim, int64_t left, int64_t sinks);
+int ua_swa_decode(const void *q, const void *k_cache, const void *v_cache, void *o, float *lse, const int32_t *lens,
+                  int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int head_dim, int dtype,
+                  const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides, const int64_t *o_strides,
+                  int64_t left, int64_t sinks, float softmax_scale, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,6 +45,8 @@ SIGNATURES = {
     "ua_swa_bwd_delta": (c_int, [c_void_p] * 3 + [c_int] * 5 + [_i64p] * 2 + [c_void_p]),
     "ua_swa_bwd_workspace_bytes": (c_int64, [c_int] * 6 + [c_int64] * 5),
     "ua_swa_bwd": (c_int, [c_void_p] * 9 + [c_int] * 7 + [_i64p] * 7 + [c_int64] * 5 + [c_float, c_void_p, c_int64, c_void_p]),
+    "ua_swa_decode_workspace_bytes": (c_int64, [c_int] * 6 + [c_int64] * 2),
+    "ua_swa_decode": (c_int, [c_void_p] * 6 + [c_int] * 7 + [_i64p] * 4 + [c_int64] * 2 + [c_float, c_void_p, c_int64, c_void_p]),
     "ua_copy_in": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }
 

@@ -881,6 +881,31 @@ PyObject* swa_backward(PyObject* const* a) {
   return tuple_of(dq, dk, dv);
 }
 
+// swa_decode(q, k_cache, v_cache, lens, left, sinks, softmax_scale, out, lse) -> (out, lse)
+PyObject* swa_decode(PyObject* const* a) {
+  const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k_cache"), &v = tensor(a[2], "v_cache");
+  check_swa(q, k, v, "k_cache", "v_cache");
+  const int dt = dtype_code("q", q, false);
+  const int32_t* lens = lengths(tensor(a[3], "lens"), q);
+  const int64_t left = integer(a[4]), sinks = integer(a[5]);
+  if (left < -1) fail(PyExc_ValueError, "window must be -1 (no bound) or a number of keys");
+  if (sinks < 0) fail(PyExc_ValueError, "sinks must be a number of keys");
+  const float scale = swa_scale(a[6], q.size(3));
+  Slot out(a[7]), lse(a[8]);
+  result(out, "out", q);
+  if (lse.given) check_lse("lse", lse.t = tensor(lse.given, "lse"), q);
+  else lse.t = stat_of(q);
+  const On on(q);
+  const int B = (int)q.size(0), T = (int)q.size(1), H = (int)q.size(2), Hk = (int)k.size(2), room = (int)k.size(1), D = (int)q.size(3);
+  const at::Tensor ws = scratch(ua_swa_decode_workspace_bytes(B, T, H, Hk, room, D, left, sinks), q);
+  call("ua_swa_decode", [&] {
+    return ua_swa_decode(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.t.data_ptr(), (float*)lse.t.data_ptr(), lens, B, T, H, Hk, room, D, dt, used_strides(q),
+                         used_strides(k), used_strides(v), used_strides(out.t), left, sinks, scale, ws.defined() ? ws.data_ptr() : nullptr,
+                         ws.defined() ? ws.numel() : 0, on.stream);
+  });
+  return tuple_of(out, lse);
+}
+
 // ---- module ---------------------------------------------------------------------------------------------
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -906,7 +931,7 @@ PyMethodDef methods[] = {
     UA_METHOD(dense_forward, 8), UA_METHOD(dense_backward, 14), UA_METHOD(bsa_forward, 10), UA_METHOD(bsa_backward, 15),
     UA_METHOD(delta, 3), UA_METHOD(grad_accumulate, 4), UA_METHOD(merge, 4), UA_METHOD(grad_sum, 3),
     UA_METHOD(merge_update, 5), UA_METHOD(permute_cols, 6), UA_METHOD(lists_from_mask, 5),
-    UA_METHOD(build_lists_device, 3), UA_METHOD(rope, 10), UA_METHOD(rope_append, 10), UA_METHOD(swa_forward, 11), UA_METHOD(swa_backward, 16),
+    UA_METHOD(build_lists_device, 3), UA_METHOD(rope, 10), UA_METHOD(rope_append, 10), UA_METHOD(swa_forward, 11), UA_METHOD(swa_backward, 16), UA_METHOD(swa_decode, 9),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "Native host side of the attention operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -33,3 +33,14 @@ def swa_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     ``out`` is ignored) are the rows' global statistics; dk and dv are summed over the query heads of a key head.  The same call gives the same bits."""
     left, right = window
     return native().swa_backward(dout, q, k, v, out, lse, dq, dk, dv, softmax_d, left, right, sinks, q_start, k_start, softmax_scale)
+
+
+def swa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lens: torch.Tensor, window: int = -1, sinks: int = 0,
+               softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+               lse: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """T new tokens of every sequence, q ``[B, T, Hq, D]``, against the caches ``[B, room, Hk, D]`` that hold them already -> (out, lse).
+
+    ``lens`` (int32 ``[B]`` on the device) counts the new tokens: token t of sequence b is at position ``lens[b] - T + t`` and sees the keys up to
+    itself, at most ``window`` behind it (-1: all) and the first ``sinks``.  A token before position 0 sees nothing.  What lies behind ``lens[b]`` in the
+    caches is not read.  Meant for few tokens (a step's one, or several proposed ones); a prompt's go through ``swa_fwd``."""
+    return native().swa_decode(q, k_cache, v_cache, lens, window, sinks, softmax_scale, out, lse)
