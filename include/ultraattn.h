@@ -356,13 +356,16 @@ int ua_swa_fwd(const void *q, const void *k, const void *v, void *o, float *lse,
                void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Gradients, with the same arguments; lse and delta are the rows' global statistics (of all shards).  ua_swa_bwd_delta: delta =
- * rowsum(dout * o), fp32 [batch, n_heads, seqlen_q].  dq, dk and dv are overwritten; dk and dv are the sums over the query heads that share a key
+ * rowsum(dout * o), fp32 [batch, n_heads, seqlen_q]; rows of up to 8 keys, where o's rounding counts most, take o from q, k and v again
+ * if lse is that of these keys alone.  dq, dk and dv are overwritten; dk and dv are the sums over the query heads that share a key
  * head.  Nothing is added atomically: the same call gives the same bits.  P and dS are rounded to dtype for their products; in fp16 dS below 6e-5
  * loses bits, so scale the loss as with any fp16 gradient.
  * Few long walks, and those of the sinks' columns, which all later queries see, are cut into parts if `workspace` holds
  * ua_swa_bwd_workspace_bytes(). */
-int ua_swa_bwd_delta(const void *o, const void *dout, float *delta, int batch, int n_heads, int seqlen_q, int head_dim, int dtype,
-                     const int64_t *o_strides, const int64_t *do_strides, void *stream);
+int ua_swa_bwd_delta(const void *o, const void *dout, const void *q, const void *k, const void *v, const float *lse, float *delta,
+                     int batch, int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim, int dtype,
+                     const int64_t *o_strides, const int64_t *do_strides, const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides,
+                     int64_t q_start, int64_t k_start, int64_t left, int64_t right, int64_t sinks, float softmax_scale, void *stream);
 int64_t ua_swa_bwd_workspace_bytes(int batch, int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim,
                                    int64_t q_start, int64_t k_start, int64_t left, int64_t right, int64_t sinks);
 int ua_swa_bwd(const void *dout, const void *q, const void *k, const void *v, const float *lse, const float *delta,

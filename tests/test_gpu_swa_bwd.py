@@ -101,6 +101,36 @@ def test_softmax_d_given():
     Reference(q, k, v, visible(200, 200, (33, 0), 2), dout=do).check(dq=got[0], dk=got[1], dv=got[2])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_delta_of_rows_of_few_keys_is_not_the_rounded_output_s(dtype, dim):
+    """Rows of up to 8 keys: dS must not carry the rounding of O.  In a row of one key dS = dP - delta = 0, so dQ is what is left of it."""
+    q, k, v, do = inputs(2, 400, 300, 6, 3, dim, dtype)
+    for window, sinks, start in (((0, 0), 0, None), ((0, 0), 1, -50), ((7, 0), 3, 100)):
+        out, lse = ua.swa_fwd(q, k, v, window, sinks, None, start)
+        dq = ua.swa_bwd(do, q, k, v, out, lse, window, sinks, None, start)[0]
+        n = visible(400, 300, window, sinks, start).sum(-1)
+        one = (n == 1).nonzero()[:, 0]
+        if window[0] == 0:
+            # |dP - delta| is the difference of two dot products in 32 bits, each off by (dim + 4) 2^-24 of its terms' sum, and of P = 1 by 2^-20
+            K = k.double().repeat_interleave(2, dim=2)
+            terms = (do.double().abs().sum(-1) * v.double().abs().max())[:, one]
+            assert (dq.double()[:, one].abs().amax(-1) <= dim ** -0.5 * (2 * (dim + 4) * 2.0 ** -24 + 2.0 ** -20) * terms * K.abs().max()).all()
+            assert len(one) >= 50
+
+
+def test_delta_of_a_shard_takes_the_whole_rows_output():
+    """A shard in which rows have few keys, statistics of the whole: delta must not be made of the shard's keys."""
+    q, k, v, do = inputs(1, 64, 300, 2, 2, 128, torch.bfloat16)
+    out, lse = ua.swa_fwd(q, k, v, (299, 0), q_start=290)
+    ref = Reference(q, k, v, visible(64, 300, (299, 0), 0, 290), dout=do)
+    ref.check(out=out, lse=lse)
+    parts = [ua.swa_bwd(do, q, k[:, i:j].contiguous(), v[:, i:j].contiguous(), out, lse, (299, 0), q_start=290, k_start=i) for i, j in ((0, 290), (290, 300))]
+    for b in ("dq_bound", "dk_bound", "dv_bound"):
+        setattr(ref, b, 3 * getattr(ref, b))                          # dq is rounded in either part and once more
+    ref.check(dq=ua.grad_sum([g[0] for g in parts]), dk=torch.cat([g[1] for g in parts], 1), dv=torch.cat([g[2] for g in parts], 1))
+
+
 @pytest.mark.parametrize("window,sinks,q_start", [((10, 0), 2, None), ((5, 5), 0, 3)])
 def test_against_differences(window, sinks, q_start):
     """The directional derivative of sum(out * do), by central differences of the definition in 64 bits, at the same inputs."""

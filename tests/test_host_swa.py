@@ -37,10 +37,11 @@ def test_backward_refuses(lib):
     for i, x, rc in ((14, 32, -3), (15, 2, -3), (28, -0.1, -3), (10, 5, -2), (12, -1, -2), (0, BUF + 4, -4), (16, BAD, -4), (20, NONE, -4)):
         assert lib.ua_swa_bwd(*ok[:i], x, *ok[i + 1:]) == rc, i
     assert lib.ua_swa_bwd(*ok[:9], 0, *ok[10:]) == 0
-    delta = [BUF, BUF, BUF, 1, 4, 16, 64, 0, S, S, None]
-    for i in (0, 1, 2, 8, 9):
+    delta = [BUF] * 7 + [1, 4, 2, 16, 16, 64, 0] + [S] * 5 + [0, 0, -1, 0, 0, 0.1, None]
+    for i in list(range(7)) + list(range(14, 19)):
         assert lib.ua_swa_bwd_delta(*delta[:i], None, *delta[i + 1:]) == -1
-    assert lib.ua_swa_bwd_delta(*delta[:6], 80, *delta[7:]) == -3 and lib.ua_swa_bwd_delta(*delta[:5], 0, *delta[6:]) == 0
+    assert lib.ua_swa_bwd_delta(*delta[:12], 80, *delta[13:]) == -3 and lib.ua_swa_bwd_delta(*delta[:10], 0, *delta[11:]) == 0
+    assert lib.ua_swa_bwd_delta(*delta[:2], BUF + 2, *delta[3:]) == -4
 
 
 def test_decode_refuses(lib):

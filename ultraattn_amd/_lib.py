@@ -42,7 +42,7 @@ SIGNATURES = {
     "ua_rope_append": (c_int, [c_void_p] * 8 + [c_int] * 9 + [c_float] + [_i64p] * 6 + [c_void_p]),
     "ua_swa_workspace_bytes": (c_int64, [c_int] * 6 + [c_int64] * 5),
     "ua_swa_fwd": (c_int, [c_void_p] * 5 + [c_int] * 7 + [_i64p] * 4 + [c_int64] * 5 + [c_float, c_void_p, c_int64, c_void_p]),
-    "ua_swa_bwd_delta": (c_int, [c_void_p] * 3 + [c_int] * 5 + [_i64p] * 2 + [c_void_p]),
+    "ua_swa_bwd_delta": (c_int, [c_void_p] * 7 + [c_int] * 7 + [_i64p] * 5 + [c_int64] * 5 + [c_float, c_void_p]),
     "ua_swa_bwd_workspace_bytes": (c_int64, [c_int] * 6 + [c_int64] * 5),
     "ua_swa_bwd": (c_int, [c_void_p] * 9 + [c_int] * 7 + [_i64p] * 7 + [c_int64] * 5 + [c_float, c_void_p, c_int64, c_void_p]),
     "ua_swa_decode_workspace_bytes": (c_int64, [c_int] * 6 + [c_int64] * 2),

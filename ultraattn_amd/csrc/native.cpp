@@ -868,7 +868,9 @@ PyObject* swa_backward(PyObject* const* a) {
     check_shape("out", out, q.sizes());
     delta = stat_of(q);
     call("ua_swa_bwd_delta", [&] {
-      return ua_swa_bwd_delta(out.data_ptr(), dout.data_ptr(), (float*)delta.data_ptr(), B, H, sq, D, dt, used_strides(out), used_strides(dout), on.stream);
+      return ua_swa_bwd_delta(out.data_ptr(), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), (const float*)lse.data_ptr(),
+                              (float*)delta.data_ptr(), B, H, Hk, sq, sk, D, dt, used_strides(out), used_strides(dout), used_strides(q), used_strides(k),
+                              used_strides(v), w.q_start, w.k_start, w.left, w.right, w.sinks, scale, on.stream);
     });
   }
   const at::Tensor ws = scratch(ua_swa_bwd_workspace_bytes(B, H, Hk, sq, sk, D, w.q_start, w.k_start, w.left, w.right, w.sinks), q);

@@ -406,30 +406,77 @@ __global__ __launch_bounds__(256, 2) void swa_bwd_kernel(const SwaParams p) {
 }
 
 // delta = rowsum(dO * O).  16 tokens of 4 heads a workgroup: memory sees rows of 4 heads, and 64 bytes of each head's result.
+//
+// O was rounded by half a step, u.  In a row of n keys that moves delta by about u |dO| / sqrt(n), while dP - delta is about |dO|: for
+// few keys as much as the rounding of dS, and such rows have the largest gradients (1333 queries that run out of their keys, fp16: dQ off by
+// 3.1e-4, 3.0e-4 without it).  So rows of up to kFewKeys keys make their O again, unrounded, if their LSE is that of these keys alone (of a shard it
+// is not).  All keys' loads are in flight at once, and a thread has one row: such rows one after the other, in four iterations of four keys, took 15 us.
+constexpr int kFewKeys = 8;
+// The sum over the 8 or 16 lanes of a row, in each of them.
+template <int kLanes>
+__device__ __forceinline__ float row_sum(float x) {
+  auto from = [](float y, auto ctrl) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(y), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  x += from(x, std::integral_constant<int, 0xb1>{});         // neighbours
+  x += from(x, std::integral_constant<int, 0x4e>{});         // pairs
+  x += from(x, std::integral_constant<int, 0x141>{});        // mirrored in 8 lanes
+  if (kLanes == 16) x += from(x, std::integral_constant<int, 0x140>{});        // in 16
+  return x;
+}
 template <class T, int kD>
-__global__ __launch_bounds__(256) void swa_delta_kernel(const T* o, const T* dout, float* delta, Strides3 os, Strides3 ds, int n_heads, int seq, Div by_tokens,
-                                                        Div by_heads) {
-  constexpr int kLanes = kD / 8, kRows = 256 / kLanes;
+__global__ __launch_bounds__(8 * kD) void swa_delta_kernel(const SwaParams p) {
+  constexpr int kLanes = kD / 8;
   typedef typename SwaVec<T>::x8 x8;
   __shared__ float sums[16][4];
-  const int th = quotient(blockIdx.x, by_heads), hb = blockIdx.x - th * by_heads.d, b = quotient(th, by_tokens), t0 = (th - b * by_tokens.d) * 16, h0 = 4 * hb;
-  const int lane = threadIdx.x % kLanes;
+  const int th = quotient(blockIdx.x, p.by_cut), hb = blockIdx.x - th * p.by_cut.d, b = quotient(th, p.by_parts), t0 = (th - b * p.by_parts.d) * 16, h0 = 4 * hb;
+  const int lane = threadIdx.x % kLanes, r = threadIdx.x / kLanes, t = min(t0 + r / 4, p.seq_q - 1), h = min(h0 + r % 4, p.n_heads - 1);
+  const x8 x = *reinterpret_cast<const x8*>((const T*)p.o + b * p.os.b + t * p.os.s + h * p.os.h + 8 * lane);
+  const x8 y = *reinterpret_cast<const x8*>((const T*)p.dout + b * p.ds.b + t * p.ds.s + h * p.ds.h + 8 * lane);
+  float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 64 / kRows; ++i) {
-    const int r = i * kRows + threadIdx.x / kLanes, t = min(t0 + r / 4, seq - 1), h = min(h0 + r % 4, n_heads - 1);
-    const x8 x = *reinterpret_cast<const x8*>(o + b * os.b + t * os.s + h * os.h + 8 * lane);
-    const x8 y = *reinterpret_cast<const x8*>(dout + b * ds.b + t * ds.s + h * ds.h + 8 * lane);
-    float sum = 0.f;
+  for (int j = 0; j < 8; ++j) sum = fmaf((float)x[j], (float)y[j], sum);
+  sum = row_sum<kLanes>(sum);
+  const int last = min(t + p.hi, p.seq_k - 1), first = max(t + p.lo, 0), sinks = max(min(min(p.sinks, last + 1), first), 0);
+  const int n = max(last - first + 1, 0) + sinks;
+  if (n > 0 && n <= kFewKeys) {                            // the same for all lanes of a row
+    const int hk = quotient(h, p.by_group);
+    const T* k = (const T*)p.k + b * p.ks.b + hk * p.ks.h + 8 * lane;
+    const T* v = (const T*)p.v + b * p.vs.b + hk * p.vs.h + 8 * lane;
+    x8 kr[kFewKeys], vr[kFewKeys];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fmaf((float)x[j], (float)y[j], sum);
+    for (int m = 0; m < kFewKeys; ++m) {
+      const int j = min(m, n - 1);
+      const int64_t key = j < sinks ? j : first + j - sinks;
+      kr[m] = *reinterpret_cast<const x8*>(k + key * p.ks.s);
+      vr[m] = *reinterpret_cast<const x8*>(v + key * p.vs.s);
+    }
+    const x8 q = *reinterpret_cast<const x8*>((const T*)p.q + b * p.qs.b + t * p.qs.s + h * p.qs.h + 8 * lane);
+    const float lse2 = p.lse[((int64_t)b * p.n_heads + h) * p.seq_q + t] * kLog2e;
+    float mass = 0.f, again = 0.f;
 #pragma unroll
-    for (int d = kLanes / 2; d; d /= 2) sum += __shfl_xor(sum, d);
-    if (lane == 0) sums[r / 4][r % 4] = sum;
+    for (int m = 0; m < kFewKeys; ++m) {
+      float s = 0.f, dp = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s = fmaf((float)q[j], (float)kr[m][j], s);
+        dp = fmaf((float)y[j], (float)vr[m][j], dp);
+      }
+      s = row_sum<kLanes>(s);
+      dp = row_sum<kLanes>(dp);
+      if (m < n) {
+        const float e = fast_exp2(fmaf(s, p.scale_log2, -lse2));
+        mass += e;
+        again = fmaf(e, dp, again);
+      }
+    }
+    if (fabsf(mass - 1.f) < 1.f / 16384.f) sum = again;
   }
+  if (lane == 0) sums[r / 4][r % 4] = sum;
   __syncthreads();
   if (threadIdx.x < 64) {
-    const int t = t0 + threadIdx.x % 16, h = h0 + threadIdx.x / 16;
-    if (t < seq && h < n_heads) delta[((int64_t)b * n_heads + h) * seq + t] = sums[threadIdx.x % 16][threadIdx.x / 16];
+    const int ts = t0 + threadIdx.x % 16, hs = h0 + threadIdx.x / 16;
+    if (ts < p.seq_q && hs < p.n_heads) p.delta[((int64_t)b * p.n_heads + hs) * p.seq_q + ts] = sums[threadIdx.x % 16][threadIdx.x / 16];
   }
 }
 
@@ -509,31 +556,43 @@ static int bwd_run(const SwaParams& p, unsigned n, const SwaSums& sums, hipStrea
   if (groups) swa_sum_kernel<T, kD><<<groups, 256, 0, st>>>(sums);
   return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
 }
-template <class T, int kD>
-static int delta_run(const void* o, const void* dout, float* delta, const int64_t* os, const int64_t* ds, int batch, int n_heads, int seq, hipStream_t st) {
-  const int tokens = (seq + 15) / 16, heads = (n_heads + 3) / 4;
-  swa_delta_kernel<T, kD><<<batch * tokens * heads, 256, 0, st>>>((const T*)o, (const T*)dout, delta, {os[0], os[1], os[2]}, {ds[0], ds[1], ds[2]}, n_heads, seq,
-                                                                   make_div(tokens), make_div(heads));
-  return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
-}
-
 }  // namespace ua
 
-extern "C" int ua_swa_bwd_delta(const void* o, const void* dout, float* delta, int batch, int n_heads, int seqlen_q, int head_dim, int dtype,
-                                const int64_t* o_strides, const int64_t* do_strides, void* stream) {
+extern "C" int ua_swa_bwd_delta(const void* o, const void* dout, const void* q, const void* k, const void* v, const float* lse, float* delta, int batch,
+                                int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim, int dtype, const int64_t* o_strides,
+                                const int64_t* do_strides, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, int64_t q_start,
+                                int64_t k_start, int64_t left, int64_t right, int64_t sinks, float softmax_scale, void* stream) {
   using namespace ua;
-  if (batch < 0 || n_heads <= 0 || seqlen_q < 0 || (int64_t)batch * ((seqlen_q + 15) / 16) * ((n_heads + 3) / 4) > INT32_MAX) return UA_ERR_SHAPE;
-  if ((head_dim != 64 && head_dim != 128) || (dtype != UA_BF16 && dtype != UA_FP16)) return UA_ERR_UNSUPPORTED;
-  if ((int64_t)batch * seqlen_q == 0) return UA_OK;
-  if (!o || !dout || !delta || !o_strides || !do_strides) return UA_ERR_NULL;
-  if (!aligned16(o) || !aligned16(dout) || !swa_strides_ok(o_strides, false) || !swa_strides_ok(do_strides, false)) return UA_ERR_ALIGN;
-  const int rc = check_device();
+  SwaParams p{};
+  int rc = swa_fill(p, batch, n_heads, n_kv_heads, seqlen_q, seqlen_k, head_dim, dtype, q_start, k_start, left, right, sinks, softmax_scale);
   if (rc != UA_OK) return rc;
+  const int64_t tokens = (seqlen_q + 15) / 16, heads = (n_heads + 3) / 4;
+  if (batch * tokens * heads > INT32_MAX) return UA_ERR_SHAPE;
+  if ((int64_t)batch * seqlen_q == 0) return UA_OK;
+  if (!o || !dout || !q || !lse || !delta || (seqlen_k > 0 && (!k || !v))) return UA_ERR_NULL;
+  for (const int64_t* s : {o_strides, do_strides, q_strides, k_strides, v_strides}) {
+    if (!s) return UA_ERR_NULL;
+    if (!swa_strides_ok(s, false)) return UA_ERR_ALIGN;
+  }
+  for (const void* x : {o, dout, q, k, v})
+    if (!aligned16(x)) return UA_ERR_ALIGN;
+  rc = check_device();
+  if (rc != UA_OK) return rc;
+  auto three = [](const int64_t* s) { return Strides3{s[0], s[1], s[2]}; };
+  p.o = const_cast<void*>(o); p.dout = dout; p.q = q; p.k = k; p.v = v; p.lse = const_cast<float*>(lse); p.delta = delta;
+  p.os = three(o_strides); p.ds = three(do_strides); p.qs = three(q_strides); p.ks = three(k_strides); p.vs = three(v_strides);
+  p.by_cut = make_div((uint32_t)heads);
+  p.by_parts = make_div((uint32_t)tokens);
+  const unsigned n = (unsigned)(batch * tokens * heads);
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == UA_FP16) return head_dim == 64 ? delta_run<fp16, 64>(o, dout, delta, o_strides, do_strides, batch, n_heads, seqlen_q, st)
-                                              : delta_run<fp16, 128>(o, dout, delta, o_strides, do_strides, batch, n_heads, seqlen_q, st);
-  return head_dim == 64 ? delta_run<bf16, 64>(o, dout, delta, o_strides, do_strides, batch, n_heads, seqlen_q, st)
-                        : delta_run<bf16, 128>(o, dout, delta, o_strides, do_strides, batch, n_heads, seqlen_q, st);
+  if (dtype == UA_FP16) {
+    if (head_dim == 64) swa_delta_kernel<fp16, 64><<<n, 8 * 64, 0, st>>>(p);
+    else                swa_delta_kernel<fp16, 128><<<n, 8 * 128, 0, st>>>(p);
+  } else {
+    if (head_dim == 64) swa_delta_kernel<bf16, 64><<<n, 8 * 64, 0, st>>>(p);
+    else                swa_delta_kernel<bf16, 128><<<n, 8 * 128, 0, st>>>(p);
+  }
+  return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
 }
 
 extern "C" int64_t ua_swa_bwd_workspace_bytes(int batch, int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim, int64_t q_start,
