@@ -165,27 +165,39 @@ struct SwaStream {
   }
 };
 
+#define UA_BOTH __host__ __device__ __forceinline__
+UA_BOTH int imin(int a, int b) { return a < b ? a : b; }
+UA_BOTH int imax(int a, int b) { return a > b ? a : b; }
 // Blocks of 64 keys that a tile of rows r0 .. r1 walks: those of the sinks, then those of the window.
 struct SwaWalk {
   int n_sink, first, n;
-  __device__ __forceinline__ SwaWalk(int r0, int r1, int hi, int lo, int sinks, int n_keys) {
-    const int last = min(r1 + hi, n_keys - 1), start = max(r0 + lo, 0);
-    n_sink = last >= 0 ? (min(sinks, last + 1) + kSwaBlock - 1) / kSwaBlock : 0;
-    first = max(start / kSwaBlock, n_sink);
-    n = n_sink + (last >= start ? max(last / kSwaBlock + 1 - first, 0) : 0);
+  UA_BOTH SwaWalk(int r0, int r1, int hi, int lo, int sinks, int n_keys) {
+    const int last = imin(r1 + hi, n_keys - 1), start = imax(r0 + lo, 0);
+    n_sink = last >= 0 ? (imin(sinks, last + 1) + kSwaBlock - 1) / kSwaBlock : 0;
+    first = imax(start / kSwaBlock, n_sink);
+    n = n_sink + (last >= start ? imax(last / kSwaBlock + 1 - first, 0) : 0);
   }
   __device__ __forceinline__ int at(int i) const { return i < n_sink ? i : first + i - n_sink; }
 };
 // Blocks of 64 query rows, of one head, that see a tile of keys k0 .. k1.
 struct SwaColumn {
   int first, n;
-  __device__ __forceinline__ SwaColumn(int k0, int k1, int hi, int lo, int sinks, int n_rows) {
-    const int start = max(k0 - hi, 0), end = k0 < sinks ? n_rows - 1 : min(k1 - lo, n_rows - 1);
+  UA_BOTH SwaColumn(int k0, int k1, int hi, int lo, int sinks, int n_rows) {
+    const int start = imax(k0 - hi, 0), end = k0 < sinks ? n_rows - 1 : imin(k1 - lo, n_rows - 1);
     first = start / kSwaBlock;
     n = end >= start ? end / kSwaBlock + 1 - first : 0;
   }
 };
 
+// A run of a backward's columns, tiles first .. first + tiles - 1 of every key head, whose walks are cut into n_parts: with more than one part i
+// leaves fp32 rows, contiguous [batch, key heads, 128 * tiles, head_dim], at dk + i * part and dv + i * part.
+struct SwaColumns {
+  int first, tiles, n_parts, n_blocks;
+  float *dk, *dv;
+  int64_t part;
+  BlockMap map;
+  Div by_parts;
+};
 struct SwaParams {
   const void *q, *k, *v, *dout;
   void *o, *dq, *dk, *dv;
@@ -194,14 +206,30 @@ struct SwaParams {
   int batch, n_heads, n_kv_heads, group, seq_q, seq_k, hi, lo, sinks;
   float scale, scale_log2;
   // The rows' walks are cut into n_parts; part i leaves fp32 rows (and, forward, their lse), contiguous [batch, heads, tokens, head_dim], at part_o +
-  // i * o_part and part_lse + i * lse_part.  Backward: the first n_cut columns' walks are cut into col_parts, dK and dV alike.
-  int n_parts, n_cut, col_parts;
-  float *part_o, *part_lse, *part_dk, *part_dv;
-  int64_t o_part, lse_part, col_part;
-  BlockMap map, cols;
-  Div by_heads, by_kv_heads, by_group, by_parts, by_cols, by_cut;
-  int n_qtiles, n_ktiles, n_cut_blocks, n_col_blocks;
+  // i * o_part and part_lse + i * lse_part.  Backward: the columns of the sinks and the others are cut likewise, each into parts of their own.
+  int n_parts;
+  float *part_o, *part_lse;
+  int64_t o_part, lse_part;
+  SwaColumns cols[2];
+  BlockMap map;
+  Div by_heads, by_kv_heads, by_group, by_parts;
+  int n_qtiles, n_ktiles, n_col_blocks;
 };
+// Steps of 64 rows that the walks of a side take, the mean and the most (of up to 33 of its tiles, evenly spread).
+struct SwaSteps { double mean; int most; };
+template <class Of> SwaSteps swa_steps(int first, int n, Of of) {
+  SwaSteps s{0, 0};
+  const int m = n < 33 ? n : 33;
+  for (int i = 0; i < m; ++i) {
+    const int x = of(first + (m > 1 ? (int)((int64_t)i * (n - 1) / (m - 1)) : 0));
+    s.mean += (double)x / m;
+    s.most = x > s.most ? x : s.most;
+  }
+  return s;
+}
+inline SwaSteps swa_row_steps(const SwaParams& p) {
+  return swa_steps(0, p.n_qtiles, [&](int t) { return SwaWalk(t * kSwaRows, imin((t + 1) * kSwaRows, p.seq_q) - 1, p.hi, p.lo, p.sinks, p.seq_k).n; });
+}
 
 int swa_fill(SwaParams& p, int batch, int n_heads, int n_kv_heads, int seq_q, int seq_k, int head_dim, int dtype, int64_t q_start, int64_t k_start,
              int64_t left, int64_t right, int64_t sinks, float softmax_scale);

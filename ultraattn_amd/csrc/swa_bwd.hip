@@ -11,6 +11,7 @@
 // A column of the sinks is seen by every later query: its walk is cut into parts of about the others' length, which leave fp32 dK and
 // dV that a last launch adds in their order.  So are all walks where there are few of them.
 #include <algorithm>
+#include <cmath>
 #include "swa.h"
 
 namespace ua {
@@ -132,20 +133,14 @@ __device__ __forceinline__ void columns_walk(uint32_t lds, int block) {
   using L = BwdLds<kD>;
   typedef typename SwaVec<T>::x8 x8;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int kt, bh, part = 0;
-  const bool cut = block < p.n_cut_blocks;
-  if (cut) {                                             // the parts of one column far from each other
-    const int rest = quotient(block, p.by_cols);
-    bh = block - rest * p.by_cols.d;
-    part = quotient(rest, p.by_cut);
-    kt = rest - part * p.n_cut;
-  } else {
-    map_block(block - p.n_cut_blocks, p.cols, kt, bh);
-    kt += p.n_cut;
-  }
+  const int run = block < p.cols[0].n_blocks ? 0 : 1;
+  const SwaColumns& c = p.cols[run];
+  int pos, bh;
+  map_block(block - (run ? p.cols[0].n_blocks : 0), c.map, pos, bh);
+  const int tile = quotient(pos, c.by_parts), part = pos - tile * c.n_parts, kt = c.first + tile;
   const int b = quotient(bh, p.by_kv_heads), hk = bh - b * p.n_kv_heads, k0 = kt * kSwaRows;
   const SwaColumn col(k0, min(k0 + kSwaRows, p.seq_k) - 1, p.hi, p.lo, p.sinks, p.seq_q);
-  const int total = col.n * p.group, part_len = cut ? (total + p.col_parts - 1) / p.col_parts : total;
+  const int total = col.n * p.group, part_len = (total + c.n_parts - 1) / c.n_parts;
   const int i0 = min(part * part_len, total), i1 = min(i0 + part_len, total);
 
   // a step's place: query head (of the group) and block of 64 rows
@@ -241,10 +236,11 @@ __device__ __forceinline__ void columns_walk(uint32_t lds, int block) {
   const SwaParams& e = params_again();
   const int n_rows = e.seq_k - key0;
   if (n_rows <= 0) return;
-  if (cut) {
-    const int64_t row = part * e.col_part + ((int64_t)bh * e.n_cut * kSwaRows + key0) * kD;
-    swa_store_f32<kD>(e.part_dk + row, kD, n_rows, dk, e.scale);
-    swa_store_f32<kD>(e.part_dv + row, kD, n_rows, dv, 1.f / kSwaPScale<T>);
+  const SwaColumns& ec = e.cols[run];
+  if (ec.n_parts > 1) {
+    const int64_t row = part * ec.part + ((int64_t)bh * ec.tiles * kSwaRows + key0 - ec.first * kSwaRows) * kD;
+    swa_store_f32<kD>(ec.dk + row, kD, n_rows, dk, e.scale);
+    swa_store_f32<kD>(ec.dv + row, kD, n_rows, dv, 1.f / kSwaPScale<T>);
   } else {
     const uint32_t turn = lds + wave * 32 * H::kRow;
     swa_store_rows<T, kD>((T*)e.dk + b * e.dks.b + (int64_t)key0 * e.dks.s + hk * e.dks.h, e.dks.s, n_rows, dk, e.scale, turn);
@@ -429,7 +425,7 @@ __global__ __launch_bounds__(8 * kD) void swa_delta_kernel(const SwaParams p) {
   constexpr int kLanes = kD / 8;
   typedef typename SwaVec<T>::x8 x8;
   __shared__ float sums[16][4];
-  const int th = quotient(blockIdx.x, p.by_cut), hb = blockIdx.x - th * p.by_cut.d, b = quotient(th, p.by_parts), t0 = (th - b * p.by_parts.d) * 16, h0 = 4 * hb;
+  const int th = quotient(blockIdx.x, p.by_kv_heads), hb = blockIdx.x - th * p.by_kv_heads.d, b = quotient(th, p.by_parts), t0 = (th - b * p.by_parts.d) * 16, h0 = 4 * hb;
   const int lane = threadIdx.x % kLanes, r = threadIdx.x / kLanes, t = min(t0 + r / 4, p.seq_q - 1), h = min(h0 + r % 4, p.n_heads - 1);
   const x8 x = *reinterpret_cast<const x8*>((const T*)p.o + b * p.os.b + t * p.os.s + h * p.os.h + 8 * lane);
   const x8 y = *reinterpret_cast<const x8*>((const T*)p.dout + b * p.ds.b + t * p.ds.s + h * p.ds.h + 8 * lane);
@@ -488,12 +484,12 @@ struct SwaSum {
   int n_parts, tokens, part_tokens, heads, n_rows, n_groups;     // part_tokens: rows of a head in the parts
   Div by_tokens, by_heads;
 };
-struct SwaSums { SwaSum s[3]; };
+constexpr int kMaxSums = 5;                          // dK and dV of either run of columns, dQ
+struct SwaSums { SwaSum s[kMaxSums]; };
 template <class T, int kD>
 __global__ __launch_bounds__(256) void swa_sum_kernel(const SwaSums all) {
   int block = blockIdx.x, which = 0;
-  if (block >= all.s[0].n_groups) { block -= all.s[0].n_groups; which = 1; }
-  if (which == 1 && block >= all.s[1].n_groups) { block -= all.s[1].n_groups; which = 2; }
+  while (which < kMaxSums - 1 && block >= all.s[which].n_groups) block -= all.s[which++].n_groups;
   const SwaSum& x = all.s[which];
   constexpr int kPer = kD / 16;
   const int row = block * 16 + (threadIdx.x >> 4), c = threadIdx.x & 15;
@@ -517,34 +513,33 @@ __global__ __launch_bounds__(256) void swa_sum_kernel(const SwaSums all) {
 
 // How a backward is cut, and where its parts lie in the workspace (bytes).
 struct BwdCut {
-  int row_parts, n_cut, col_parts;
-  int64_t dq_bytes, col_bytes, total;             // of a part; of a part's dK
+  int row_parts, n_sink, col_parts[2];            // n_sink: tiles of the first run of columns
+  int64_t dq_bytes, col_bytes[2], total;          // of a part; of a part's dK
 };
-static BwdCut bwd_cut(const SwaParams& p, int head_dim) {
-  // Steps of 64 rows: of a row tile, of a column, of a column of the sinks (the longest); a column's has four products and a row's three.
-  const int64_t q_blocks = (p.seq_q + kSwaBlock - 1) / kSwaBlock, k_blocks = (p.seq_k + kSwaBlock - 1) / kSwaBlock;
-  const int64_t window = p.hi >= kFar || p.lo <= -kFar ? INT32_MAX : std::max<int64_t>(((int64_t)p.hi - p.lo + kSwaRows + 2 * kSwaBlock - 1) / kSwaBlock, 1);
-  const int64_t col = std::min(window, q_blocks) * p.group, sink_col = q_blocks * p.group, row = std::min(window + (p.sinks + kSwaBlock - 1) / kSwaBlock, k_blocks);
-  const int64_t cols = (int64_t)p.batch * p.n_kv_heads * p.n_ktiles, rows = (int64_t)p.batch * p.n_heads * p.n_qtiles;
-  const int64_t sink_tiles = p.sinks ? (p.sinks + kSwaRows - 1) / kSwaRows : 0;
-  BwdCut c{1, 0, 1, 0, 0, 0};
-  if (cols == 0 || rows == 0) return c;
-  const int64_t work = 4 * cols * col + 3 * rows * row;
-  const int64_t each = std::max<int64_t>(work / kDenseTargetGroups, 32);       // products of a workgroup, where there are few
-  auto parts = [&](int64_t steps) { return (int)std::min<int64_t>((steps + each - 1) / each, UA_MAX_PARTS); };
-  if (cols + rows < kDenseFullLaunch) {
-    c.row_parts = parts(3 * row);
-    c.col_parts = parts(4 * col);
-    if (c.col_parts > 1) c.n_cut = p.n_ktiles;
-  }
-  // the sinks' columns: parts of the other columns' length
-  if (sink_tiles && c.n_cut == 0 && sink_col > 2 * col) {
-    c.n_cut = (int)std::min<int64_t>(sink_tiles, p.n_ktiles);
-    c.col_parts = (int)std::min<int64_t>((sink_col + col - 1) / col, UA_MAX_PARTS);
-  }
+// Walks are cut to about what a workgroup has on average with two of them on every CU, if they are much longer and there is something to
+// gain beside the launch that adds the parts.  Lengths are counted in products of 64 rows, a column's step has four of them and a row's three.
+static BwdCut bwd_cut(const SwaParams& p, int head_dim, bool cut) {
+  BwdCut c{1, 0, {1, 1}, 0, {0, 0}, 0};
+  const double cols = (double)p.batch * p.n_kv_heads, rows = (double)p.batch * p.n_heads * p.n_qtiles;
+  if (!cut || cols * p.n_ktiles == 0 || rows == 0) return c;
+  auto column = [&](int t) { return SwaColumn(t * kSwaRows, imin((t + 1) * kSwaRows, p.seq_k) - 1, p.hi, p.lo, p.sinks, p.seq_q).n * p.group; };
+  const int sink_tiles = std::min((p.sinks + kSwaRows - 1) / kSwaRows, p.n_ktiles);
+  const SwaSteps row = swa_row_steps(p), sink = swa_steps(0, sink_tiles, column), col = swa_steps(sink_tiles, p.n_ktiles - sink_tiles, column);
+  const double work = 3 * rows * row.mean + 4 * cols * (sink_tiles * sink.mean + (p.n_ktiles - sink_tiles) * col.mean);
+  const double each = std::max(work / (2 * kCus), 32.0);
+  auto parts = [&](double products) { return products > 1.5 * each + 24 ? (int)std::min(std::ceil(products / each), (double)UA_MAX_PARTS) : 1; };
+  c.row_parts = parts(3.0 * row.most);
+  c.col_parts[0] = parts(4.0 * sink.most);
+  c.col_parts[1] = parts(4.0 * col.most);
+  if (c.col_parts[0] == c.col_parts[1]) c.col_parts[0] = 1;
+  else c.n_sink = sink_tiles;
   if (c.row_parts > 1) c.dq_bytes = align256((int64_t)p.batch * p.n_heads * p.seq_q * head_dim * 4);
-  if (c.n_cut) c.col_bytes = align256((int64_t)p.batch * p.n_kv_heads * c.n_cut * kSwaRows * head_dim * 4);
-  c.total = (c.row_parts > 1 ? c.row_parts * c.dq_bytes : 0) + 2 * c.col_parts * c.col_bytes;
+  const int tiles[2] = {c.n_sink, p.n_ktiles - c.n_sink};
+  for (int i = 0; i < 2; ++i) {
+    if (c.col_parts[i] > 1) c.col_bytes[i] = align256((int64_t)p.batch * p.n_kv_heads * tiles[i] * kSwaRows * head_dim * 4);
+    c.total += 2 * c.col_parts[i] * c.col_bytes[i];
+  }
+  c.total += c.row_parts * c.dq_bytes;
   return c;
 }
 
@@ -552,7 +547,8 @@ template <class T, int kD>
 static int bwd_run(const SwaParams& p, unsigned n, const SwaSums& sums, hipStream_t st) {
   if (n) swa_bwd_kernel<T, kD><<<n, 256, 0, st>>>(p);
   if (hipGetLastError() != hipSuccess) return UA_ERR_LAUNCH;
-  const int groups = sums.s[0].n_groups + sums.s[1].n_groups + sums.s[2].n_groups;
+  int groups = 0;
+  for (const SwaSum& x : sums.s) groups += x.n_groups;
   if (groups) swa_sum_kernel<T, kD><<<groups, 256, 0, st>>>(sums);
   return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
 }
@@ -581,7 +577,7 @@ extern "C" int ua_swa_bwd_delta(const void* o, const void* dout, const void* q, 
   auto three = [](const int64_t* s) { return Strides3{s[0], s[1], s[2]}; };
   p.o = const_cast<void*>(o); p.dout = dout; p.q = q; p.k = k; p.v = v; p.lse = const_cast<float*>(lse); p.delta = delta;
   p.os = three(o_strides); p.ds = three(do_strides); p.qs = three(q_strides); p.ks = three(k_strides); p.vs = three(v_strides);
-  p.by_cut = make_div((uint32_t)heads);
+  p.by_kv_heads = make_div((uint32_t)heads);             // (of this launch: groups of four heads, and of 16 tokens)
   p.by_parts = make_div((uint32_t)tokens);
   const unsigned n = (unsigned)(batch * tokens * heads);
   const hipStream_t st = (hipStream_t)stream;
@@ -600,7 +596,7 @@ extern "C" int64_t ua_swa_bwd_workspace_bytes(int batch, int n_heads, int n_kv_h
   using namespace ua;
   SwaParams p{};
   if (swa_fill(p, batch, n_heads, n_kv_heads, seqlen_q, seqlen_k, head_dim, UA_BF16, q_start, k_start, left, right, sinks, 1.f) != UA_OK) return 0;
-  return bwd_cut(p, head_dim).total;
+  return bwd_cut(p, head_dim, true).total;
 }
 
 extern "C" int ua_swa_bwd(const void* dout, const void* q, const void* k, const void* v, const float* lse, const float* delta, void* dq, void* dk, void* dv,
@@ -632,37 +628,44 @@ extern "C" int ua_swa_bwd(const void* dout, const void* q, const void* k, const 
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.ds = three(do_strides); p.qs = three(q_strides); p.ks = three(k_strides); p.vs = three(v_strides);
   p.dqs = three(dq_strides); p.dks = three(dk_strides); p.dvs = three(dv_strides);
-  BwdCut cut = bwd_cut(p, head_dim);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < cut.total) cut = BwdCut{1, 0, 1, 0, 0, 0};
+  BwdCut cut = bwd_cut(p, head_dim, workspace && aligned16(workspace));
+  if (workspace_bytes < cut.total) cut = bwd_cut(p, head_dim, false);
   p.n_parts = cut.row_parts;
-  p.n_cut = cut.n_cut;
-  p.col_parts = cut.col_parts;
-  char* at = (char*)workspace;
-  p.part_dk = (float*)at;
-  p.part_dv = (float*)(at + cut.col_parts * cut.col_bytes);
-  p.col_part = cut.col_bytes / 4;
-  p.part_o = (float*)(at + 2 * cut.col_parts * cut.col_bytes);
-  p.o_part = cut.dq_bytes / 4;
-  const int col_heads = batch * n_kv_heads;
   p.by_parts = make_div(p.n_parts);
-  p.by_cols = make_div(std::max(col_heads, 1));
-  p.by_cut = make_div(std::max(p.n_cut, 1));
-  p.n_cut_blocks = col_heads * p.n_cut * p.col_parts;
-  p.n_col_blocks = p.n_cut_blocks + col_heads * (p.n_ktiles - p.n_cut);
-  p.cols = block_map(std::max(col_heads, 1), std::max(p.n_ktiles - p.n_cut, 1));
-  p.map = block_map(batch * n_heads, std::max(p.n_qtiles * p.n_parts, 1));
-  const unsigned n = (unsigned)(p.n_col_blocks + batch * n_heads * p.n_qtiles * p.n_parts);
+  const int key_heads = batch * n_kv_heads;
+  char* at = (char*)workspace;
   SwaSums sums{};
-  auto sum = [&](int i, const float* parts, int64_t part, int n_parts, void* out, const Strides3& os, int tokens, int part_tokens, int heads) {
+  int n_sums = 0;
+  auto sum = [&](const float* parts, int64_t part, int n_parts, void* out, const Strides3& os, int tokens, int part_tokens, int heads) {
     const int rows = batch * heads * tokens;
-    sums.s[i] = {parts, out, part, os, n_parts, tokens, part_tokens, heads, rows, (rows + 15) / 16, make_div(std::max(tokens, 1)), make_div(heads)};
+    sums.s[n_sums++] = {parts, out, part, os, n_parts, tokens, part_tokens, heads, rows, (rows + 15) / 16, make_div(std::max(tokens, 1)), make_div(heads)};
   };
-  if (p.n_cut) {
-    const int tokens = std::min(p.n_cut * kSwaRows, seqlen_k);
-    sum(0, p.part_dk, p.col_part, p.col_parts, dk, p.dks, tokens, p.n_cut * kSwaRows, n_kv_heads);
-    sum(1, p.part_dv, p.col_part, p.col_parts, dv, p.dvs, tokens, p.n_cut * kSwaRows, n_kv_heads);
+  const int size = 2;                                     // bytes of an element
+  for (int i = 0; i < 2; ++i) {
+    SwaColumns& c = p.cols[i];
+    c.first = i ? cut.n_sink : 0;
+    c.tiles = i ? p.n_ktiles - cut.n_sink : cut.n_sink;
+    c.n_parts = cut.col_parts[i];
+    c.by_parts = make_div(c.n_parts);
+    c.n_blocks = key_heads * c.tiles * c.n_parts;
+    c.map = block_map(std::max(key_heads, 1), std::max(c.tiles * c.n_parts, 1));
+    p.n_col_blocks += c.n_blocks;
+    if (c.n_parts == 1 || c.tiles == 0) continue;
+    c.part = cut.col_bytes[i] / 4;
+    c.dk = (float*)at;
+    c.dv = (float*)(at + c.n_parts * cut.col_bytes[i]);
+    at += 2 * c.n_parts * cut.col_bytes[i];
+    const int row = c.first * kSwaRows, tokens = std::min(c.tiles * kSwaRows, seqlen_k - row);
+    sum(c.dk, c.part, c.n_parts, (char*)dk + row * p.dks.s * size, p.dks, tokens, c.tiles * kSwaRows, n_kv_heads);
+    sum(c.dv, c.part, c.n_parts, (char*)dv + row * p.dvs.s * size, p.dvs, tokens, c.tiles * kSwaRows, n_kv_heads);
   }
-  if (p.n_parts > 1) sum(2, p.part_o, p.o_part, p.n_parts, dq, p.dqs, seqlen_q, seqlen_q, n_heads);
+  if (p.n_parts > 1) {
+    p.part_o = (float*)at;
+    p.o_part = cut.dq_bytes / 4;
+    sum(p.part_o, p.o_part, p.n_parts, dq, p.dqs, seqlen_q, seqlen_q, n_heads);
+  }
+  p.map = block_map(std::max(batch * n_heads, 1), std::max(p.n_qtiles * p.n_parts, 1));
+  const unsigned n = (unsigned)(p.n_col_blocks + batch * n_heads * p.n_qtiles * p.n_parts);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == UA_FP16) return head_dim == 64 ? bwd_run<fp16, 64>(p, n, sums, st) : bwd_run<fp16, 128>(p, n, sums, st);
   return head_dim == 64 ? bwd_run<bf16, 64>(p, n, sums, st) : bwd_run<bf16, 128>(p, n, sums, st);

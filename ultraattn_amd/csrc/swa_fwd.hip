@@ -259,17 +259,28 @@ int swa_fill(SwaParams& p, int batch, int n_heads, int n_kv_heads, int seq_q, in
   return UA_OK;
 }
 
-// Blocks of 64 keys that the longest walk of a call has.
-static int64_t longest_walk(const SwaParams& p) {
-  const int64_t blocks = ((int64_t)p.seq_k + kSwaBlock - 1) / kSwaBlock;
-  const int64_t window = p.hi >= kFar || p.lo <= -kFar ? blocks : ((int64_t)p.hi - p.lo + kSwaRows + 2 * kSwaBlock - 1) / kSwaBlock + (p.sinks + kSwaBlock - 1) / kSwaBlock;
-  return std::max<int64_t>(std::min(window, blocks), 0);
-}
-// Parts that a forward's walks are cut into.
-static int fwd_parts(const SwaParams& p) {
-  const int64_t lines = (int64_t)p.batch * p.n_heads * p.n_qtiles, walk = longest_walk(p);
-  if (lines == 0 || lines >= kDenseFullLaunch || walk < 8) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({kDenseTargetGroups / lines, walk / 4, UA_MAX_PARTS}));
+// Parts that a forward's walks are cut into: what an estimate of the launch's time in microseconds says.  A step takes `alone` where a CU has one
+// workgroup and `shared` where it has two; parts cost a launch for their merge, and each its rows' way through the caches.  us, whole and in
+// 2, 4, 8 and 16 parts (heads, queries x keys, window; what is taken in brackets):
+//     128 columns   4, 2048 causal     37.2   28.7  [25.3]  27.8   39.0          64 columns   8, 2048 causal       28.3  24.6  [24.0]  29.4  39.9
+//                   8, 128 x 4096      67.0   41.4   27.8  [23.6]  27.2                       2, 8192, 2047        32.9 [26.4]  27.2   31.9  44.1
+//                  32, 100 x 16384    256    136     75.5  [50.2]  53.9                       8, 512 causal       [10.6] 12.1   12.4   15.0  19.0
+//                   4, 8192, 2047     [44.5]  53.2   60.7   79.2  137                         2 x 10, 1333 x 2048, 700 [19.5] 25.4
+static int fwd_parts(const SwaParams& p, int head_dim) {
+  const double lines = (double)p.batch * p.n_heads * p.n_qtiles;
+  if (lines == 0 || lines >= 2 * kCus) return 1;
+  const SwaSteps s = swa_row_steps(p);
+  const double alone = head_dim == 64 ? 0.75 : 1.0, shared = head_dim == 64 ? 1.2 : 2.05;
+  const double part_us = 0.3 + (double)p.batch * p.n_heads * p.seq_q * head_dim * 8e-7;      // written and read
+  int best = 1;
+  double best_us = 1e30;
+  for (int parts = 1; parts <= UA_MAX_PARTS && (parts == 1 || 2 * parts <= s.most); ++parts) {
+    const double busy = lines * parts * s.mean / std::max(s.most, 1), beside = std::min(std::max((busy - kCus) / kCus, 0.0), 1.0);
+    const double walk = std::max((s.most + parts - 1) / parts * (alone + (shared - alone) * beside), lines * s.mean / (2 * kCus) * shared);
+    const double us = 5 + walk + (parts > 1 ? 5 + part_us * parts : 0);
+    if (us < 0.93 * best_us) { best_us = us; best = parts; }
+  }
+  return best;
 }
 static int64_t part_rows(const SwaParams& p) { return (int64_t)p.batch * p.n_heads * p.seq_q; }
 
@@ -280,7 +291,7 @@ extern "C" int64_t ua_swa_workspace_bytes(int batch, int n_heads, int n_kv_heads
   using namespace ua;
   SwaParams p{};
   if (swa_fill(p, batch, n_heads, n_kv_heads, seqlen_q, seqlen_k, head_dim, UA_BF16, q_start, k_start, left, right, sinks, 1.f) != UA_OK) return 0;
-  const int parts = fwd_parts(p);
+  const int parts = fwd_parts(p, head_dim);
   return parts > 1 ? parts * (align256(part_rows(p) * head_dim * 4) + align256(part_rows(p) * 4)) : 0;
 }
 
@@ -306,7 +317,7 @@ extern "C" int ua_swa_fwd(const void* q, const void* k, const void* v, void* o, 
   p.vs = {v_strides[0], v_strides[1], v_strides[2]};
   p.os = {o_strides[0], o_strides[1], o_strides[2]};
   const hipStream_t st = (hipStream_t)stream;
-  const int parts = fwd_parts(p);
+  const int parts = fwd_parts(p, head_dim);
   const int64_t o_bytes = align256(part_rows(p) * head_dim * 4), lse_bytes = align256(part_rows(p) * 4);
   if (parts > 1 && workspace && aligned16(workspace) && workspace_bytes >= parts * (o_bytes + lse_bytes)) {
     p.n_parts = parts;
