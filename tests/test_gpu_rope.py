@@ -127,13 +127,28 @@ def test_views_and_in_place():
     assert ua.rope_fwd(empty, None, f)[0].shape == empty.shape
 
 
-def test_infinities_stay_in_their_pair():
-    f = ua.rope_freqs(16, device=DEV)[0]
+@pytest.mark.parametrize("rotary,interleaved,partner", [(16, False, 11), (20, False, 13), (20, True, 2), (6, True, 2), (6, False, None)])
+def test_infinities_stay_in_their_pair(rotary, interleaved, partner):
+    f = ua.rope_freqs(rotary, device=DEV)[0]
     q = rows(1, 4, 1, 32, torch.bfloat16)
-    q[0, 2, 0, 3] = torch.inf
-    got = ua.rope_fwd(q, None, f)[0]
+    at = 3 if partner is not None else 7                              # (behind the pairs: alone)
+    q[0, 2, 0, at] = torch.inf
+    got = ua.rope_fwd(q, None, f, start=1, interleaved=interleaved)[0]
     bad = ~torch.isfinite(got)
-    assert bad[0, 2, 0, 3] and bad[0, 2, 0, 11] and bad.sum() == 2
+    assert bad[0, 2, 0, at] and (partner is None or bad[0, 2, 0, partner]) and bad.sum() == (1 if partner is None else 2)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rotary", [(128, 20), (64, 12), (64, 6), (128, 36), (48, 46)])
+def test_parts_that_no_vector_divides_in_place_and_not(dim, rotary, interleaved):
+    q, k = rows(2, 40, 3, dim, torch.float16), rows(2, 40, 2, dim, torch.float16, 1)
+    f = ua.rope_freqs(rotary, device=DEV)[0]
+    qo, ko = ua.rope_fwd(q, k, f, start=9, interleaved=interleaved)
+    check(qo, q, positions(2, 40, 9), f, interleaved=interleaved)
+    check(ko, k, positions(2, 40, 9), f, interleaved=interleaved)
+    x = q.clone()
+    ua.rope_fwd(x, None, f, start=9, interleaved=interleaved, q_out=x)
+    assert torch.equal(x, qo)
 
 
 @pytest.mark.parametrize("interleaved", [False, True])

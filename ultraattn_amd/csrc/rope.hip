@@ -15,7 +15,7 @@ typedef _Float16 fp16;
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeAngles = 512;           // pairs of all of a workgroup's tokens (a head of 256 has up to 128)
-constexpr int kRopeMaxTokens = 16;
+constexpr int kRopeMaxTokens = 16, kRopePad = 8;
 constexpr int kRopeAhead = 4;              // items of a thread whose loads are in flight together
 
 // One of the tensors that a call goes through: x [batch, tokens, heads, head_dim] to y, turned or (kRotate = 0) as it is.  An item is
@@ -75,22 +75,29 @@ template <class T, int kV> __device__ __forceinline__ void rope_store(T* p, cons
   }
 }
 
-// kV elements a vector: the most that sizes, strides and pointers allow, up to 16 bytes.  A workgroup goes through the tensors one after the
-// other, or, where there are few tokens, takes one of them (blockIdx.y): which one is then a scalar either way.
-template <class T, int kV, bool kInterleaved>
+// Three ways through a head, by what its layout allows:
+//   kPairs   two vectors of kV entries and their partners, rotary_dim / 2 apart (kV divides that); interleaved only as single entries;
+//   kBeside  interleaved: one vector holds kV / 2 pairs;
+//   kGather  one vector, and its entries' partners one by one: where rotary_dim / 2 is odd or twice odd, so that pairs of vectors would be
+//            of 4 bytes or less (16 heads, 4096 tokens, 20 of 128 entries: GATHER).  Not in place: a partner may have been written.
+enum RopeWay { kPairs, kBeside, kGather };
+// A workgroup goes through the tensors one after the other, or, where there are few tokens, takes one of them (blockIdx.y): which one is
+// then a scalar either way.
+template <class T, int kV, RopeWay kWay, bool kInterleaved>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) {
-  __shared__ __attribute__((aligned(16))) float cosine[kRopeAngles], sine[kRopeAngles];
+  static_assert(kWay == kPairs ? !kInterleaved || kV == 1 : (kWay == kBeside) == kInterleaved && kV > 1, "ways");
+  __shared__ __attribute__((aligned(16))) float cosine[kRopeAngles + kRopePad], sine[kRopeAngles + kRopePad];
   __shared__ int64_t position[kRopeMaxTokens];
   const int first = blockIdx.x * p.tokens_per_group, n_here = min(p.tokens_per_group, p.n_tokens - first);
   const int begin = gridDim.y > 1 ? blockIdx.y : 0, end = gridDim.y > 1 ? begin + 1 : 3;
   bool made = false;
   for (int which = begin; which < end; ++which) {
     const RopeTensor& x = p.t[which];
-    const int n = n_here * x.items, n_turned = x.rotate ? p.n_half / kV : 0;
+    const int n = n_here * x.items, n_turned = x.rotate ? p.n_half / kV : 0, n_pairs = x.rotate ? p.n_half : 0;
     for (int i0 = 0; i0 < n; i0 += kRopeThreads * kRopeAhead) {
       T a[kRopeAhead][kV], b2[kRopeAhead][kV];
       T* to[kRopeAhead];
-      int token[kRopeAhead], angle[kRopeAhead], second[kRopeAhead];    // first angle, -1: passes through; elements to the second vector, 0: none
+      int token[kRopeAhead], angle[kRopeAhead], second[kRopeAhead];    // kPairs: first angle, -1 passes through; entries to the second vector, 0 none
 #pragma unroll
       for (int u = 0; u < kRopeAhead; ++u) {
         const int i = i0 + u * kRopeThreads + threadIdx.x;
@@ -98,21 +105,31 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
         if (i >= n) continue;
         const int t = quotient(i, x.by_token), r = i - t * x.items, h = quotient(r, x.by_head), item = r - h * x.by_head.d;
         const int b = quotient(first + t, p.by_seq), s = first + t - b * p.seqlen;
-        int at;                                           // the first vector, in vectors
-        if (item < n_turned) {
-          angle[u] = t * p.n_half + item * kV;
-          at = kInterleaved ? 2 * item : item;
-          second[u] = kInterleaved ? kV : p.n_half;
-        } else {
-          angle[u] = -1;
-          at = 2 * item;                                  // (2 * n_turned vectors are turned)
-          second[u] = at + 1 < p.head_vecs ? kV : 0;
-        }
         token[u] = t;
-        const T* from = static_cast<const T*>(x.x) + b * x.xs.b + s * x.xs.s + h * x.xs.h + at * kV;
+        const T* head = static_cast<const T*>(x.x) + b * x.xs.b + s * x.xs.s + h * x.xs.h;
+        int at = item;                                      // the (first) vector
+        if constexpr (kWay == kPairs) {
+          if (item < n_turned) {
+            angle[u] = t * p.n_half + item * kV;
+            if (kInterleaved) at = 2 * item;
+            second[u] = kInterleaved ? kV : p.n_half;
+          } else {
+            angle[u] = -1;
+            at = 2 * item;                                  // (2 * n_turned vectors are turned)
+            second[u] = at + 1 < p.head_vecs ? kV : 0;
+          }
+          if (second[u]) rope_load<T, kV>(b2[u], head + at * kV + second[u]);
+        } else {
+          angle[u] = at * kV;                               // the first entry
+          if (kWay == kGather && angle[u] < 2 * n_pairs)
+#pragma unroll
+            for (int j = 0; j < kV; ++j) {
+              const int e = min(angle[u] + j, 2 * n_pairs - 1);
+              b2[u][j] = head[e < n_pairs ? e + n_pairs : e - n_pairs];
+            }
+        }
         to[u] = static_cast<T*>(x.y) + b * x.ys.b + (x.cached ? 0 : s * x.ys.s) + h * x.ys.h + at * kV;
-        rope_load<T, kV>(a[u], from);
-        if (second[u]) rope_load<T, kV>(b2[u], from + second[u]);
+        rope_load<T, kV>(a[u], head + at * kV);
       }
       if (!made) {                                        // workgroup-uniform; the first loads are on their way meanwhile
         made = true;
@@ -137,41 +154,60 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
           if (row < 0 || row >= p.room) continue;
           to[u] += row * x.ys.s;
         }
-        if (angle[u] >= 0) {
-          // entries 0 .. 2 kV - 1 of the two vectors; pair j is (j, kV + j), or (2j, 2j + 1)
-          float f[2 * kV];
+        if constexpr (kWay == kPairs) {
+          if (angle[u] >= 0)
 #pragma unroll
-          for (int j = 0; j < kV; ++j) { f[j] = (float)a[u][j]; f[kV + j] = (float)b2[u][j]; }
+            for (int j = 0; j < kV; ++j) {
+              const float c = cosine[angle[u] + j], s = sine[angle[u] + j], g = (float)a[u][j], e = (float)b2[u][j];
+              a[u][j] = (T)(g * c - e * s);
+              b2[u][j] = (T)(e * c + g * s);
+            }
+          if (second[u]) rope_store<T, kV>(to[u] + second[u], b2[u]);
+        } else if constexpr (kWay == kBeside) {
+          const int pair0 = angle[u] / 2, base = token[u] * p.n_half;
+#pragma unroll
+          for (int j = 0; j < kV / 2; ++j) {
+            if (pair0 + j >= n_pairs) continue;
+            const float c = cosine[base + pair0 + j], s = sine[base + pair0 + j], g = (float)a[u][2 * j], e = (float)a[u][2 * j + 1];
+            a[u][2 * j] = (T)(g * c - e * s);
+            a[u][2 * j + 1] = (T)(e * c + g * s);
+          }
+        } else {
 #pragma unroll
           for (int j = 0; j < kV; ++j) {
-            const int lo = kInterleaved ? 2 * j : j, hi = kInterleaved ? 2 * j + 1 : kV + j;
-            const float c = cosine[angle[u] + j], s = sine[angle[u] + j], g = f[lo], e = f[hi];
-            f[lo] = g * c - e * s;
-            f[hi] = e * c + g * s;
+            const int e = angle[u] + j;
+            if (e >= 2 * n_pairs) continue;
+            const bool lower = e < n_pairs;
+            const int at = token[u] * p.n_half + (lower ? e : e - n_pairs);
+            const float c = cosine[at], s = lower ? -sine[at] : sine[at];
+            a[u][j] = (T)((float)a[u][j] * c + (float)b2[u][j] * s);
           }
-#pragma unroll
-          for (int j = 0; j < kV; ++j) { a[u][j] = (T)f[j]; b2[u][j] = (T)f[kV + j]; }
         }
         rope_store<T, kV>(to[u], a[u]);
-        if (second[u]) rope_store<T, kV>(to[u] + second[u], b2[u]);
       }
     }
   }
 }
 
 template <class T, int kV>
-static void rope_launch(const RopeParams& p, bool interleaved, dim3 groups, hipStream_t st) {
-  if (interleaved) rope_kernel<T, kV, true><<<groups, kRopeThreads, 0, st>>>(p);
-  else             rope_kernel<T, kV, false><<<groups, kRopeThreads, 0, st>>>(p);
+static void rope_launch(const RopeParams& p, bool interleaved, RopeWay way, dim3 groups, hipStream_t st) {
+  if constexpr (kV > 1) {
+    if (way == kBeside)     rope_kernel<T, kV, kBeside, true><<<groups, kRopeThreads, 0, st>>>(p);
+    else if (way == kGather) rope_kernel<T, kV, kGather, false><<<groups, kRopeThreads, 0, st>>>(p);
+    else                    rope_kernel<T, kV, kPairs, false><<<groups, kRopeThreads, 0, st>>>(p);
+  } else {
+    if (interleaved) rope_kernel<T, 1, kPairs, true><<<groups, kRopeThreads, 0, st>>>(p);
+    else             rope_kernel<T, 1, kPairs, false><<<groups, kRopeThreads, 0, st>>>(p);
+  }
 }
 
 struct RopeShape { int batch, seqlen, head_dim, rotary_dim, dtype; };
 
-// The widest vector (in elements) that the layout allows.
-static int rope_vector(const RopeShape& s, const RopeTensor* t, const int* heads, int n) {
+// The widest vector (in elements) that the tensors allow and that divides `unit` and the head.
+static int rope_vector(const RopeShape& s, const RopeTensor* t, const int* heads, int n, int unit) {
   const int size = s.dtype == UA_FP32 ? 4 : 2;
   for (int v = 16 / size; v > 1; v /= 2) {
-    bool ok = s.rotary_dim / 2 % v == 0 && s.head_dim % v == 0;
+    bool ok = unit % v == 0 && s.head_dim % v == 0;
     for (int i = 0; i < n && ok; ++i) {
       if (!heads[i]) continue;
       const int64_t all[6] = {t[i].xs.b, t[i].xs.s, t[i].xs.h, t[i].ys.b, t[i].ys.s, t[i].ys.h};
@@ -184,17 +220,27 @@ static int rope_vector(const RopeShape& s, const RopeTensor* t, const int* heads
 }
 
 static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_tensors, int interleaved, hipStream_t st) {
-  const int v = rope_vector(s, p.t, heads, n_tensors);
+  const int size = s.dtype == UA_FP32 ? 4 : 2;
   p.n_half = s.rotary_dim / 2;
+  bool in_place = false;
+  for (int i = 0; i < n_tensors; ++i) in_place = in_place || (heads[i] && p.t[i].x == p.t[i].y);
+  const int wide = rope_vector(s, p.t, heads, n_tensors, s.head_dim);
+  int v = interleaved ? wide : rope_vector(s, p.t, heads, n_tensors, p.n_half);
+  RopeWay way = interleaved && v > 1 ? kBeside : kPairs;
+  if (!interleaved && v * size <= 4 && wide > v && !in_place) {
+    way = kGather;
+    v = wide;
+  }
   p.head_vecs = s.head_dim / v;
   p.seqlen = s.seqlen;
   int64_t n_items = 0;
   for (int i = 0; i < 3; ++i) {
     RopeTensor& t = p.t[i];
     if (i >= n_tensors || !heads[i]) { t.items = 0; t.by_head = t.by_token = make_div(1); continue; }
-    const int turned = t.rotate ? p.n_half / v : 0, rest = p.head_vecs - 2 * turned;
-    const bool in_place = t.rotate && !t.cached && t.x == t.y && t.xs.b == t.ys.b && t.xs.s == t.ys.s && t.xs.h == t.ys.h;   // what passes through is there already
-    const int per_head = turned + (in_place ? 0 : (rest + 1) / 2);
+    // what passes through is there already
+    const bool same = t.rotate && !t.cached && t.x == t.y && t.xs.b == t.ys.b && t.xs.s == t.ys.s && t.xs.h == t.ys.h;
+    const int turned = t.rotate ? p.n_half / v : 0;
+    const int per_head = way == kPairs ? turned + (same ? 0 : (p.head_vecs - 2 * turned + 1) / 2) : same ? (s.rotary_dim + v - 1) / v : p.head_vecs;
     if ((int64_t)per_head * heads[i] * kRopeMaxTokens > INT32_MAX) return UA_ERR_SHAPE;
     t.items = per_head * heads[i];
     t.by_head = make_div(per_head);
@@ -211,21 +257,18 @@ static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_t
   const dim3 groups(lines, lines <= 4 * kCus ? n_tensors : 1);
   const int rc = check_device();
   if (rc != UA_OK) return rc;
-  if (s.dtype == UA_FP32) {
-    if (v == 4) rope_launch<float, 4>(p, interleaved, groups, st);
-    else if (v == 2) rope_launch<float, 2>(p, interleaved, groups, st);
-    else rope_launch<float, 1>(p, interleaved, groups, st);
-  } else if (s.dtype == UA_FP16) {
-    if (v == 8) rope_launch<fp16, 8>(p, interleaved, groups, st);
-    else if (v == 4) rope_launch<fp16, 4>(p, interleaved, groups, st);
-    else if (v == 2) rope_launch<fp16, 2>(p, interleaved, groups, st);
-    else rope_launch<fp16, 1>(p, interleaved, groups, st);
-  } else {
-    if (v == 8) rope_launch<bf16, 8>(p, interleaved, groups, st);
-    else if (v == 4) rope_launch<bf16, 4>(p, interleaved, groups, st);
-    else if (v == 2) rope_launch<bf16, 2>(p, interleaved, groups, st);
-    else rope_launch<bf16, 1>(p, interleaved, groups, st);
-  }
+  auto launch = [&](auto element) {
+    typedef decltype(element) T;
+    if constexpr (sizeof(T) == 2) {
+      if (v == 8) return rope_launch<T, 8>(p, interleaved, way, groups, st);
+    }
+    if (v == 4) rope_launch<T, 4>(p, interleaved, way, groups, st);
+    else if (v == 2) rope_launch<T, 2>(p, interleaved, way, groups, st);
+    else rope_launch<T, 1>(p, interleaved, way, groups, st);
+  };
+  if (s.dtype == UA_FP32) launch(0.f);
+  else if (s.dtype == UA_FP16) launch(fp16(0));
+  else launch(bf16(0.f));
   return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
 }
 
