@@ -15,7 +15,7 @@ typedef _Float16 fp16;
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeAngles = 512;           // pairs of all of a workgroup's tokens (a head of 256 has up to 128)
-constexpr int kRopeMaxTokens = 16, kRopePad = 8;
+constexpr int kRopeMaxTokens = 16;
 constexpr int kRopeAhead = 4;              // items of a thread whose loads are in flight together
 
 // One of the tensors that a call goes through: x [batch, tokens, heads, head_dim] to y, turned or (kRotate = 0) as it is.  An item is
@@ -64,29 +64,30 @@ template <class T, int kV> __device__ __forceinline__ void rope_load(T (&d)[kV],
     for (int j = 0; j < kV; ++j) d[j] = x[j];
   }
 }
-template <class T, int kV> __device__ __forceinline__ void rope_store(T* p, const T (&d)[kV]) {
+// kStream: results that are more than the caches hold go past them (2 x 8192 tokens, 40 heads of 128, 168 MB: 70.1 us, past them 54.5; 42 MB
+// 16.5 either way).
+constexpr int64_t kRopeStreamBytes = int64_t(128) << 20;
+template <class T, int kV, bool kStream> __device__ __forceinline__ void rope_store(T* p, const T (&d)[kV]) {
   typedef __attribute__((ext_vector_type(kV))) T vec;
   if constexpr (kV == 1) *p = d[0];
   else {
     vec x;
 #pragma unroll
     for (int j = 0; j < kV; ++j) x[j] = d[j];
-    *reinterpret_cast<vec*>(p) = x;
+    if constexpr (kStream) __builtin_nontemporal_store(x, reinterpret_cast<vec*>(p)); else *reinterpret_cast<vec*>(p) = x;
   }
 }
 
-// Three ways through a head, by what its layout allows:
+// Two ways through a head, by what its layout allows:
 //   kPairs   two vectors of kV entries and their partners, rotary_dim / 2 apart (kV divides that); interleaved only as single entries;
-//   kBeside  interleaved: one vector holds kV / 2 pairs;
-//   kGather  one vector, and its entries' partners one by one: where rotary_dim / 2 is odd or twice odd, so that pairs of vectors would be
-//            of 4 bytes or less (16 heads, 4096 tokens, 20 of 128 entries: GATHER).  Not in place: a partner may have been written.
-enum RopeWay { kPairs, kBeside, kGather };
+//   kBeside  interleaved: one vector holds kV / 2 pairs (2 x 8192 tokens, 16 heads of 128, 20 entries turned: as pairs of two vectors 31.5 us, so 23.5).
+enum RopeWay { kPairs, kBeside };
 // A workgroup goes through the tensors one after the other, or, where there are few tokens, takes one of them (blockIdx.y): which one is
 // then a scalar either way.
-template <class T, int kV, RopeWay kWay, bool kInterleaved>
+template <class T, int kV, RopeWay kWay, bool kInterleaved, bool kStream>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) {
-  static_assert(kWay == kPairs ? !kInterleaved || kV == 1 : (kWay == kBeside) == kInterleaved && kV > 1, "ways");
-  __shared__ __attribute__((aligned(16))) float cosine[kRopeAngles + kRopePad], sine[kRopeAngles + kRopePad];
+  static_assert(kWay == kPairs ? !kInterleaved || kV == 1 : kInterleaved && kV > 1, "ways");
+  __shared__ __attribute__((aligned(16))) float cosine[kRopeAngles], sine[kRopeAngles];
   __shared__ int64_t position[kRopeMaxTokens];
   const int first = blockIdx.x * p.tokens_per_group, n_here = min(p.tokens_per_group, p.n_tokens - first);
   const int begin = gridDim.y > 1 ? blockIdx.y : 0, end = gridDim.y > 1 ? begin + 1 : 3;
@@ -118,18 +119,12 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
             at = 2 * item;                                  // (2 * n_turned vectors are turned)
             second[u] = at + 1 < p.head_vecs ? kV : 0;
           }
-          if (second[u]) rope_load<T, kV>(b2[u], head + at * kV + second[u]);
         } else {
           angle[u] = at * kV;                               // the first entry
-          if (kWay == kGather && angle[u] < 2 * n_pairs)
-#pragma unroll
-            for (int j = 0; j < kV; ++j) {
-              const int e = min(angle[u] + j, 2 * n_pairs - 1);
-              b2[u][j] = head[e < n_pairs ? e + n_pairs : e - n_pairs];
-            }
         }
         to[u] = static_cast<T*>(x.y) + b * x.ys.b + (x.cached ? 0 : s * x.ys.s) + h * x.ys.h + at * kV;
         rope_load<T, kV>(a[u], head + at * kV);
+        if (kWay == kPairs && second[u]) rope_load<T, kV>(b2[u], head + at * kV + second[u]);
       }
       if (!made) {                                        // workgroup-uniform; the first loads are on their way meanwhile
         made = true;
@@ -162,8 +157,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
               a[u][j] = (T)(g * c - e * s);
               b2[u][j] = (T)(e * c + g * s);
             }
-          if (second[u]) rope_store<T, kV>(to[u] + second[u], b2[u]);
-        } else if constexpr (kWay == kBeside) {
+        } else {
           const int pair0 = angle[u] / 2, base = token[u] * p.n_half;
 #pragma unroll
           for (int j = 0; j < kV / 2; ++j) {
@@ -172,33 +166,21 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
             a[u][2 * j] = (T)(g * c - e * s);
             a[u][2 * j + 1] = (T)(e * c + g * s);
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kV; ++j) {
-            const int e = angle[u] + j;
-            if (e >= 2 * n_pairs) continue;
-            const bool lower = e < n_pairs;
-            const int at = token[u] * p.n_half + (lower ? e : e - n_pairs);
-            const float c = cosine[at], s = lower ? -sine[at] : sine[at];
-            a[u][j] = (T)((float)a[u][j] * c + (float)b2[u][j] * s);
-          }
         }
-        rope_store<T, kV>(to[u], a[u]);
+        rope_store<T, kV, kStream>(to[u], a[u]);
+        if (kWay == kPairs && second[u]) rope_store<T, kV, kStream>(to[u] + second[u], b2[u]);
       }
     }
   }
 }
 
 template <class T, int kV>
-static void rope_launch(const RopeParams& p, bool interleaved, RopeWay way, dim3 groups, hipStream_t st) {
-  if constexpr (kV > 1) {
-    if (way == kBeside)     rope_kernel<T, kV, kBeside, true><<<groups, kRopeThreads, 0, st>>>(p);
-    else if (way == kGather) rope_kernel<T, kV, kGather, false><<<groups, kRopeThreads, 0, st>>>(p);
-    else                    rope_kernel<T, kV, kPairs, false><<<groups, kRopeThreads, 0, st>>>(p);
-  } else {
-    if (interleaved) rope_kernel<T, 1, kPairs, true><<<groups, kRopeThreads, 0, st>>>(p);
-    else             rope_kernel<T, 1, kPairs, false><<<groups, kRopeThreads, 0, st>>>(p);
-  }
+static void rope_launch(const RopeParams& p, bool interleaved, bool stream, dim3 groups, hipStream_t st) {
+  constexpr bool kWide = kV * sizeof(T) == 16;
+  auto run = [&](auto kernel) { kernel<<<groups, kRopeThreads, 0, st>>>(p); };
+  if constexpr (kV == 1) interleaved ? run(rope_kernel<T, 1, kPairs, true, false>) : run(rope_kernel<T, 1, kPairs, false, false>);
+  else if (interleaved)  kWide && stream ? run(rope_kernel<T, kV, kBeside, true, kWide>) : run(rope_kernel<T, kV, kBeside, true, false>);
+  else                   kWide && stream ? run(rope_kernel<T, kV, kPairs, false, kWide>) : run(rope_kernel<T, kV, kPairs, false, false>);
 }
 
 struct RopeShape { int batch, seqlen, head_dim, rotary_dim, dtype; };
@@ -222,18 +204,11 @@ static int rope_vector(const RopeShape& s, const RopeTensor* t, const int* heads
 static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_tensors, int interleaved, hipStream_t st) {
   const int size = s.dtype == UA_FP32 ? 4 : 2;
   p.n_half = s.rotary_dim / 2;
-  bool in_place = false;
-  for (int i = 0; i < n_tensors; ++i) in_place = in_place || (heads[i] && p.t[i].x == p.t[i].y);
-  const int wide = rope_vector(s, p.t, heads, n_tensors, s.head_dim);
-  int v = interleaved ? wide : rope_vector(s, p.t, heads, n_tensors, p.n_half);
-  RopeWay way = interleaved && v > 1 ? kBeside : kPairs;
-  if (!interleaved && v * size <= 4 && wide > v && !in_place) {
-    way = kGather;
-    v = wide;
-  }
+  const int v = rope_vector(s, p.t, heads, n_tensors, interleaved ? s.head_dim : p.n_half);
+  const RopeWay way = interleaved && v > 1 ? kBeside : kPairs;
   p.head_vecs = s.head_dim / v;
   p.seqlen = s.seqlen;
-  int64_t n_items = 0;
+  int64_t n_items = 0, bytes = 0;
   for (int i = 0; i < 3; ++i) {
     RopeTensor& t = p.t[i];
     if (i >= n_tensors || !heads[i]) { t.items = 0; t.by_head = t.by_token = make_div(1); continue; }
@@ -243,6 +218,7 @@ static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_t
     const int per_head = way == kPairs ? turned + (same ? 0 : (p.head_vecs - 2 * turned + 1) / 2) : same ? (s.rotary_dim + v - 1) / v : p.head_vecs;
     if ((int64_t)per_head * heads[i] * kRopeMaxTokens > INT32_MAX) return UA_ERR_SHAPE;
     t.items = per_head * heads[i];
+    bytes += (int64_t)s.batch * s.seqlen * heads[i] * s.head_dim * size;
     t.by_head = make_div(per_head);
     t.by_token = make_div(t.items);
     n_items += t.items;
@@ -250,6 +226,7 @@ static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_t
   if ((int64_t)s.batch * s.seqlen > INT32_MAX) return UA_ERR_SHAPE;
   p.n_tokens = s.batch * s.seqlen;
   if (p.n_tokens == 0 || n_items == 0) return UA_OK;
+  const bool stream = bytes > kRopeStreamBytes;
   p.by_seq = make_div(s.seqlen);
   // Tokens of a workgroup: as many as give each thread an angle, while that leaves four workgroups a CU.
   p.tokens_per_group = std::max(1, std::min({kRopeAngles / p.n_half, kRopeMaxTokens, (kRopeThreads + p.n_half - 1) / p.n_half, p.n_tokens / (4 * kCus)}));
@@ -260,11 +237,11 @@ static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_t
   auto launch = [&](auto element) {
     typedef decltype(element) T;
     if constexpr (sizeof(T) == 2) {
-      if (v == 8) return rope_launch<T, 8>(p, interleaved, way, groups, st);
+      if (v == 8) return rope_launch<T, 8>(p, interleaved, stream, groups, st);
     }
-    if (v == 4) rope_launch<T, 4>(p, interleaved, way, groups, st);
-    else if (v == 2) rope_launch<T, 2>(p, interleaved, way, groups, st);
-    else rope_launch<T, 1>(p, interleaved, way, groups, st);
+    if (v == 4) rope_launch<T, 4>(p, interleaved, stream, groups, st);
+    else if (v == 2) rope_launch<T, 2>(p, interleaved, stream, groups, st);
+    else rope_launch<T, 1>(p, interleaved, stream, groups, st);
   };
   if (s.dtype == UA_FP32) launch(0.f);
   else if (s.dtype == UA_FP16) launch(fp16(0));
