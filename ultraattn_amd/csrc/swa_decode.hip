@@ -7,6 +7,7 @@
 //
 // Bound: HBM, the visible keys and values once per key head.  Two stages of 16 KiB a wave keep 64 to 128 KiB in flight on every CU.
 #include <algorithm>
+#include <cmath>
 #include "swa.h"
 
 namespace ua {
@@ -229,16 +230,31 @@ __global__ __launch_bounds__(64 * kDecWaves) void swa_decode_kernel(const DecPar
 }
 
 struct DecShape { int tiles, row_tiles, parts; };        // 16-row tiles of a workgroup, workgroups of a key head's rows, parts of its keys
-// Parts: as many as make four workgroups a CU of all of them, of at least two blocks a wave.
-static DecShape dec_shape(int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int64_t left, int64_t sinks) {
+// Parts of a key head's keys: what an estimate in microseconds says of the longest caches that the call allows (lengths are on the device).  A round of
+// workgroups on all CUs takes its start and its iterations, or what its keys take from memory; whole caches of a batch differ in length, and the longest
+// ones end alone (64 x 8 of 8192 to 16384 keys, whole 584 us, in four parts 552); parts cost the launch that merges them.
+// us in 1, 2, 4, 8, 16 and 32 parts (sequences x key heads, keys, columns):
+//     1 x 8, 1027, 128    11.7  11.3  10.3  10.3  10.1  10.3        8 x 8, 4000, 128      32.3  27.0  26.8  28.8  36.0  43.7
+//     1 x 8, 8000, 128    56.1  34.5  22.0  15.5  13.0  12.8        16 x 8, 1027, 128     15.6  17.5  22.4  30.0  38.5  63.6
+//     4 x 1, 16000, 128  106.3  59.8  34.3  22.0  16.0  14.5        32 x 8, 2000, 64      24.2  26.0  26.4  29.5  34.6  55.8
+static DecShape dec_shape(int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int head_dim, int64_t left, int64_t sinks) {
   DecShape s;
   const int64_t rows = (int64_t)n_tokens * (n_heads / n_kv_heads);
   s.tiles = rows <= 16 ? 1 : 2;
   s.row_tiles = (int)((rows + 16 * s.tiles - 1) / (16 * s.tiles));
   const int64_t blocks = ((int64_t)room + kDecBlock - 1) / kDecBlock;
-  const int64_t seen = left < 0 ? blocks : std::min(blocks, (std::min<int64_t>(left, kFar) + n_tokens + 2 * kDecBlock - 2) / kDecBlock + (std::min<int64_t>(sinks, room) + kDecBlock - 1) / kDecBlock);
-  const int64_t groups = (int64_t)batch * n_kv_heads * s.row_tiles;
-  s.parts = (int)std::max<int64_t>(1, std::min<int64_t>({kDecMaxParts, 4 * kCus / std::max<int64_t>(groups, 1), seen / (2 * kDecWaves)}));
+  const int64_t seen = left < 0 ? blocks : std::min(blocks, (std::min<int64_t>(left, kFar) + n_tokens + 2 * kDecBlock - 2) / kDecBlock +
+                                                               (std::min<int64_t>(sinks, room) + kDecBlock - 1) / kDecBlock);
+  const double groups = (double)batch * n_kv_heads * s.row_tiles, slots = head_dim == 64 ? 2 * kCus : kCus;
+  const double memory_us = groups * seen * kDecBlock * head_dim * 4 / 7e6;
+  s.parts = 1;
+  double best_us = 1e30;
+  for (int parts = 1; parts <= kDecMaxParts && (parts == 1 || kDecWaves * (parts - 1) < seen); ++parts) {
+    const double rounds = std::ceil(groups * parts / slots), iterations = std::ceil((double)seen / (kDecWaves * parts));
+    const double tail = batch > 1 && left < 0 ? 0.4 * iterations : 0;
+    const double us = 2 * rounds + std::max(0.8 * rounds * iterations, memory_us) + tail + (parts > 1 ? 3.5 + 0.03 * parts : 0);
+    if (us < 0.99 * best_us) { best_us = us; s.parts = parts; }
+  }
   return s;
 }
 static int dec_check(int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int head_dim, int dtype, int64_t left, int64_t sinks, float scale) {
@@ -260,7 +276,7 @@ static void dec_launch(const DecParams& p, int tiles, unsigned n, hipStream_t st
 extern "C" int64_t ua_swa_decode_workspace_bytes(int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int head_dim, int64_t left, int64_t sinks) {
   using namespace ua;
   if (dec_check(batch, n_tokens, n_heads, n_kv_heads, room, head_dim, UA_BF16, left, sinks, 1.f) != UA_OK) return 0;
-  const int parts = dec_shape(batch, n_tokens, n_heads, n_kv_heads, room, left, sinks).parts;
+  const int parts = dec_shape(batch, n_tokens, n_heads, n_kv_heads, room, head_dim, left, sinks).parts;
   const int64_t rows = (int64_t)batch * n_tokens * n_heads;
   return parts > 1 ? parts * (align256(rows * head_dim * 4) + align256(rows * 4)) : 0;
 }
@@ -280,7 +296,7 @@ extern "C" int ua_swa_decode(const void* q, const void* k_cache, const void* v_c
   if (k_strides[1] > (INT32_MAX >> 9) || v_strides[1] > (INT32_MAX >> 9)) return UA_ERR_SHAPE;
   rc = check_device();
   if (rc != UA_OK) return rc;
-  DecShape s = dec_shape(batch, n_tokens, n_heads, n_kv_heads, room, left, sinks);
+  DecShape s = dec_shape(batch, n_tokens, n_heads, n_kv_heads, room, head_dim, left, sinks);
   DecParams p{};
   p.q = q; p.k = k_cache; p.v = v_cache; p.o = o; p.lse = lse; p.lens = lens;
   p.qs = {q_strides[0], q_strides[1], q_strides[2]};

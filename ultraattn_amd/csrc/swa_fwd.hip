@@ -7,6 +7,7 @@
 //
 // The running maximum is raised only where a block's sums show a score far above it, or where a row has not seen a key yet.
 #include <algorithm>
+#include <type_traits>
 #include "swa.h"
 
 namespace ua {
@@ -181,49 +182,76 @@ __global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
 
 // Partial rows of fp32 and their lse, part i of row (b, h, s) at part_o + i * o_part + row * kD:
 //   LSE = log sum_p exp(lse_p),  O = sum_p exp(lse_p - LSE) O_p.
-// Four rows a wave, 16 lanes on a row; bound by the launch and the caches, the partials having just been written.
-template <class T, int kD>
+// kLanes a row: a lane a part for the statistics, then groups of 16 lanes that take the parts' rows in turn.  Bound by the launch and by how many loads
+// follow one another with many parts (a new token against 8000 keys in 31: 16 lanes a row 29.9 us, 64 13.1), by the rows with few (4 heads of 8192 in two:
+// 16 lanes 53.2 us, 64 58.6).
+template <class T, int kD, int kLanes>
 __global__ __launch_bounds__(256) void merge_rows_kernel(const float* part_o, int64_t o_part, const float* part_lse, int64_t lse_part, int n_parts,
                                                          T* o, Strides3 os, float* lse, int n_rows, int n_heads, int seq, Div by_seq, Div by_heads) {
   constexpr int kPer = kD / 16;
-  const int row = blockIdx.x * 16 + (threadIdx.x >> 4), c = threadIdx.x & 15;
+  constexpr int kGroups = kLanes / 16;
+  const int row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes, lane = threadIdx.x % kLanes, c = lane & 15;
   if (row >= n_rows) return;
-  float top = -INFINITY;
-  for (int i = 0; i < n_parts; ++i) top = fmaxf(top, part_lse[i * lse_part + row]);
-  const float at = top == -INFINITY ? 0.f : top;
-  float total = 0.f, acc[kPer] = {};
-  for (int i = 0; i < n_parts; ++i) {
-    const float l = part_lse[i * lse_part + row];
-    if (l == -INFINITY) continue;                        // (such a part left no row)
-    const float w = fast_exp2((l - at) * kLog2e);
-    total += w;
-    const float* x = part_o + i * o_part + (int64_t)row * kD + c * kPer;
+  const float l = lane < n_parts ? part_lse[lane * lse_part + row] : -INFINITY;
+  float top = l;
 #pragma unroll
-    for (int j = 0; j < kPer; j += 4) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(x + j);
+  for (int d = kLanes / 2; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+  const float at = top == -INFINITY ? 0.f : top, w = l == -INFINITY ? 0.f : fast_exp2((l - at) * kLog2e);
+  float total = w, acc[kPer] = {};
 #pragma unroll
-      for (int n = 0; n < 4; ++n) acc[j + n] += w * y[n];
+  for (int d = kLanes / 2; d; d /= 2) total += __shfl_xor(total, d);
+#pragma unroll 4
+  for (int i0 = 0; i0 < n_parts; i0 += kGroups) {
+    const int i = i0 + (lane >> 4);
+    const float f = __shfl(w, i % kLanes, kLanes);
+    if (i < n_parts && f != 0.f) {                       // (a part that saw nothing left no row)
+      const float* x = part_o + i * o_part + (int64_t)row * kD + c * kPer;
+#pragma unroll
+      for (int j = 0; j < kPer; j += 4) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(x + j);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[j + n] += f * y[n];
+      }
     }
   }
-  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
-  const int bh = quotient(row, by_seq), s = row - bh * seq, b = quotient(bh, by_heads), h = bh - b * n_heads;
-  T* out = o + b * os.b + (int64_t)s * os.s + h * os.h + c * kPer;
-  typedef __attribute__((ext_vector_type(kPer))) T vec;
-  vec w;
+  if constexpr (kGroups == 4)
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) w[j] = (T)(acc[j] * inv);
-  *reinterpret_cast<vec*>(out) = w;
-  if (c == 0) lse[row] = total > 0.f || total != total ? at + __builtin_amdgcn_logf(total) * kLn2 : -INFINITY;
+    for (int j = 0; j < kPer; ++j) {
+      acc[j] += __shfl_xor(acc[j], 16);
+      acc[j] += __shfl_xor(acc[j], 32);
+    }
+  const bool any = total > 0.f || total != total;        // (NaN stays)
+  const float inv = any ? 1.f / total : 0.f;
+  const int bh = quotient(row, by_seq), s = row - bh * seq, b = quotient(bh, by_heads), h = bh - b * n_heads;
+  if (lane < 16) {
+    typedef __attribute__((ext_vector_type(kPer))) T vec;
+    vec x;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) x[j] = (T)(acc[j] * inv);
+    *reinterpret_cast<vec*>(o + b * os.b + (int64_t)s * os.s + h * os.h + c * kPer) = x;
+  }
+  if (lane == 0) lse[row] = any ? at + __builtin_amdgcn_logf(total) * kLn2 : -INFINITY;
 }
 
 int swa_merge(const float* part_o, int64_t o_part, const float* part_lse, int64_t lse_part, int n_parts, void* o, const Strides3& os, float* lse,
               int batch, int n_heads, int seq, int head_dim, int dtype, hipStream_t st) {
-  const int n_rows = batch * n_heads * seq, groups = (n_rows + 15) / 16;
-  auto run = [&](auto kernel, auto* out) {
-    kernel<<<groups, 256, 0, st>>>(part_o, o_part, part_lse, lse_part, n_parts, out, os, lse, n_rows, n_heads, seq, make_div(seq), make_div(n_heads));
+  const int n_rows = batch * n_heads * seq;
+  auto run = [&](auto kernel, int lanes, auto* out) {
+    const int rows = 256 / lanes;
+    kernel<<<(n_rows + rows - 1) / rows, 256, 0, st>>>(part_o, o_part, part_lse, lse_part, n_parts, out, os, lse, n_rows, n_heads, seq, make_div(seq),
+                                                       make_div(n_heads));
   };
-  if (dtype == UA_FP16) head_dim == 64 ? run(merge_rows_kernel<fp16, 64>, (fp16*)o) : run(merge_rows_kernel<fp16, 128>, (fp16*)o);
-  else                  head_dim == 64 ? run(merge_rows_kernel<bf16, 64>, (bf16*)o) : run(merge_rows_kernel<bf16, 128>, (bf16*)o);
+  auto by_lanes = [&](auto* out, auto dim) {
+    typedef std::remove_pointer_t<decltype(out)> T;
+    constexpr int kD = decltype(dim)::value;
+    if (n_parts <= 4) run(merge_rows_kernel<T, kD, 16>, 16, out);
+    else              run(merge_rows_kernel<T, kD, 64>, 64, out);
+  };
+  auto by_dim = [&](auto* out) {
+    if (head_dim == 64) by_lanes(out, std::integral_constant<int, 64>{});
+    else                by_lanes(out, std::integral_constant<int, 128>{});
+  };
+  if (dtype == UA_FP16) by_dim((fp16*)o); else by_dim((bf16*)o);
   return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
 }
 
@@ -261,17 +289,17 @@ int swa_fill(SwaParams& p, int batch, int n_heads, int n_kv_heads, int seq_q, in
 
 // Parts that a forward's walks are cut into: what an estimate of the launch's time in microseconds says.  A step takes `alone` where a CU has one
 // workgroup and `shared` where it has two; parts cost a launch for their merge, and each its rows' way through the caches.  us, whole and in
-// 2, 4, 8 and 16 parts (heads, queries x keys, window; what is taken in brackets):
-//     128 columns   4, 2048 causal     37.2   28.7  [25.3]  27.8   39.0          64 columns   8, 2048 causal       28.3  24.6  [24.0]  29.4  39.9
-//                   8, 128 x 4096      67.0   41.4   27.8  [23.6]  27.2                       2, 8192, 2047        32.9 [26.4]  27.2   31.9  44.1
-//                  32, 100 x 16384    256    136     75.5  [50.2]  53.9                       8, 512 causal       [10.6] 12.1   12.4   15.0  19.0
-//                   4, 8192, 2047     [44.5]  53.2   60.7   79.2  137                         2 x 10, 1333 x 2048, 700 [19.5] 25.4
+// 2, 4, 8 and 16 parts (heads, queries x keys, window):
+//     128 columns   4, 2048 causal     37.3   28.6   24.1   26.5   34.4          64 columns   8, 2048 causal       28.2  24.4  22.5  28.6  33.8
+//                   8, 128 x 4096      67.1   41.3   27.0   19.7   18.2                       2, 8192, 2047        32.8  26.0  26.0  32.5  40.0
+//                  32, 100 x 16384    255    135     73.9   48.8   47.2                       8, 512 causal        10.6  12.0  11.7  11.7  13.1
+//                   4, 8192, 2047      44.3   53.1   60.1   83.9  137                         2 x 10, 1333 x 2048, 700  19.5  25.4
 static int fwd_parts(const SwaParams& p, int head_dim) {
   const double lines = (double)p.batch * p.n_heads * p.n_qtiles;
   if (lines == 0 || lines >= 2 * kCus) return 1;
   const SwaSteps s = swa_row_steps(p);
   const double alone = head_dim == 64 ? 0.75 : 1.0, shared = head_dim == 64 ? 1.2 : 2.05;
-  const double part_us = 0.3 + (double)p.batch * p.n_heads * p.seq_q * head_dim * 8e-7;      // written and read
+  const double part_us = 0.15 + (double)p.batch * p.n_heads * p.seq_q * head_dim * 8e-7;      // written and read
   int best = 1;
   double best_us = 1e30;
   for (int parts = 1; parts <= UA_MAX_PARTS && (parts == 1 || 2 * parts <= s.most); ++parts) {
