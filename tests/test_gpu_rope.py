@@ -214,6 +214,9 @@ def test_refusals():
            lambda: ua.rope_append(q, k, k, cache, cache, lens.long(), f), lambda: ua.rope_append(q, k, k, cache, cache, lens[:1], f),
            lambda: ua.rope_append(q, k, k[:, :1], cache, cache, lens, f), lambda: ua.rope_append(q, k, k, cache[:1].expand(2, 8, 2, 64), cache, lens, f),
            lambda: ua.rope_append(q, k, k, cache, cache, lens.cpu(), f)]
+    same = rows(2, 4, 4, 64, torch.bfloat16, 7)
+    bad += [lambda: ua.rope_fwd(q, same, f, q_out=same), lambda: ua.rope_fwd(q, same, f, k_out=q), lambda: ua.rope_fwd(q, same, f, q_out=q, k_out=q),
+            lambda: ua.rope_append(q, k, k, cache, cache, lens, f)]
     before = q.clone(), k.clone(), cache.clone()
     for i, call in enumerate(bad):
         with pytest.raises((ValueError, TypeError)):

@@ -189,6 +189,8 @@ def test_refusals():
            lambda: ua.swa_bwd(do, q, k, v, out, lse, dk=q), lambda: ua.swa_bwd(do, q, k, v, out, lse, dk=k[:, :, :1].expand_as(k)),
            lambda: ua.swa_bwd(do, q, k, v, None, lse, softmax_d=lse[:, :2]), lambda: ua.swa_bwd(do, q, k, v, out, lse, softmax_scale=-1.0),
            lambda: ua.swa_bwd(do, q, k, v, out, lse, (-3, 0)), lambda: ua.swa_bwd(do, q, k, v, out.cpu(), lse), lambda: ua.swa_bwd(do, q, k, v, out, lse.cpu())]
+    bad += [lambda: ua.swa_bwd(do, q, k, v, out, lse, dq=q), lambda: ua.swa_bwd(do, q, k, v, out, lse, dq=do), lambda: ua.swa_bwd(do, q, k, v, out, lse, dk=k),
+            lambda: ua.swa_bwd(do, q, k, v, out, lse, dk=out[:, :, :2], dv=out[:, :, :2])]
     for i, call in enumerate(bad):
         with pytest.raises((ValueError, TypeError)):
             call()

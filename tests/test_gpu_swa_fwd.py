@@ -109,6 +109,14 @@ def test_few_rows_and_many_keys(dtype, dim, seq_q, seq_k, window, sinks):
     run(q, k, v, window, sinks, q_start=40)                         # parts in which some rows see nothing
 
 
+def test_out_in_place_of_q():
+    for seq_k in (200, 5000):                                        # whole, and cut into parts
+        q, k, v, _ = inputs(1, 150, seq_k, 2, 2, 64, torch.bfloat16)
+        want = ua.swa_fwd(q, k, v)[0]
+        x = q.clone()
+        assert ua.swa_fwd(x, k, v, out=x)[0] is x and torch.equal(x, want)
+
+
 def test_larger_grids():
     q, k, v, _ = inputs(3, 1111, 1111, 24, 8, 128, torch.bfloat16)
     run(q, k, v, (256, 0), 4)
@@ -163,6 +171,7 @@ def test_refusals():
            lambda: ua.swa_fwd(q, k, v, lse=torch.empty(2, 16, 4, device=DEV)), lambda: ua.swa_fwd(q, k, v, lse=torch.empty(2, 4, 16)),
            lambda: ua.swa_fwd(q, k.cpu(), v), lambda: ua.swa_fwd(q.cpu(), k.cpu(), v.cpu()), lambda: ua.swa_fwd(q[:, :, 0], k, v),
            lambda: ua.swa_fwd(q.transpose(2, 3), k, v), lambda: ua.swa_fwd(q, k[:, :, :0], v[:, :, :0])]
+    bad += [lambda: ua.swa_fwd(q, k.repeat(1, 1, 2, 1), q, out=q)]
     for i, call in enumerate(bad):
         with pytest.raises((ValueError, TypeError, RuntimeError)):
             call()

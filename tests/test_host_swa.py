@@ -22,7 +22,7 @@ def test_forward_refuses(lib):
     assert fwd(lib, q=None) == -1 and fwd(lib, k=None) == -1 and fwd(lib, lse=None) == -1 and fwd(lib, qs=None) == -1
     assert fwd(lib, heads=3) == -2 and fwd(lib, kv=0) == -2 and fwd(lib, batch=-1) == -2 and fwd(lib, sq=-1) == -2 and fwd(lib, sk=2 ** 29) == -2
     assert fwd(lib, left=-2) == -2 and fwd(lib, right=-2) == -2 and fwd(lib, sinks=-1) == -2 and fwd(lib, start=2 ** 61) == -2
-    assert fwd(lib, batch=2 ** 20, heads=2 ** 11, sq=2 ** 20) == -2
+    assert fwd(lib, batch=2 ** 20, heads=2 ** 11, sq=2 ** 20) == -2 and fwd(lib, batch=2 ** 20, heads=2 ** 12, kv=1, sq=0) == -2
     assert fwd(lib, dim=96) == -3 and fwd(lib, dtype=2) == -3 and fwd(lib, scale=0.0) == -3 and fwd(lib, scale=math.nan) == -3
     assert fwd(lib, q=BUF + 2) == -4 and fwd(lib, qs=BAD) == -4 and fwd(lib, os=NONE) == -4
     assert fwd(lib, batch=0, q=None) == 0 and fwd(lib, sq=0) == 0                    # nothing to do

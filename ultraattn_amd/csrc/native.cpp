@@ -684,6 +684,12 @@ at::Tensor result(Slot& s, const char* name, const at::Tensor& ref) {
   check_written(name, s.t);
   return s.t;
 }
+// A result that other workgroups still read as an operand, or that two results share, would race.
+void check_apart(const char* name, const at::Tensor& written, std::initializer_list<const at::Tensor*> others) {
+  for (const at::Tensor* o : others)
+    if (written.numel() > 0 && o->numel() > 0 && written.data_ptr() == o->data_ptr())
+      fail(PyExc_ValueError, std::string(name) + " must not be another operand or result of the call");
+}
 const double* frequencies(const at::Tensor& f, const at::Tensor& x, int64_t& rotary) {
   if (f.scalar_type() != at::kDouble || f.dim() != 1 || !f.is_contiguous() || f.device() != x.device())
     fail(PyExc_ValueError, "freqs must be a contiguous float64 vector on the tensors' device");
@@ -736,8 +742,13 @@ PyObject* rope(PyObject* const* a) {
   Slot qo(a[8]), ko(a[9]);
   if (!has_k && ko.given) fail(PyExc_ValueError, "k_out without k");
   result(qo, "q_out", q);
-  if (has_k) result(ko, "k_out", k);
+  if (has_k) {
+    result(ko, "k_out", k);
+    check_apart("q_out", qo.t, {&k, &ko.t});
+    check_apart("k_out", ko.t, {&q});
+  }
   const On on(q);
+  init_device(on.device);
   call("ua_rope", [&] {
     return ua_rope(q.data_ptr(), has_k ? k.data_ptr() : nullptr, qo.t.data_ptr(), has_k ? ko.t.data_ptr() : nullptr, f, pos, pos64, pos_b, pos_s, start,
                    (int)q.size(0), (int)q.size(1), (int)q.size(2), has_k ? (int)k.size(2) : 0, (int)q.size(3), (int)rotary, dt, interleaved, inverse,
@@ -773,7 +784,11 @@ PyObject* rope_append(PyObject* const* a) {
   const float scale = positive(a[8], "scale");
   Slot qo(a[9]);
   result(qo, "q_out", q);
+  check_apart("q_out", qo.t, {&k, &v, &kc, &vc});
+  check_apart("k_cache", kc, {&q, &k, &v, &vc});
+  check_apart("v_cache", vc, {&q, &k, &v});
   const On on(q);
+  init_device(on.device);
   call("ua_rope_append", [&] {
     return ua_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), qo.t.data_ptr(), kc.data_ptr(), vc.data_ptr(), f, lens, (int)q.size(0),
                           (int)q.size(1), (int)q.size(2), (int)k.size(2), (int)kc.size(1), (int)q.size(3), (int)rotary, dt, interleaved, scale, Strides(q),
@@ -830,7 +845,9 @@ PyObject* swa_forward(PyObject* const* a) {
   result(out, "out", q);
   if (lse.given) check_lse("lse", lse.t = tensor(lse.given, "lse"), q);
   else lse.t = stat_of(q);
+  check_apart("out", out.t, {&k, &v});
   const On on(q);
+  init_device(on.device);
   const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), sq = (int)q.size(1), sk = (int)k.size(1), D = (int)q.size(3);
   const at::Tensor ws = scratch(ua_swa_workspace_bytes(B, H, Hk, sq, sk, D, w.q_start, w.k_start, w.left, w.right, w.sinks), q);
   call("ua_swa_fwd", [&] {
@@ -855,8 +872,12 @@ PyObject* swa_backward(PyObject* const* a) {
   result(dq, "dq", q);
   result(dk, "dk", k);
   result(dv, "dv", v);
+  check_apart("dq", dq.t, {&dout, &q, &k, &v, &dk.t, &dv.t});
+  check_apart("dk", dk.t, {&dout, &q, &k, &v, &dv.t});
+  check_apart("dv", dv.t, {&dout, &q, &k, &v});
   const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), sq = (int)q.size(1), sk = (int)k.size(1), D = (int)q.size(3);
   const On on(q);
+  init_device(on.device);
   at::Tensor delta;
   if (a[9] != Py_None) {
     delta = tensor(a[9], "softmax_d");
@@ -897,7 +918,9 @@ PyObject* swa_decode(PyObject* const* a) {
   result(out, "out", q);
   if (lse.given) check_lse("lse", lse.t = tensor(lse.given, "lse"), q);
   else lse.t = stat_of(q);
+  check_apart("out", out.t, {&k, &v});
   const On on(q);
+  init_device(on.device);
   const int B = (int)q.size(0), T = (int)q.size(1), H = (int)q.size(2), Hk = (int)k.size(2), room = (int)k.size(1), D = (int)q.size(3);
   const at::Tensor ws = scratch(ua_swa_decode_workspace_bytes(B, T, H, Hk, room, D, left, sinks), q);
   call("ua_swa_decode", [&] {

@@ -230,7 +230,8 @@ static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_t
   p.by_seq = make_div(s.seqlen);
   // Tokens of a workgroup: as many as give each thread an angle, while that leaves four workgroups a CU.
   p.tokens_per_group = std::max(1, std::min({kRopeAngles / p.n_half, kRopeMaxTokens, (kRopeThreads + p.n_half - 1) / p.n_half, p.n_tokens / (4 * kCus)}));
-  const int lines = (p.n_tokens + p.tokens_per_group - 1) / p.tokens_per_group;
+  const uint32_t lines = (uint32_t)(((int64_t)p.n_tokens + p.tokens_per_group - 1) / p.tokens_per_group);
+  if (lines > UINT32_MAX / kRopeThreads) return UA_ERR_SHAPE;              // (a launch counts its threads in 32 bits)
   const dim3 groups(lines, lines <= 4 * kCus ? n_tensors : 1);
   const int rc = check_device();
   if (rc != UA_OK) return rc;

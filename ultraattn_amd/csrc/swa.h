@@ -10,6 +10,7 @@ namespace ua {
 typedef _Float16 fp16;
 constexpr int kFar = 1 << 29;
 constexpr int64_t kSwaMaxLen = 1 << 28;            // of queries and keys: no sum of a row and a bound leaves 32 bits
+constexpr int64_t kSwaMaxGroups = UINT32_MAX / 256; // a launch counts its threads in 32 bits
 constexpr int kSwaRows = 128;                      // of a workgroup's tile, 32 a wave
 constexpr int kSwaBlock = 64;                      // rows of the other side that a step goes through
 

@@ -563,7 +563,7 @@ extern "C" int ua_swa_bwd_delta(const void* o, const void* dout, const void* q, 
   int rc = swa_fill(p, batch, n_heads, n_kv_heads, seqlen_q, seqlen_k, head_dim, dtype, q_start, k_start, left, right, sinks, softmax_scale);
   if (rc != UA_OK) return rc;
   const int64_t tokens = (seqlen_q + 15) / 16, heads = (n_heads + 3) / 4;
-  if (batch * tokens * heads > INT32_MAX) return UA_ERR_SHAPE;
+  if (batch * tokens * heads > (int64_t)UINT32_MAX / (8 * head_dim)) return UA_ERR_SHAPE;
   if ((int64_t)batch * seqlen_q == 0) return UA_OK;
   if (!o || !dout || !q || !lse || !delta || (seqlen_k > 0 && (!k || !v))) return UA_ERR_NULL;
   for (const int64_t* s : {o_strides, do_strides, q_strides, k_strides, v_strides}) {

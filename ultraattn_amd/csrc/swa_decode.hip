@@ -324,7 +324,7 @@ extern "C" int ua_swa_decode(const void* q, const void* k_cache, const void* v_c
   p.by_parts = make_div(p.n_parts);
   const hipStream_t st = (hipStream_t)stream;
   const int64_t n = (int64_t)batch * n_kv_heads * p.n_tiles * p.n_parts;
-  if (n > INT32_MAX) return UA_ERR_SHAPE;
+  if (n > kSwaMaxGroups) return UA_ERR_SHAPE;
   if (dtype == UA_FP16) head_dim == 64 ? dec_launch<fp16, 64>(p, s.tiles, (unsigned)n, st) : dec_launch<fp16, 128>(p, s.tiles, (unsigned)n, st);
   else                  head_dim == 64 ? dec_launch<bf16, 64>(p, s.tiles, (unsigned)n, st) : dec_launch<bf16, 128>(p, s.tiles, (unsigned)n, st);
   if (hipGetLastError() != hipSuccess) return UA_ERR_LAUNCH;

@@ -264,8 +264,9 @@ int swa_fill(SwaParams& p, int batch, int n_heads, int n_kv_heads, int seq_q, in
              int64_t left, int64_t right, int64_t sinks, float softmax_scale) {
   constexpr int64_t kMost = int64_t(1) << 60;
   if (batch < 0 || n_heads <= 0 || n_kv_heads <= 0 || seq_q < 0 || seq_k < 0 || n_heads % n_kv_heads) return UA_ERR_SHAPE;
-  if (seq_q > kSwaMaxLen || seq_k > kSwaMaxLen || (int64_t)batch * n_heads * ((seq_q + kSwaRows - 1) / kSwaRows) > INT32_MAX / UA_MAX_PARTS ||
-      (int64_t)batch * n_heads * ((seq_k + kSwaRows - 1) / kSwaRows) > INT32_MAX / UA_MAX_PARTS)
+  const int64_t heads = (int64_t)batch * n_heads;
+  if (seq_q > kSwaMaxLen || seq_k > kSwaMaxLen || heads > kSwaMaxGroups || heads * ((seq_q + kSwaRows - 1) / kSwaRows) > kSwaMaxGroups / 2 ||
+      heads * ((seq_k + kSwaRows - 1) / kSwaRows) > kSwaMaxGroups / 2)
     return UA_ERR_SHAPE;
   if (q_start > kMost || q_start < -kMost || k_start > kMost || k_start < -kMost || left < -1 || right < -1 || left > kMost || right > kMost || sinks < 0 ||
       sinks > kMost)
