@@ -516,21 +516,30 @@ struct BwdCut {
   int row_parts, n_sink, col_parts[2];            // n_sink: tiles of the first run of columns
   int64_t dq_bytes, col_bytes[2], total;          // of a part; of a part's dK
 };
-// Walks are cut to about what a workgroup has on average with two of them on every CU, if they are much longer and there is something to
-// gain beside the launch that adds the parts.  Lengths are counted in products of 64 rows, a column's step has four of them and a row's three.
+// Walks are cut to about what a workgroup has on average with two of them on every CU, `each`, where the time that the longest take beyond that
+// is well above what the parts cost: their rows' way through memory and the launch that adds them.  Lengths are counted in products of 64 rows (0.8 us where
+// two workgroups share every CU, 0.5 where they hardly do); a column's step has four of them and a row's three.  us, whole and cut as taken here:
+//     128 columns   16 heads, 4096, window 1024, 4 sinks      155   120        64 columns   14 heads on 2, 3000, window 464        99    38
+//                   4, 2048 causal                           61.7  44.2                     2, 8192, window 2048, 70 sinks        184    54
+//                   32 on 8, 100 x 16384                      374   128                     2 x 10 on 5, 1333 x 2048, window 700  47.1  43.5
+//                   8 on 2, 16384, window 4096, 16 sinks     2085   728                     (the sinks' columns alone: 740)
 static BwdCut bwd_cut(const SwaParams& p, int head_dim, bool cut) {
   BwdCut c{1, 0, {1, 1}, 0, {0, 0}, 0};
   const double cols = (double)p.batch * p.n_kv_heads, rows = (double)p.batch * p.n_heads * p.n_qtiles;
   if (!cut || cols * p.n_ktiles == 0 || rows == 0) return c;
   auto column = [&](int t) { return SwaColumn(t * kSwaRows, imin((t + 1) * kSwaRows, p.seq_k) - 1, p.hi, p.lo, p.sinks, p.seq_q).n * p.group; };
-  const int sink_tiles = std::min((p.sinks + kSwaRows - 1) / kSwaRows, p.n_ktiles);
-  const SwaSteps row = swa_row_steps(p), sink = swa_steps(0, sink_tiles, column), col = swa_steps(sink_tiles, p.n_ktiles - sink_tiles, column);
-  const double work = 3 * rows * row.mean + 4 * cols * (sink_tiles * sink.mean + (p.n_ktiles - sink_tiles) * col.mean);
-  const double each = std::max(work / (2 * kCus), 32.0);
-  auto parts = [&](double products) { return products > 1.5 * each + 24 ? (int)std::min(std::ceil(products / each), (double)UA_MAX_PARTS) : 1; };
-  c.row_parts = parts(3.0 * row.most);
-  c.col_parts[0] = parts(4.0 * sink.most);
-  c.col_parts[1] = parts(4.0 * col.most);
+  const int sink_tiles = std::min((p.sinks + kSwaRows - 1) / kSwaRows, p.n_ktiles), other_tiles = p.n_ktiles - sink_tiles;
+  const SwaSteps row = swa_row_steps(p), sink = swa_steps(0, sink_tiles, column), col = swa_steps(sink_tiles, other_tiles, column);
+  const double work = 3 * rows * row.mean + 4 * cols * (sink_tiles * sink.mean + other_tiles * col.mean);
+  const double each = std::max(work / (2 * kCus), 32.0), product_us = each > 64 ? 0.8 : 0.5, row_bytes = head_dim * 4;
+  auto parts = [&](double products, double part_bytes) {
+    const int n = (int)std::min(std::ceil(products / each), (double)UA_MAX_PARTS);
+    const double gain = product_us * (products - std::max(products / n, each)), cost = 6 + 2 * n * part_bytes / 5e6;
+    return gain > 1.3 * cost ? n : 1;
+  };
+  c.row_parts = parts(3.0 * row.most, rows * kSwaRows * row_bytes);
+  c.col_parts[0] = parts(4.0 * sink.most, 2 * cols * sink_tiles * kSwaRows * row_bytes);
+  c.col_parts[1] = parts(4.0 * col.most, 2 * cols * other_tiles * kSwaRows * row_bytes);
   if (c.col_parts[0] == c.col_parts[1]) c.col_parts[0] = 1;
   else c.n_sink = sink_tiles;
   if (c.row_parts > 1) c.dq_bytes = align256((int64_t)p.batch * p.n_heads * p.seq_q * head_dim * 4);
