@@ -347,7 +347,8 @@ int ua_rope_append(const void *q, const void *k, const void *v, void *q_out, voi
  * Few long walks are cut into parts, whose fp32 results are merged in a second launch, if `workspace` (16-byte aligned,
  * overwritten) holds ua_swa_workspace_bytes(); calls that overlap in time need one each.  With less nothing is cut.
  * A key's or value's NaN or infinity reaches rows that see it, and may reach rows whose tile of 128 sees it (so it is with the gradients, and with
- * ua_swa_decode's blocks of 32).  o may be q; no other result may be an operand. */
+ * ua_swa_decode's blocks of 32).  o may be q itself, element for element; no result may otherwise overlap an
+ * operand or another result. */
 int64_t ua_swa_workspace_bytes(int batch, int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim,
                                int64_t q_start, int64_t k_start, int64_t left, int64_t right, int64_t sinks);
 int ua_swa_fwd(const void *q, const void *k, const void *v, void *o, float *lse,

@@ -684,11 +684,52 @@ at::Tensor result(Slot& s, const char* name, const at::Tensor& ref) {
   check_written(name, s.t);
   return s.t;
 }
+// Whether two tensors of one type have an element in common: whether the distance of their starts, in elements, is a sum of steps that both can take.
+// Axes of both by falling stride, each with the steps it allows; what the axes below reach leaves few to try (the parts of a packed row: one or two).
+struct Step { int64_t stride, lo, hi; };
+bool reaches(const Step* s, size_t n, int64_t distance, int& budget) {
+  if (n == 0) return distance == 0;
+  int64_t least = 0, most = 0;                              // of the axes below
+  for (size_t i = 1; i < n; ++i) { least += s[i].stride * s[i].lo; most += s[i].stride * s[i].hi; }
+  auto down = [](int64_t a, int64_t b) { return a / b - (a % b != 0 && a < 0); };
+  const int64_t first = std::max(s[0].lo, -down(most - distance, s[0].stride)), last = std::min(s[0].hi, down(distance - least, s[0].stride));
+  for (int64_t c = first; c <= last; ++c) {
+    if (--budget < 0) return true;                          // (no layout of rows gets here: taken as shared)
+    if (reaches(s + 1, n - 1, distance - c * s[0].stride, budget)) return true;
+  }
+  return false;
+}
+bool share(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0 || a.device() != b.device()) return false;
+  const int64_t bytes = (int64_t)((intptr_t)b.data_ptr() - (intptr_t)a.data_ptr()), size = a.element_size();
+  std::vector<Step> s;
+  int64_t least = 0, most = 0;
+  for (const at::Tensor* t : {&a, &b})
+    for (int64_t i = 0; i < t->dim(); ++i) {
+      const int64_t n = t->size(i) - 1, stride = t->stride(i);
+      if (n == 0 || stride == 0) continue;
+      const bool ours = t == &a;
+      (ours ? most : least) += (ours ? n : -n) * stride;
+      auto same = std::find_if(s.begin(), s.end(), [&](const Step& x) { return x.stride == stride; });
+      if (same == s.end()) same = s.insert(s.end(), Step{stride, 0, 0});
+      (ours ? same->hi : same->lo) += ours ? n : -n;
+    }
+  if (bytes > (most + 1) * size || bytes < (least - 1) * size) return false;      // apart altogether
+  if (bytes % size) return true;
+  std::sort(s.begin(), s.end(), [](const Step& x, const Step& y) { return x.stride > y.stride; });
+  int budget = 4096;
+  return reaches(s.data(), s.size(), bytes / size, budget);
+}
 // A result that other workgroups still read as an operand, or that two results share, would race.
 void check_apart(const char* name, const at::Tensor& written, std::initializer_list<const at::Tensor*> others) {
   for (const at::Tensor* o : others)
-    if (written.numel() > 0 && o->numel() > 0 && written.data_ptr() == o->data_ptr())
-      fail(PyExc_ValueError, std::string(name) + " must not be another operand or result of the call");
+    if (share(written, *o)) fail(PyExc_ValueError, std::string(name) + " must not overlap another operand or result of the call");
+}
+// A result that may be its operand, element for element, but not another view of its memory.
+void check_in_place(const char* name, const at::Tensor& written, const at::Tensor& x) {
+  bool same = written.data_ptr() == x.data_ptr();
+  for (int64_t i = 0; i < x.dim(); ++i) same = same && (x.size(i) <= 1 || written.stride(i) == x.stride(i));
+  if (!same && share(written, x)) fail(PyExc_ValueError, std::string(name) + " must be its operand's own memory or overlap none of it");
 }
 const double* frequencies(const at::Tensor& f, const at::Tensor& x, int64_t& rotary) {
   if (f.scalar_type() != at::kDouble || f.dim() != 1 || !f.is_contiguous() || f.device() != x.device())
@@ -746,7 +787,9 @@ PyObject* rope(PyObject* const* a) {
     result(ko, "k_out", k);
     check_apart("q_out", qo.t, {&k, &ko.t});
     check_apart("k_out", ko.t, {&q});
+    check_in_place("k_out", ko.t, k);
   }
+  check_in_place("q_out", qo.t, q);
   const On on(q);
   init_device(on.device);
   call("ua_rope", [&] {
@@ -785,6 +828,7 @@ PyObject* rope_append(PyObject* const* a) {
   Slot qo(a[9]);
   result(qo, "q_out", q);
   check_apart("q_out", qo.t, {&k, &v, &kc, &vc});
+  check_in_place("q_out", qo.t, q);
   check_apart("k_cache", kc, {&q, &k, &v, &vc});
   check_apart("v_cache", vc, {&q, &k, &v});
   const On on(q);
@@ -846,6 +890,7 @@ PyObject* swa_forward(PyObject* const* a) {
   if (lse.given) check_lse("lse", lse.t = tensor(lse.given, "lse"), q);
   else lse.t = stat_of(q);
   check_apart("out", out.t, {&k, &v});
+  check_in_place("out", out.t, q);
   const On on(q);
   init_device(on.device);
   const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), sq = (int)q.size(1), sk = (int)k.size(1), D = (int)q.size(3);
@@ -919,6 +964,7 @@ PyObject* swa_decode(PyObject* const* a) {
   if (lse.given) check_lse("lse", lse.t = tensor(lse.given, "lse"), q);
   else lse.t = stat_of(q);
   check_apart("out", out.t, {&k, &v});
+  check_in_place("out", out.t, q);
   const On on(q);
   init_device(on.device);
   const int B = (int)q.size(0), T = (int)q.size(1), H = (int)q.size(2), Hk = (int)k.size(2), room = (int)k.size(1), D = (int)q.size(3);

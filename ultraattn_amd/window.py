@@ -2,7 +2,7 @@
 
 Host side of ``ua_swa_*`` in ``include/ultraattn.h``, beside the block-sparse operators of ``ops.py`` and in their manner: row tensors
 ``[B, S, H, D]`` with any (batch, token, head) strides, ``lse`` ``[B, H, S]`` fp32 in natural logarithm, results written in place when
-given, everything on the current CUDA(HIP) stream, nothing synchronises.  Types are bf16 and fp16, D is 64 or 128, lengths are arbitrary, and keys
+given (``out`` may be ``q`` itself; results overlap nothing else), everything on the current CUDA(HIP) stream, nothing synchronises.  Types are bf16 and fp16, D is 64 or 128, lengths are arbitrary, and keys
 may have fewer heads than queries (each serves ``Hq / Hk`` consecutive ones).
 
 Query i is at position ``q_start + i`` and key j at ``k_start + j``.  With ``window=(left, right)`` a query at p sees the keys at
