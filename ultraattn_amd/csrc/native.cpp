@@ -699,23 +699,32 @@ bool reaches(const Step* s, size_t n, int64_t distance, int& budget) {
   }
   return false;
 }
+inline intptr_t end_of(const at::Tensor& t, intptr_t begin, int64_t size) {        // the byte behind the last element; `begin` if there is none
+  const int64_t *n = t.sizes().data(), *stride = t.strides().data();
+  int64_t last = 0;
+  for (int64_t i = 0; i < (int64_t)t.sizes().size(); ++i) {
+    if (n[i] == 0) return begin;
+    last += (n[i] - 1) * stride[i];
+  }
+  return begin + (last + 1) * size;
+}
 bool share(const at::Tensor& a, const at::Tensor& b) {
-  if (a.numel() == 0 || b.numel() == 0 || a.device() != b.device()) return false;
-  const int64_t bytes = (int64_t)((intptr_t)b.data_ptr() - (intptr_t)a.data_ptr()), size = a.element_size();
+  const int64_t size = a.element_size();
+  const intptr_t from_a = (intptr_t)a.data_ptr(), from_b = (intptr_t)b.data_ptr();
+  const intptr_t to_a = end_of(a, from_a, size), to_b = end_of(b, from_b, size);
+  if (from_a >= to_b || from_b >= to_a || from_a == to_a || from_b == to_b) return false;      // apart altogether, as most are
+  const int64_t bytes = from_b - from_a;
+  if (bytes % size) return true;
   std::vector<Step> s;
-  int64_t least = 0, most = 0;
   for (const at::Tensor* t : {&a, &b})
     for (int64_t i = 0; i < t->dim(); ++i) {
       const int64_t n = t->size(i) - 1, stride = t->stride(i);
       if (n == 0 || stride == 0) continue;
       const bool ours = t == &a;
-      (ours ? most : least) += (ours ? n : -n) * stride;
       auto same = std::find_if(s.begin(), s.end(), [&](const Step& x) { return x.stride == stride; });
       if (same == s.end()) same = s.insert(s.end(), Step{stride, 0, 0});
       (ours ? same->hi : same->lo) += ours ? n : -n;
     }
-  if (bytes > (most + 1) * size || bytes < (least - 1) * size) return false;      // apart altogether
-  if (bytes % size) return true;
   std::sort(s.begin(), s.end(), [](const Step& x, const Step& y) { return x.stride > y.stride; });
   int budget = 4096;
   return reaches(s.data(), s.size(), bytes / size, budget);
@@ -785,11 +794,13 @@ PyObject* rope(PyObject* const* a) {
   result(qo, "q_out", q);
   if (has_k) {
     result(ko, "k_out", k);
-    check_apart("q_out", qo.t, {&k, &ko.t});
-    check_apart("k_out", ko.t, {&q});
-    check_in_place("k_out", ko.t, k);
+    if (qo.given) check_apart("q_out", qo.t, {&k, &ko.t});
+    if (ko.given) {
+      check_apart("k_out", ko.t, {&q});
+      check_in_place("k_out", ko.t, k);
+    }
   }
-  check_in_place("q_out", qo.t, q);
+  if (qo.given) check_in_place("q_out", qo.t, q);
   const On on(q);
   init_device(on.device);
   call("ua_rope", [&] {
@@ -827,8 +838,10 @@ PyObject* rope_append(PyObject* const* a) {
   const float scale = positive(a[8], "scale");
   Slot qo(a[9]);
   result(qo, "q_out", q);
-  check_apart("q_out", qo.t, {&k, &v, &kc, &vc});
-  check_in_place("q_out", qo.t, q);
+  if (qo.given) {
+    check_apart("q_out", qo.t, {&k, &v, &kc, &vc});
+    check_in_place("q_out", qo.t, q);
+  }
   check_apart("k_cache", kc, {&q, &k, &v, &vc});
   check_apart("v_cache", vc, {&q, &k, &v});
   const On on(q);
@@ -889,8 +902,10 @@ PyObject* swa_forward(PyObject* const* a) {
   result(out, "out", q);
   if (lse.given) check_lse("lse", lse.t = tensor(lse.given, "lse"), q);
   else lse.t = stat_of(q);
-  check_apart("out", out.t, {&k, &v});
-  check_in_place("out", out.t, q);
+  if (out.given) {
+    check_apart("out", out.t, {&k, &v});
+    check_in_place("out", out.t, q);
+  }
   const On on(q);
   init_device(on.device);
   const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), sq = (int)q.size(1), sk = (int)k.size(1), D = (int)q.size(3);
@@ -917,9 +932,9 @@ PyObject* swa_backward(PyObject* const* a) {
   result(dq, "dq", q);
   result(dk, "dk", k);
   result(dv, "dv", v);
-  check_apart("dq", dq.t, {&dout, &q, &k, &v, &dk.t, &dv.t});
-  check_apart("dk", dk.t, {&dout, &q, &k, &v, &dv.t});
-  check_apart("dv", dv.t, {&dout, &q, &k, &v});
+  if (dq.given) check_apart("dq", dq.t, {&dout, &q, &k, &v, &dk.t, &dv.t});
+  if (dk.given) check_apart("dk", dk.t, {&dout, &q, &k, &v, &dv.t});
+  if (dv.given) check_apart("dv", dv.t, {&dout, &q, &k, &v});
   const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), sq = (int)q.size(1), sk = (int)k.size(1), D = (int)q.size(3);
   const On on(q);
   init_device(on.device);
@@ -963,8 +978,10 @@ PyObject* swa_decode(PyObject* const* a) {
   result(out, "out", q);
   if (lse.given) check_lse("lse", lse.t = tensor(lse.given, "lse"), q);
   else lse.t = stat_of(q);
-  check_apart("out", out.t, {&k, &v});
-  check_in_place("out", out.t, q);
+  if (out.given) {
+    check_apart("out", out.t, {&k, &v});
+    check_in_place("out", out.t, q);
+  }
   const On on(q);
   init_device(on.device);
   const int B = (int)q.size(0), T = (int)q.size(1), H = (int)q.size(2), Hk = (int)k.size(2), room = (int)k.size(1), D = (int)q.size(3);
