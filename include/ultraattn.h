@@ -346,8 +346,9 @@ int ua_rope_append(const void *q, const void *k, const void *v, void *q_out, voi
  * to dtype for its product with V, as it is in ua_bsa_fwd.
  * Few long walks are cut into parts, whose fp32 results are merged in a second launch, if `workspace` (16-byte aligned,
  * overwritten) holds ua_swa_workspace_bytes(); calls that overlap in time need one each.  With less nothing is cut.
- * A key's or value's NaN or infinity reaches rows that see it, and may reach rows whose tile of 128 sees it (so it is with the gradients, and with
- * ua_swa_decode's blocks of 32).  o may be q itself, element for element; no result may otherwise overlap an
+ * A key's or value's NaN or infinity reaches rows that see it, and may reach others in a tile of 128 rows (from row 0 on; ua_swa_decode: of up to 32 rows of
+ * a key head) of which one sees it, not rows of other tiles.  In the gradients the keys are tiles likewise: NaN in a query, or in its row of dout, may reach
+ * the keys of tiles that it sees.  o may be q itself, element for element; no result may otherwise overlap an
  * operand or another result. */
 int64_t ua_swa_workspace_bytes(int batch, int n_heads, int n_kv_heads, int seqlen_q, int seqlen_k, int head_dim,
                                int64_t q_start, int64_t k_start, int64_t left, int64_t right, int64_t sinks);

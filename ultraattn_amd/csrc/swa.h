@@ -1,7 +1,7 @@
 // What the sliding-window attention kernels share: which keys a row sees, element types, LDS layouts for heads of 64 and 128, row tiles.
 //
 // Row r (query) of a call sees key j iff  j <= r + hi  and  (j >= r + lo  or  j < sinks);  hi and lo hold the window and the
-// difference of the positions of query 0 and key 0, clamped to +-kFar, which is beyond any length.
+// difference of the positions of query 0 and key 0, clamped to +-kFar, which is beyond any length.  What nothing in a workgroup's tile sees may be NaN.
 #pragma once
 #include "ua_common.h"
 
@@ -66,6 +66,21 @@ struct SwaHead {
     return at_b(row, 4 * m + 2 * (lane >> 4 & 1) + ((i & 3) >> 1)) + (i & 1) * 8;
   }
 };
+// Zeros in rows from .. to - 1 of a tile in LDS, for a wave whose next reads are of them.  A walk's first block may hold rows before the first one that
+// anything in the workgroup's tile sees: their weights are 0, which would make NaN of NaN or infinity.  (Rows behind the last one seen are not
+// copied.)  Every wave that reads the block does this itself, so none waits for another; 16 writes at the most.
+template <int kD, int kPitch, int kAlso = 0>                       // kAlso: bytes to a second tile of which the same rows are cleared
+__device__ __forceinline__ void lds_clear_rows(uint32_t tile, int from, int to) {
+  constexpr int kCopyRows = 1024 / (2 * kD);
+  for (int u = from / kCopyRows; u * kCopyRows < to; ++u) {
+    const int lane = fresh_lane(), r = u * kCopyRows + lane / (kD / 8);
+    if (r >= from && r < to) {
+      lds_put(tile + u * kPitch + 16 * lane, u32x4{0, 0, 0, 0});
+      if (kAlso) lds_put(tile + u * kPitch + 16 * lane + kAlso, u32x4{0, 0, 0, 0});
+    }
+  }
+  asm volatile("" ::: "memory");
+}
 
 // 32 rows between memory and a wave's own LDS (32 * kRow bytes): memory sees whole rows.  Rows from `n_rows` on are read as the last one
 // and not written.
@@ -171,22 +186,28 @@ UA_BOTH int imin(int a, int b) { return a < b ? a : b; }
 UA_BOTH int imax(int a, int b) { return a > b ? a : b; }
 // Blocks of 64 keys that a tile of rows r0 .. r1 walks: those of the sinks, then those of the window.
 struct SwaWalk {
-  int n_sink, first, n;
+  int n_sink, first, n, start, sinks_end, end;     // of the keys that a row sees: start .. end - 1, and those before sinks_end
   UA_BOTH SwaWalk(int r0, int r1, int hi, int lo, int sinks, int n_keys) {
-    const int last = imin(r1 + hi, n_keys - 1), start = imax(r0 + lo, 0);
+    const int last = imin(r1 + hi, n_keys - 1);
+    start = imax(r0 + lo, 0);
+    end = imax(last + 1, 0);
+    sinks_end = imin(sinks, end);
     n_sink = last >= 0 ? (imin(sinks, last + 1) + kSwaBlock - 1) / kSwaBlock : 0;
     first = imax(start / kSwaBlock, n_sink);
     n = n_sink + (last >= start ? imax(last / kSwaBlock + 1 - first, 0) : 0);
   }
   __device__ __forceinline__ int at(int i) const { return i < n_sink ? i : first + i - n_sink; }
+  // A block's keys from here on are not copied: nothing sees them.
+  __device__ __forceinline__ int end_of(int block) const { return (block + 1) * kSwaBlock <= start ? sinks_end : end; }
 };
 // Blocks of 64 query rows, of one head, that see a tile of keys k0 .. k1.
 struct SwaColumn {
-  int first, n;
+  int first, n, start, end;                        // the rows that see a key: start .. end - 1
   UA_BOTH SwaColumn(int k0, int k1, int hi, int lo, int sinks, int n_rows) {
-    const int start = imax(k0 - hi, 0), end = k0 < sinks ? n_rows - 1 : imin(k1 - lo, n_rows - 1);
+    start = imax(k0 - hi, 0);
+    end = imax(k0 < sinks ? n_rows : imin(k1 - lo + 1, n_rows), 0);
     first = start / kSwaBlock;
-    n = end >= start ? end / kSwaBlock + 1 - first : 0;
+    n = end > start ? (end - 1) / kSwaBlock + 1 - first : 0;
   }
 };
 

@@ -106,7 +106,7 @@ __device__ __forceinline__ void dkdv_rows(const BwdAddr<T, kD>& ad, uint32_t sta
     const int row = row0 + 4 * (fresh_lane() >> 5) - first;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if ((uint32_t)(row + 8 * (i >> 2) + (i & 3)) >= seen) s[i] = -INFINITY;
+      if ((uint32_t)(row + 8 * (i >> 2) + (i & 3)) >= seen) { s[i] = -INFINITY; dp[i] = 0.f; }      // (dp: NaN of a row not seen stays out)
   }
   x8 pb[2], dsb[2];
 #pragma unroll
@@ -164,7 +164,7 @@ __device__ __forceinline__ void columns_walk(uint32_t lds, int block) {
   float stat = 0.f;
   if (i0 < i1) {
     base(g);
-    in.block((col.first + at) * kSwaBlock, p.seq_q, true);
+    in.block((col.first + at) * kSwaBlock, col.end, true);
 #pragma unroll
     for (int n = 0; n < in.kPieces; ++n) in.copy(n, lds);
     stat = load_stat(g, (col.first + at) * kSwaBlock);
@@ -198,8 +198,9 @@ __device__ __forceinline__ void columns_walk(uint32_t lds, int block) {
     const int row0 = (col.first + at) * kSwaBlock;
     if (++at == col.n) { at = 0; base(++g < p.group ? g : 0); }
     const int next0 = (col.first + at) * kSwaBlock;
-    in.block(next0, p.seq_q, i + 1 < i1);
+    in.block(next0, col.end, i + 1 < i1);
     if (i + 1 < i1) stat = load_stat(g, next0);
+    if (row0 < col.start) lds_clear_rows<kD, H::kPitchB, BwdStream<kD>::kSecond>(lds + kStage * L::kStage, 0, col.start - row0);
     const uint32_t other = lds + (kStage ^ 1) * L::kStage;
     auto rows = [&](auto mb_tag) {
       constexpr int kMb = decltype(mb_tag)::value, kCopies = BwdStream<kD>::kPieces / 2;
@@ -217,7 +218,7 @@ __device__ __forceinline__ void columns_walk(uint32_t lds, int block) {
       uint32_t seen = 0;
       if (!whole) {
         first = key - p.hi;
-        const int last = key < p.sinks ? 2 * kFar - 1 : key - p.lo;
+        const int last = min(key < p.sinks ? kFar : key - p.lo, col.end - 1);      // (a row that is not there: 0 times NaN of the key)
         seen = last >= first ? (uint32_t)last - (uint32_t)first + 1u : 0u;
       }
       dkdv_rows<T, kD, kStage * L::kStage + kMb * BwdAddr<T, kD>::kRows32, kCopies>(
@@ -284,7 +285,7 @@ __device__ __forceinline__ void dq_keys(const BwdAddr<T, kD>& ad, const typename
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int k = key + 8 * (i >> 2) + (i & 3);
-      if ((uint32_t)(k - first) >= seen && k >= sinks) s[i] = -INFINITY;
+      if ((uint32_t)(k - first) >= seen && k >= sinks) { s[i] = -INFINITY; dp[i] = 0.f; }
     }
   }
   x8 dsb[2];
@@ -316,7 +317,7 @@ __device__ __forceinline__ void rows_walk(uint32_t lds, int block) {
   BwdStream<kD> in(p.ks.s, p.vs.s, wave, lane);
   in.of((const T*)p.k + b * p.ks.b + hk * p.ks.h, (const T*)p.v + b * p.vs.b + hk * p.vs.h);
   if (i0 < i1) {
-    in.block(walk.at(i0) * kSwaBlock, p.seq_k, true);
+    in.block(walk.at(i0) * kSwaBlock, walk.end_of(walk.at(i0)), true);
 #pragma unroll
     for (int n = 0; n < in.kPieces; ++n) in.copy(n, lds);
   }
@@ -350,9 +351,11 @@ __device__ __forceinline__ void rows_walk(uint32_t lds, int block) {
   auto step = [&](int i, auto stage_tag) {
     constexpr int kStage = decltype(stage_tag)::value;
     const int block0 = walk.at(i) * kSwaBlock;
-    in.block(walk.at(i + 1) * kSwaBlock, p.seq_k, i + 1 < i1);
+    in.block(walk.at(i + 1) * kSwaBlock, walk.end_of(walk.at(i + 1)), i + 1 < i1);
     wait_vmem_all();
     __syncthreads();                        // this block has landed, and everyone has left the other stage
+    if (block0 < walk.start && block0 + kSwaBlock > walk.start)
+      lds_clear_rows<kD, H::kPitchB>(lds + kStage * L::kStage, max(p.sinks - block0, 0), walk.start - block0);
     const uint32_t other = lds + (kStage ^ 1) * L::kStage;
     auto keys = [&](auto mb_tag) {
       constexpr int kMb = decltype(mb_tag)::value, kCopies = BwdStream<kD>::kPieces / 2;

@@ -52,7 +52,7 @@ __global__ __launch_bounds__(64 * kDecWaves) void swa_decode_kernel(const DecPar
   const int row0 = tile * kRows, row1 = min(row0 + kRows, p.rows) - 1;
   const int pos0 = next - p.n_tokens + quotient(row0, p.by_group), pos1 = next - p.n_tokens + quotient(row1, p.by_group);
   const int last = min(pos1, len - 1), start = max(pos0 - p.left, 0);
-  const int n_sink = last >= 0 ? (min(p.sinks, last + 1) + kDecBlock - 1) / kDecBlock : 0, first = max(start / kDecBlock, n_sink);
+  const int sinks_end = min(p.sinks, last + 1), n_sink = last >= 0 ? (sinks_end + kDecBlock - 1) / kDecBlock : 0, first = max(start / kDecBlock, n_sink);
   const int n_all = n_sink + (last >= start ? max(last / kDecBlock + 1 - first, 0) : 0);
   const int part_len = (n_all + p.n_parts - 1) / p.n_parts, i0 = min(part * part_len, n_all), i1 = min(i0 + part_len, n_all);
   auto key_of = [&](int i) { return (i < n_sink ? i : first + i - n_sink) * kDecBlock; };
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(64 * kDecWaves) void swa_decode_kernel(const DecPar
   const uint32_t mine = lds0 + wave * H::kWave;
   const int copy_row = lane / H::kChunks, chunk = lane % H::kChunks, k_off = copy_row * (int)k_row, v_off = copy_row * (int)v_row;
   auto copy_in = [&](int i, uint32_t stage) {
-    const int key0 = key_of(i), n = i < i1 ? min(len - key0, kDecBlock) : 0;
+    const int key0 = key_of(i), n = i < i1 ? min((key0 + kDecBlock <= start ? sinks_end : last + 1) - key0, kDecBlock) : 0;       // (what no row sees is not read)
     const u32x4 rk = make_rsrc_words(kbase + key0 * k_row, n > 0 ? (uint32_t)((n - 1) * k_row + H::kRow) : 0);
     const u32x4 rv = make_rsrc_words(vbase + key0 * v_row, n > 0 ? (uint32_t)((n - 1) * v_row + H::kRow) : 0);
 #pragma unroll
@@ -116,6 +116,7 @@ __global__ __launch_bounds__(64 * kDecWaves) void swa_decode_kernel(const DecPar
         const int r = 16 * n + col;
         kf[n][s] = lds_get<x8>(stage + r * H::kRow + (H::slot_k(r, 4 * s + quad) << 4));
       }
+    if (key0 < start && key0 + kDecBlock > start) lds_clear_rows<kD, 1024>(stage + H::kTile, max(p.sinks - key0, 0), start - key0);
     x8 vf[H::kBlocks];
 #pragma unroll
     for (int d = 0; d < H::kBlocks; ++d) {

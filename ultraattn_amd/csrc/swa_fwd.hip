@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
   Stream in(p.ks.s, p.vs.s, wave, lane);
   in.of((const T*)p.k + b * p.ks.b + hk * p.ks.h, (const T*)p.v + b * p.vs.b + hk * p.vs.h);
   if (i0 < i1) {
-    in.block(walk.at(i0) * kSwaBlock, p.seq_k, true);
+    in.block(walk.at(i0) * kSwaBlock, walk.end_of(walk.at(i0)), true);
 #pragma unroll
     for (int n = 0; n < in.kPieces; ++n) in.copy(n, lds[0]);
   }
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
     constexpr int kStage = decltype(stage_tag)::value;
     const uint32_t here = lds[kStage], other = lds[kStage ^ 1];
     const int key0 = walk.at(i) * kSwaBlock;
-    in.block(walk.at(i + 1) * kSwaBlock, p.seq_k, i + 1 < i1);
+    in.block(walk.at(i + 1) * kSwaBlock, walk.end_of(walk.at(i + 1)), i + 1 < i1);
     wait_vmem_all();
     __syncthreads();                        // this block has landed, and everyone has left the other stage
     const bool hidden = key0 > row0 + 31 + p.hi || (key0 + kSwaBlock <= row0 + p.lo && key0 >= p.sinks);
@@ -108,6 +108,7 @@ __global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
           const int k = key + 32 * mb + 8 * (j >> 2) + (j & 3);
           if ((uint32_t)(k - first) >= seen && k >= sinks) s[mb][j] = -INFINITY;
         }
+      if (key0 < walk.start && key0 + kSwaBlock > walk.start) lds_clear_rows<kD, 1024>(here + Stream::kSecond, max(p.sinks - key0, 0), walk.start - key0);
     }
     constexpr int kVAhead = 3, kVAll = 4 * H::kBlocks;
     x8 vf[4];

@@ -9,8 +9,8 @@ Query i is at position ``q_start + i`` and key j at ``k_start + j``.  With ``win
 ``p - left .. p + right`` (-1: no bound on that side) and, up to ``p + right``, the first ``sinks`` positions of the sequence.
 ``q_start=None`` puts the last query at the last key.  A query that sees no key gets ``out = 0``, ``lse = -inf`` and no gradient, so
 results over shards of the keys (``k_start``) are joined by ``merge_partials`` / ``update_out_and_lse``.
-NaN or infinity in a key or value reaches the rows that see it, and may reach others whose tile of 128 (in a decode, whose block of 32 keys) holds
-one that does.
+NaN or infinity in a key or value reaches the rows that see it, and may reach others of their tile of 128 rows (in a decode, of up to 32 rows of a key
+head); it reaches no tile that has none that does.  So a cache may hold anything in rows that no new token sees.
 """
 from typing import Optional, Tuple
 
