@@ -14,6 +14,10 @@ namespace ua {
 
 constexpr int kDecBlock = 32, kDecWaves = 4, kDecMaxParts = 64;
 
+// P is held times 2^kDecBits of the largest score's, which no score exceeds here: fp16 then has it down to 2^-38 of that.
+template <class T> constexpr float kDecBits = 0.f;
+template <> constexpr float kDecBits<fp16> = 14.f;
+
 struct DecParams {
   const void *q, *k, *v;
   void* o;
@@ -147,8 +151,8 @@ __global__ __launch_bounds__(64 * kDecWaves) void swa_decode_kernel(const DecPar
       mx = fmaxf(a, c) * p.scale_log2;
       if (__builtin_amdgcn_ballot_w64(mx > m_run[t]) != 0) {
         const float m_new = fmaxf(m_run[t], mx);
-        m_use[t] = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = m_new == m_run[t] ? 1.f : fast_exp2(m_run[t] - m_use[t]);
+        m_use[t] = m_new == -INFINITY ? 0.f : m_new - kDecBits<T>;
+        const float alpha = m_new == m_run[t] ? 1.f : fast_exp2(m_run[t] - m_new);
         m_run[t] = m_new;
         l_run[t] *= alpha;
 #pragma unroll
@@ -209,7 +213,7 @@ __global__ __launch_bounds__(64 * kDecWaves) void swa_decode_kernel(const DecPar
       }
     }
     const bool any = l > 0.f || l != l;
-    const float inv = any ? 1.f / l : 0.f, lse = any ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+    const float inv = any ? 1.f / l : 0.f, lse = any ? (m - kDecBits<T> + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
     const int token = quotient(row, p.by_group), h = hk * p.group + row - token * p.group;
     const int64_t out_row = ((int64_t)b * p.n_heads + h) * p.n_tokens + token;
     if (p.n_parts > 1) {

@@ -12,10 +12,12 @@
 
 namespace ua {
 
-// Sums of a lane's 32 exponentials from which the reference is raised.  fp16 holds P up to 65504.
+// kSum: sums of a lane's 32 exponentials from which the reference is raised; kBits: P is held times 2^kBits of the largest score's.  fp16 holds P up
+// to 65504 and, times 2^7, down to 2^-31 of the largest: without that, 70000 keys at 2^-26 of it, a thousandth of the row, vanished.
+// (32 equal keys leave the sum 8 times below the bound.)
 template <class T> struct SwaRaise;
-template <> struct SwaRaise<bf16> { static constexpr float kSum = 16777216.f; };
-template <> struct SwaRaise<fp16> { static constexpr float kSum = 1024.f; };
+template <> struct SwaRaise<bf16> { static constexpr float kSum = 16777216.f, kBits = 0.f; };
+template <> struct SwaRaise<fp16> { static constexpr float kSum = 32768.f, kBits = 7.f; };
 
 template <class T, int kD>
 __global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
@@ -140,8 +142,8 @@ __global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
         for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[mb][j]);
       swap_lanes<32>(mx, a, c);
       const float m_new = fmaxf(m_run, fmaxf(a, c) * p.scale_log2);
-      m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = m_new == m_run ? 1.f : fast_exp2(m_run - m_use);      // m_run = -inf -> 0
+      m_use = m_new == -INFINITY ? 0.f : m_new - SwaRaise<T>::kBits;
+      const float alpha = m_new == m_run ? 1.f : fast_exp2(m_run - m_new);      // m_run = -inf -> 0
       m_run = m_new;
       l_run *= alpha;
 #pragma unroll
@@ -169,7 +171,7 @@ __global__ __launch_bounds__(256, 2) void swa_fwd_kernel(const SwaParams p) {
   float a, c;
   swap_lanes<32>(l_run, a, c);
   const float l = a + c, inv = l > 0.f || l != l ? 1.f / l : 0.f;      // (NaN stays)
-  const float lse = l > 0.f || l != l ? (m_run + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+  const float lse = l > 0.f || l != l ? (m_use + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
   const int out_lane = fresh_lane();
   if (p.n_parts > 1) {
     const int64_t row = ((int64_t)bh * p.seq_q + row0);
