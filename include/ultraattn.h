@@ -361,8 +361,8 @@ int ua_swa_fwd(const void *q, const void *k, const void *v, void *o, float *lse,
 /* Gradients, with the same arguments; lse and delta are the rows' global statistics (of all shards).  ua_swa_bwd_delta: delta =
  * rowsum(dout * o), fp32 [batch, n_heads, seqlen_q]; rows of up to 8 keys, where o's rounding counts most, take o from q, k and v again
  * if lse is that of these keys alone.  dq, dk and dv are overwritten; dk and dv are the sums over the query heads that share a key
- * head.  Nothing is added atomically: the same call gives the same bits.  P and dS are rounded to dtype for their products; in fp16 dS below 6e-5
- * loses bits, so scale the loss as with any fp16 gradient.
+ * head.  Nothing is added atomically: the same call gives the same bits.  P and dS are rounded to dtype for their products; in fp16 both are
+ * held times powers of two there, so that small ones keep their bits: gradients lose what fp16 results lose (2^-24 is their last place), nothing before.
  * Few long walks, and those of the sinks' columns, which all later queries see, are cut into parts if `workspace` holds
  * ua_swa_bwd_workspace_bytes(). */
 int ua_swa_bwd_delta(const void *o, const void *dout, const void *q, const void *k, const void *v, const float *lse, float *delta,

@@ -16,9 +16,31 @@
 
 namespace ua {
 
-// P <= 1 in fp16 is below its normal range from 6e-5 on, where long rows are: it is held times 2^14, dV is divided by that.
-template <class T> constexpr float kSwaPScale = 1.f;
-template <> constexpr float kSwaPScale<fp16> = 16384.f;
+// P <= 1 in fp16 is below its normal range from 6e-5 on, where long rows are: it is held times 2^14, dV is divided by that.  So is dS = P (dP - delta):
+// times 2^(14 - k), where a wave's k begins at 4 and grows with the largest |dP - delta| that it meets, below 2^(k + 1); the gradient summed so far shrinks by as
+// much and is multiplied by 2^(k - 14) at its end.  So dS down to 2^-29 of the largest dP - delta has all bits, whatever the size of dO.  (bf16 has
+// fp32's range.)  It costs 2 of 66 us (2 x 10 heads of 64, 1333 x 2048), 3 of 185 (16 of 128, 4096): the largest
+// one is known late.  Found beside dV's products, which then come before dK's, it cost no less, and registers.
+template <class T> constexpr int kSwaBits = 0;
+template <> constexpr int kSwaBits<fp16> = 14;
+template <class T> constexpr int kSwaFirst = kSwaBits<T> ? 4 : 0;
+__device__ __forceinline__ float power2(int n) { return __int_as_float((127 + n) << 23); }
+// How much k has to grow by, seldom anything, with the gradient so far.  (Infinities stay; they say nothing of the others.  2^60 is beyond any other.)
+template <int kN>
+__device__ __forceinline__ int swa_grow(const f32x16& dp, int k, f32x16 (&acc)[kN]) {
+  float half[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) half[i >> 1 & 1] = fmaxf(fmaxf(half[i >> 1 & 1], fabsf(dp[i])), fabsf(dp[i + 1]));
+  const float most = fmaxf(half[0], half[1]);
+  if (__builtin_amdgcn_ballot_w64(most >= power2(1 + k)) == 0) return 0;
+  int more = 0;
+  while (k + more < 60 && __builtin_amdgcn_ballot_w64(most >= power2(1 + k + more) && most < INFINITY) != 0) more += 2;
+#pragma unroll
+  for (int m = 0; m < kN; ++m)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[m][i] *= power2(-more);
+  return more;
+}
 
 template <int kD> using BwdStream = SwaStream<kD, kB, kB>;
 template <int kD> struct BwdLds {
@@ -66,7 +88,7 @@ __device__ __forceinline__ const SwaParams& params_again() {
 template <class T, int kD, int kOff, int kCopies, class Copy>
 __device__ __forceinline__ void dkdv_rows(const BwdAddr<T, kD>& ad, uint32_t stat, const typename SwaVec<T>::x8 (&kf)[kD / 16],
                                           const typename SwaVec<T>::x8 (&vf)[kD / 16], f32x16 (&dk)[kD / 32], f32x16 (&dv)[kD / 32], float scale_log2,
-                                          bool mask, int row0, int first, uint32_t seen, Copy copy) {
+                                          int& ds_k, bool mask, int row0, int first, uint32_t seen, Copy copy) {
   using V = SwaVec<T>;
   using H = SwaHead<kD>;
   typedef typename V::x8 x8;
@@ -108,12 +130,13 @@ __device__ __forceinline__ void dkdv_rows(const BwdAddr<T, kD>& ad, uint32_t sta
     for (int i = 0; i < 16; ++i)
       if ((uint32_t)(row + 8 * (i >> 2) + (i & 3)) >= seen) { s[i] = -INFINITY; dp[i] = 0.f; }      // (dp: NaN of a row not seen stays out)
   }
+  if constexpr (kSwaBits<T> != 0) ds_k += swa_grow(dp, ds_k, dk);
   x8 pb[2], dsb[2];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float e = fast_exp2(s[i] * scale_log2);
-    pb[i >> 3][i & 7] = (T)(kSwaPScale<T> == 1.f ? e : e * kSwaPScale<T>);
-    dsb[i >> 3][i & 7] = (T)(e * dp[i]);
+    const float e = fast_exp2(kSwaBits<T> ? fmaf(s[i], scale_log2, kSwaBits<T>) : s[i] * scale_log2);
+    pb[i >> 3][i & 7] = (T)e;
+    dsb[i >> 3][i & 7] = (T)(kSwaBits<T> ? e * dp[i] * power2(-ds_k) : e * dp[i]);
   }
 #pragma unroll
   for (int i = 0; i < kTAll; ++i) {
@@ -184,6 +207,7 @@ __device__ __forceinline__ void columns_walk(uint32_t lds, int block) {
   f32x16 dk[H::kBlocks], dv[H::kBlocks];
 #pragma unroll
   for (int m = 0; m < H::kBlocks; ++m) { dk[m] = f32x16{0}; dv[m] = f32x16{0}; }
+  int ds_k = kSwaFirst<T>;
   const BwdAddr<T, kD> ad(lds);
   if (i0 < i1) put_stat(0, stat);
 #pragma unroll
@@ -222,7 +246,7 @@ __device__ __forceinline__ void columns_walk(uint32_t lds, int block) {
         seen = last >= first ? (uint32_t)last - (uint32_t)first + 1u : 0u;
       }
       dkdv_rows<T, kD, kStage * L::kStage + kMb * BwdAddr<T, kD>::kRows32, kCopies>(
-          ad, lds + L::kStat + kStage * L::kStatBytes + kMb * 128, kf, vf, dk, dv, scale_log2, !whole, r0, first, seen, copy);
+          ad, lds + L::kStat + kStage * L::kStatBytes + kMb * 128, kf, vf, dk, dv, scale_log2, ds_k, !whole, r0, first, seen, copy);
     };
     rows(std::integral_constant<int, 0>{});
     rows(std::integral_constant<int, 1>{});
@@ -238,21 +262,22 @@ __device__ __forceinline__ void columns_walk(uint32_t lds, int block) {
   const int n_rows = e.seq_k - key0;
   if (n_rows <= 0) return;
   const SwaColumns& ec = e.cols[run];
+  const float dk_scale = e.scale * power2(ds_k - kSwaBits<T>);
   if (ec.n_parts > 1) {
     const int64_t row = part * ec.part + ((int64_t)bh * ec.tiles * kSwaRows + key0 - ec.first * kSwaRows) * kD;
-    swa_store_f32<kD>(ec.dk + row, kD, n_rows, dk, e.scale);
-    swa_store_f32<kD>(ec.dv + row, kD, n_rows, dv, 1.f / kSwaPScale<T>);
+    swa_store_f32<kD>(ec.dk + row, kD, n_rows, dk, dk_scale);
+    swa_store_f32<kD>(ec.dv + row, kD, n_rows, dv, power2(-kSwaBits<T>));
   } else {
     const uint32_t turn = lds + wave * 32 * H::kRow;
-    swa_store_rows<T, kD>((T*)e.dk + b * e.dks.b + (int64_t)key0 * e.dks.s + hk * e.dks.h, e.dks.s, n_rows, dk, e.scale, turn);
-    swa_store_rows<T, kD>((T*)e.dv + b * e.dvs.b + (int64_t)key0 * e.dvs.s + hk * e.dvs.h, e.dvs.s, n_rows, dv, 1.f / kSwaPScale<T>, turn);
+    swa_store_rows<T, kD>((T*)e.dk + b * e.dks.b + (int64_t)key0 * e.dks.s + hk * e.dks.h, e.dks.s, n_rows, dk, dk_scale, turn);
+    swa_store_rows<T, kD>((T*)e.dv + b * e.dvs.b + (int64_t)key0 * e.dvs.s + hk * e.dvs.h, e.dvs.s, n_rows, dv, power2(-kSwaBits<T>), turn);
   }
 }
 
 // ---- rows ---------------------------------------------------------------------------------------------------------
 template <class T, int kD, int kOff, int kCopies, class Copy>
 __device__ __forceinline__ void dq_keys(const BwdAddr<T, kD>& ad, const typename SwaVec<T>::x8 (&qf)[kD / 16], const typename SwaVec<T>::x8 (&dof)[kD / 16],
-                                        const f32x16& neg_delta, f32x16 (&dq)[kD / 32], float scale_log2, float lse2, bool mask, int key0, int first,
+                                        const f32x16& neg_delta, f32x16 (&dq)[kD / 32], float scale_log2, float& lse2, int& ds_k, bool mask, int key0, int first,
                                         uint32_t seen, int sinks, Copy copy) {
   using V = SwaVec<T>;
   using H = SwaHead<kD>;
@@ -287,6 +312,11 @@ __device__ __forceinline__ void dq_keys(const BwdAddr<T, kD>& ad, const typename
       const int k = key + 8 * (i >> 2) + (i & 3);
       if ((uint32_t)(k - first) >= seen && k >= sinks) { s[i] = -INFINITY; dp[i] = 0.f; }
     }
+  }
+  if constexpr (kSwaBits<T> != 0) {
+    const int more = swa_grow(dp, ds_k, dq);
+    ds_k += more;
+    lse2 += more;                           // 2^(14 - k) is in the exponent
   }
   x8 dsb[2];
 #pragma unroll
@@ -337,7 +367,8 @@ __device__ __forceinline__ void rows_walk(uint32_t lds, int block) {
     swa_put_rows<kD>(doraw, turn);
     swa_frags<T, kD>(dof, turn);
   }
-  const float lse2 = lse_raw == -INFINITY ? INFINITY : lse_raw * kLog2e;        // (P = 0 in rows that see nothing)
+  float lse2 = lse_raw == -INFINITY ? INFINITY : lse_raw * kLog2e - (kSwaBits<T> - kSwaFirst<T>);        // (P = 0 in rows that see nothing)
+  int ds_k = kSwaFirst<T>;
   f32x16 nd, dq[H::kBlocks];
 #pragma unroll
   for (int i = 0; i < 16; ++i) nd[i] = neg_delta;
@@ -376,7 +407,7 @@ __device__ __forceinline__ void rows_walk(uint32_t lds, int block) {
         seen = (uint32_t)max(last - first + 1, 0);
         sinks = min(p.sinks, last + 1);
       }
-      dq_keys<T, kD, kStage * L::kStage + kMb * BwdAddr<T, kD>::kRows32, kCopies>(ad, qf, dof, nd, dq, p.scale_log2, lse2, !whole, key0, first, seen, sinks,
+      dq_keys<T, kD, kStage * L::kStage + kMb * BwdAddr<T, kD>::kRows32, kCopies>(ad, qf, dof, nd, dq, p.scale_log2, lse2, ds_k, !whole, key0, first, seen, sinks,
                                                                                   copy);
     };
     keys(std::integral_constant<int, 0>{});
@@ -390,10 +421,11 @@ __device__ __forceinline__ void rows_walk(uint32_t lds, int block) {
   __syncthreads();
   if (n_rows <= 0) return;
   const SwaParams& e = params_again();
+  const float dq_scale = e.scale * power2(ds_k - kSwaBits<T>);
   if (e.n_parts > 1)
-    swa_store_f32<kD>(e.part_o + part * e.o_part + ((int64_t)bh * e.seq_q + row0) * kD, kD, n_rows, dq, e.scale);
+    swa_store_f32<kD>(e.part_o + part * e.o_part + ((int64_t)bh * e.seq_q + row0) * kD, kD, n_rows, dq, dq_scale);
   else
-    swa_store_rows<T, kD>((T*)e.dq + b * e.dqs.b + (int64_t)row0 * e.dqs.s + h * e.dqs.h, e.dqs.s, n_rows, dq, e.scale, lds + wave * 32 * H::kRow);
+    swa_store_rows<T, kD>((T*)e.dq + b * e.dqs.b + (int64_t)row0 * e.dqs.s + h * e.dqs.h, e.dqs.s, n_rows, dq, dq_scale, lds + wave * 32 * H::kRow);
 }
 
 template <class T, int kD>
