@@ -68,8 +68,8 @@ extern "C" {
 
 /* 100 * major + minor.  102: `nnz` argument of the attention entry points, ua_merge_update, the
  * no-allocation builder, `work` of ua_tilelist_build_device grown to n_qtiles + n_ktiles + 7.  104: ua_bsa_bwd.
- * 105: ua_tilelist_build_device_scratch.  106: ua_copy_in.  107: ua_rope, ua_rope_append.  108: ua_swa_*.  */
-#define UA_VERSION 108
+ * 105: ua_tilelist_build_device_scratch.  106: ua_copy_in.  107: ua_rope, ua_rope_append.  108: ua_swa_*.  109: ua_rows_*.  */
+#define UA_VERSION 109
 int ua_version(void);
 const char *ua_strerror(int rc);
 
@@ -342,7 +342,7 @@ int ua_rope_append(const void *q, const void *k, const void *v, void *q_out, voi
  * q, o [batch, seqlen_q, n_heads, head_dim]; k, v [batch, seqlen_k, n_kv_heads, head_dim]: key head h serves query heads
  * h * n_heads / n_kv_heads ...  Any lengths (0 too, up to 2^28), head_dim 64 or 128, dtype UA_BF16 or UA_FP16; pointers 16-byte
  * aligned, element strides multiples of 8 (inputs may have strides of 0: broadcast).  lse [batch, n_heads, seqlen_q] fp32, contiguous, natural log: rows
- * that see no key get o = 0, lse = -inf, and ua_merge / ua_merge_update join shards.  Scores, statistics and sums are 32 bits; P is rounded
+ * that see no key get o = 0, lse = -inf, and ua_rows_merge / ua_rows_update join shards (bf16 heads of 128 also ua_merge / ua_merge_update).  Scores, statistics and sums are 32 bits; P is rounded
  * to dtype for its product with V, as it is in ua_bsa_fwd.
  * Few long walks are cut into parts, whose fp32 results are merged in a second launch, if `workspace` (16-byte aligned,
  * overwritten) holds ua_swa_workspace_bytes(); calls that overlap in time need one each.  With less nothing is cut.
@@ -391,6 +391,23 @@ int ua_swa_decode(const void *q, const void *k_cache, const void *v_cache, void 
                   int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int head_dim, int dtype,
                   const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides, const int64_t *o_strides,
                   int64_t left, int64_t sinks, float softmax_scale, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* What joins shards of these rows: ua_merge, ua_merge_update, ua_grad_sum and ua_bsa_bwd_delta for head_dim 64 or 128 and dtype UA_BF16 or UA_FP16, with
+ * their arguments and layouts; where those take fp32 rows (`*_is_fp32`, parts_fp32) so do these, and dtype is that of the others.  Any number of heads;
+ * batch or seqlen 0 writes nothing.  Strides and pointers as there (16 bytes; multiples of 8 elements, 4 of fp32). */
+int ua_rows_merge(const void *const *o_parts, const float *const *lse_parts, int n_parts,
+                  void *o, float *lse, int batch, int seqlen, int n_heads, int head_dim, int dtype, void *stream);
+int ua_rows_update(const void *out, const float *lse, const void *block_out, const float *block_lse,
+                   void *new_out, float *new_lse, int batch, int n_rows, int n_heads, int head_dim, int dtype,
+                   int out_is_fp32, int block_is_fp32, int new_is_fp32,
+                   const int64_t *out_strides, const int64_t *lse_strides,
+                   const int64_t *block_out_strides, const int64_t *block_lse_strides,
+                   const int64_t *new_out_strides, const int64_t *new_lse_strides, void *stream);
+int ua_rows_sum(const void *const *parts, int n_parts, int parts_fp32, void *out,
+                int batch, int seqlen, int n_heads, int head_dim, int dtype, const int64_t *out_strides, float scale, void *stream);
+int ua_rows_delta(const void *o, const void *dout, float *delta,
+                  int batch, int seqlen_q, int n_heads, int head_dim, int dtype,
+                  const int64_t *o_strides, const int64_t *do_strides, void *stream);
 
 #ifdef __cplusplus
 }

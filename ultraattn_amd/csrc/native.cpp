@@ -190,7 +190,41 @@ void init_device(int device) {
   if (device >= 0 && device < 64) done[device] = true;
 }
 
+// Rows that results are joined in: bf16 heads of 128, which have kernels of their own, and else bf16 or fp16 heads of 64 or 128 (ua_rows_*).
+bool rows_plain(const at::Tensor& t) { return !(t.scalar_type() == at::kHalf || (t.dim() == 4 && t.size(3) == 64)); }
+int rows_code(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? UA_FP16 : UA_BF16; }
+void check_rows_of(const char* name, const at::Tensor& t, at::ScalarType dt, int64_t dim) {
+  if (!t.is_cuda()) fail(PyExc_ValueError, std::string(name) + " must be a CUDA (HIP) tensor");
+  if (t.scalar_type() != dt) fail(PyExc_TypeError, std::string(name) + " must be " + c10::toString(dt) + ", got " + c10::toString(t.scalar_type()));
+  if (t.dim() != 4 || t.size(3) != dim) fail(PyExc_ValueError, std::string(name) + " must be [B, S, Nh, " + std::to_string(dim) + "], got " + shape_str(t.sizes()));
+  if (t.stride(3) != 1) fail(PyExc_ValueError, std::string(name) + ": head_dim axis must be contiguous");
+}
+// Of the first tensor of a call: its type and head size, which the others have to have.
+void check_rows_first(const char* name, const at::Tensor& t) {
+  if (t.scalar_type() != at::kHalf && t.scalar_type() != at::kBFloat16)
+    fail(PyExc_TypeError, std::string(name) + " must be bfloat16 or float16, got " + c10::toString(t.scalar_type()));
+  check_rows_of(name, t, t.scalar_type(), t.dim() == 4 && t.size(3) == 64 ? 64 : kDim);
+}
+void check_beside(const char* name, const at::Tensor& t, const at::Tensor& first) {
+  if (t.device() != first.device()) fail(PyExc_ValueError, std::string(name) + " is on another device than the first tensor");
+}
+
 at::Tensor delta_of(const at::Tensor& out, const at::Tensor& dout, at::Tensor delta) {
+  if (!rows_plain(out)) {
+    check_rows_first("out", out);
+    check_rows_of("dout", dout, out.scalar_type(), out.size(3));
+    check_beside("dout", dout, out);
+    if (!out.sizes().equals(dout.sizes())) fail(PyExc_ValueError, "out and dout must have the same shape");
+    if (!delta.defined()) delta = stat_of(out);
+    check_stat("delta", delta, out);
+    check_beside("delta", delta, out);
+    const On on(out);
+    call("ua_rows_delta", [&] {
+      return ua_rows_delta(out.data_ptr(), dout.data_ptr(), (float*)delta.data_ptr(), (int)out.size(0), (int)out.size(1), (int)out.size(2), (int)out.size(3),
+                           rows_code(out), Strides(out), Strides(dout), on.stream);
+    });
+    return delta;
+  }
   check_rows16("out", out, 1);
   check_rows16("dout", dout, 1);
   if (!out.sizes().equals(dout.sizes())) fail(PyExc_ValueError, "out and dout must have the same shape");
@@ -525,6 +559,7 @@ PyObject* merge(PyObject* const* a) {
   if (n == 0 || n != lses.size()) fail(PyExc_ValueError, "need as many lses as outs, at least one");
   const at::Tensor& first = outs.at(0, "partial out");
   if (n > UA_MAX_PARTS) check_rc(UA_ERR_UNSUPPORTED, "ua_merge");
+  const bool plain = rows_plain(first);
   const void* op[UA_MAX_PARTS];
   const float* lp[UA_MAX_PARTS];
   auto is_stat = [&](const at::Tensor& l) {
@@ -533,7 +568,14 @@ PyObject* merge(PyObject* const* a) {
   };
   for (int64_t i = 0; i < n; ++i) {
     const at::Tensor &o = outs.at(i, "partial out"), &l = lses.at(i, "partial lse");
-    check_rows16("partial out", o, 1);
+    if (plain) {
+      check_rows16("partial out", o, 1);
+    } else {
+      check_rows_first("partial out", first);
+      check_rows_of("partial out", o, first.scalar_type(), first.size(3));
+      check_beside("partial out", o, first);
+      check_beside("partial lse", l, first);
+    }
     if (!o.sizes().equals(first.sizes()) || !o.is_contiguous()) fail(PyExc_ValueError, "partial outs must be contiguous and of equal shape");
     if (!is_stat(l)) fail(PyExc_ValueError, "partial lses must be contiguous fp32 [B, Nh, S]");
     op[i] = o.data_ptr();
@@ -542,10 +584,19 @@ PyObject* merge(PyObject* const* a) {
   Slot out(a[2]), lse(a[3]);
   out.t = out.given ? tensor(out.given, "out") : like(first);
   lse.t = lse.given ? tensor(lse.given, "lse") : stat_of(first);
-  if (!out.t.sizes().equals(first.sizes()) || !out.t.is_contiguous() || out.t.scalar_type() != at::kBFloat16)
-    fail(PyExc_ValueError, "out must be a contiguous bf16 tensor of the partials' shape");
+  if (!out.t.sizes().equals(first.sizes()) || !out.t.is_contiguous() || out.t.scalar_type() != (plain ? at::kBFloat16 : first.scalar_type()))
+    fail(PyExc_ValueError, plain ? "out must be a contiguous bf16 tensor of the partials' shape" : "out must be a contiguous tensor of the partials' shape and type");
   if (!is_stat(lse.t)) fail(PyExc_ValueError, "lse must be a contiguous fp32 [B, Nh, S] tensor");
   const On on(out.t);
+  if (!plain) {
+    check_beside("out", out.t, first);
+    check_beside("lse", lse.t, first);
+    call("ua_rows_merge", [&] {
+      return ua_rows_merge(op, lp, (int)n, out.t.data_ptr(), (float*)lse.t.data_ptr(), (int)first.size(0), (int)first.size(1), (int)first.size(2),
+                           (int)first.size(3), rows_code(first), on.stream);
+    });
+    return tuple_of(out, lse);
+  }
   call("ua_merge", [&] {
     return ua_merge(op, lp, (int)n, out.t.data_ptr(), (float*)lse.t.data_ptr(), (int)first.size(0), (int)first.size(1), (int)first.size(2), (int)kDim,
                     on.stream);
@@ -560,21 +611,36 @@ PyObject* grad_sum(PyObject* const* a) {
   if (n == 0) fail(PyExc_ValueError, "need at least one partial gradient");
   const at::Tensor& first = parts.at(0, "partial gradient");
   const at::ScalarType dt = first.scalar_type();
-  if (dt != at::kBFloat16 && dt != at::kFloat) fail(PyExc_TypeError, "partial gradients must be bfloat16 or float32");
+  if (dt != at::kBFloat16 && dt != at::kFloat && dt != at::kHalf) fail(PyExc_TypeError, "partial gradients must be bfloat16, float16 or float32");
+  const int64_t dim = first.dim() == 4 && first.size(3) == 64 ? 64 : kDim;
   const void* pp[UA_MAX_PARTS];
   for (int64_t i = 0; i < n; ++i) {
     const at::Tensor& t = parts.at(i, "partial gradient");
-    if (!t.is_cuda() || t.scalar_type() != dt || !t.sizes().equals(first.sizes()) || !t.is_contiguous() || t.dim() != 4 || t.size(3) != kDim)
-      fail(PyExc_ValueError, "partial gradients must be contiguous [B, S, Nh, 128] CUDA tensors of one dtype and shape");
+    if (!t.is_cuda() || t.scalar_type() != dt || !t.sizes().equals(first.sizes()) || !t.is_contiguous() || t.dim() != 4 || t.size(3) != dim)
+      fail(PyExc_ValueError, "partial gradients must be contiguous [B, S, Nh, 128] (or 64) CUDA tensors of one dtype and shape");
     if (i < UA_MAX_PARTS) pp[i] = t.data_ptr();
   }
   if (n > UA_MAX_PARTS) check_rc(UA_ERR_UNSUPPORTED, "ua_grad_sum");
   Slot out(a[1]);
-  out.t = out.given ? tensor(out.given, "out") : at::empty(first.sizes(), first.options().dtype(at::kBFloat16));
-  check_rows16("out", out.t, 1);
+  out.t = out.given ? tensor(out.given, "out") : at::empty(first.sizes(), first.options().dtype(dt == at::kHalf ? at::kHalf : at::kBFloat16));
+  const bool plain = dt != at::kHalf && out.t.scalar_type() != at::kHalf && dim == kDim;
+  if (plain) {
+    check_rows16("out", out.t, 1);
+  } else {
+    check_rows_first("out", out.t);
+    check_rows_of("out", out.t, dt == at::kFloat ? out.t.scalar_type() : dt, dim);
+    for (int64_t i = 0; i < n; ++i) check_beside("partial gradient", parts.at(i, "partial gradient"), out.t);
+  }
   if (!out.t.sizes().equals(first.sizes())) fail(PyExc_ValueError, "out must have the partials' shape");
   const float scale = (float)number(a[2]);
   const On on(out.t);
+  if (!plain) {
+    call("ua_rows_sum", [&] {
+      return ua_rows_sum(pp, (int)n, dt == at::kFloat, out.t.data_ptr(), (int)first.size(0), (int)first.size(1), (int)first.size(2), (int)dim,
+                         rows_code(out.t), Strides(out.t), scale, on.stream);
+    });
+    return out.wrap();
+  }
   call("ua_grad_sum", [&] {
     return ua_grad_sum(pp, (int)n, dt == at::kFloat, out.t.data_ptr(), (int)first.size(0), (int)first.size(1), (int)first.size(2), (int)kDim,
                        Strides(out.t), scale, on.stream);
@@ -583,10 +649,10 @@ PyObject* grad_sum(PyObject* const* a) {
 }
 
 void check_rows_any(const char* name, const at::Tensor& t) {
-  if (!t.is_cuda() || (t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kFloat))
-    fail(PyExc_TypeError, std::string(name) + " must be a bfloat16 or float32 CUDA tensor");
-  if (t.dim() != 4 || t.size(3) != kDim || t.stride(3) != 1)
-    fail(PyExc_ValueError, std::string(name) + " must be [B, S, Nh, " + std::to_string(kDim) + "] with a contiguous last axis, got " + shape_str(t.sizes()));
+  if (!t.is_cuda() || (t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kFloat && t.scalar_type() != at::kHalf))
+    fail(PyExc_TypeError, std::string(name) + " must be a bfloat16, float16 or float32 CUDA tensor");
+  if (t.dim() != 4 || (t.size(3) != kDim && t.size(3) != 64) || t.stride(3) != 1)
+    fail(PyExc_ValueError, std::string(name) + " must be [B, S, Nh, " + std::to_string(kDim) + "] (or 64) with a contiguous last axis, got " + shape_str(t.sizes()));
 }
 // (batch, token, head) strides of the statistics of `rows`, given as [B, S, Nh, 1] or [B, Nh, S].
 Strides stat_strides(const char* name, const at::Tensor& t, const at::Tensor& rows) {
@@ -612,6 +678,18 @@ PyObject* merge_update(PyObject* const* a) {
   new_lse.t = in_place ? lse : at::empty(lse.sizes(), lse.options());
   const Strides nls = stat_strides("lse", new_lse.t, out);
   const On on(out);
+  const bool half = out.scalar_type() == at::kHalf || blk.scalar_type() == at::kHalf;
+  if (half || out.size(3) != kDim) {
+    if (half && (out.scalar_type() == at::kBFloat16 || blk.scalar_type() == at::kBFloat16)) fail(PyExc_TypeError, "out and block_out must be of one type, or float32");
+    for (const at::Tensor* t : {&lse, &blk, &blk_lse}) check_beside("an operand", *t, out);
+    call("ua_rows_update", [&] {
+      return ua_rows_update(out.data_ptr(), (const float*)lse.data_ptr(), blk.data_ptr(), (const float*)blk_lse.data_ptr(), new_out.t.data_ptr(),
+                            (float*)new_lse.t.data_ptr(), (int)out.size(0), (int)out.size(1), (int)out.size(2), (int)out.size(3), half ? UA_FP16 : UA_BF16,
+                            out.scalar_type() == at::kFloat, blk.scalar_type() == at::kFloat, new_out.t.scalar_type() == at::kFloat, Strides(out), ls,
+                            Strides(blk), bls, Strides(new_out.t), nls, on.stream);
+    });
+    return tuple_of(new_out, new_lse);
+  }
   call("ua_merge_update", [&] {
     return ua_merge_update(out.data_ptr(), (const float*)lse.data_ptr(), blk.data_ptr(), (const float*)blk_lse.data_ptr(), new_out.t.data_ptr(),
                            (float*)new_lse.t.data_ptr(), (int)out.size(0), (int)out.size(1), (int)out.size(2), (int)kDim, out.scalar_type() == at::kFloat,

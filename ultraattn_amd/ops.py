@@ -48,7 +48,7 @@ def bsa_fwd(q, k, v, tiles, softmax_scale: Optional[float] = None, causal: bool 
 
 def softmax_delta(out, dout, delta: Optional[torch.Tensor] = None) -> torch.Tensor:
     """delta = rowsum(dout * out) as fp32 [B, Nh, Sq]: the ``softmax_d`` input of the fork's
-    backward (``orchestrated_attn/orchestrated_attn_impl.py:595``)."""
+    backward (``orchestrated_attn/orchestrated_attn_impl.py:595``).  bf16 or fp16 rows, heads of 128 or 64."""
     return native().delta(out, dout, delta)
 
 
@@ -67,7 +67,7 @@ def merge_partials(outs: Sequence[torch.Tensor], lses: Sequence[torch.Tensor],
                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
     """LSE-weighted merge of partial outputs -> (out, lse): one pass in place of the chain of
     ``update_out_and_lse`` calls (``ring_flash_attn/utils.py:38-52, 78-99``).
-    outs[p]: contiguous [B, S, Nh, 128] bf16; lses[p]: contiguous [B, Nh, S] fp32."""
+    outs[p]: contiguous [B, S, Nh, D] of one type, bf16 or fp16, D 128 or 64; lses[p]: contiguous [B, Nh, S] fp32."""
     return native().merge(outs, lses, out, lse)
 
 
@@ -86,8 +86,8 @@ def grad_accumulate(partial: torch.Tensor, out: Optional[torch.Tensor], acc: Opt
 
 def grad_sum(parts: Sequence[torch.Tensor], out: Optional[torch.Tensor] = None, scale: float = 1.0) -> torch.Tensor:
     """``out = bf16(scale * sum(parts))`` with the sum carried in fp32, one pass (``ua_grad_sum``).
-    parts: 1..16 contiguous ``[B, S, Nh, 128]`` tensors, all bf16 or all fp32; ``out`` bf16, may be a
-    strided view (head_dim contiguous)."""
+    parts: 1..16 contiguous ``[B, S, Nh, D]`` tensors, D 128 or 64, all bf16, all fp16 or all fp32; ``out`` (of their type, of fp32 parts bf16 or, if
+    given so, fp16) may be a strided view (head_dim contiguous)."""
     return native().grad_sum(parts, out, scale)
 
 
@@ -107,7 +107,7 @@ def update_out_and_lse(out: Optional[torch.Tensor], lse: Optional[torch.Tensor],
     One kernel (``ua_merge_update``) in place of the reference's eight element-wise launches; the
     arithmetic is max-stabilised and treats ``lse = -inf`` as "no keys", which the literal formula
     does not (it agrees with it on every input where that one is finite).  ``block_lse`` may also
-    come as ``[B,Sb,Nh,1]`` (the hierarchy executor's ``forward`` closure, ``:40-53``)."""
+    come as ``[B,Sb,Nh,1]`` (the hierarchy executor's ``forward`` closure, ``:40-53``).  Rows are bf16 or fp16 (or the fp32 of a later step), heads 128 or 64."""
     if out is None:
         if slice_ is not None:
             raise RuntimeError("first update_out_and_lse should not pass slice_ args")
