@@ -762,7 +762,7 @@ at::Tensor result(Slot& s, const char* name, const at::Tensor& ref) {
   check_written(name, s.t);
   return s.t;
 }
-// Whether two tensors of one type have an element in common: whether the distance of their starts, in elements, is a sum of steps that both can take.
+// Whether two tensors have memory in common: whether the distance of their starts, in elements of the smaller type, is a sum of steps that both can take.
 // Axes of both by falling stride, each with the steps it allows; what the axes below reach leaves few to try (the parts of a packed row: one or two).
 struct Step { int64_t stride, lo, hi; };
 bool reaches(const Step* s, size_t n, int64_t distance, int& budget) {
@@ -787,22 +787,24 @@ inline intptr_t end_of(const at::Tensor& t, intptr_t begin, int64_t size) {     
   return begin + (last + 1) * size;
 }
 bool share(const at::Tensor& a, const at::Tensor& b) {
-  const int64_t size = a.element_size();
+  const int64_t size_a = a.element_size(), size_b = b.element_size(), size = std::min(size_a, size_b);
   const intptr_t from_a = (intptr_t)a.data_ptr(), from_b = (intptr_t)b.data_ptr();
-  const intptr_t to_a = end_of(a, from_a, size), to_b = end_of(b, from_b, size);
+  const intptr_t to_a = end_of(a, from_a, size_a), to_b = end_of(b, from_b, size_b);
   if (from_a >= to_b || from_b >= to_a || from_a == to_a || from_b == to_b) return false;      // apart altogether, as most are
   const int64_t bytes = from_b - from_a;
   if (bytes % size) return true;
   std::vector<Step> s;
-  for (const at::Tensor* t : {&a, &b})
-    for (int64_t i = 0; i < t->dim(); ++i) {
-      const int64_t n = t->size(i) - 1, stride = t->stride(i);
+  for (const at::Tensor* t : {&a, &b}) {
+    const bool ours = t == &a;
+    const int64_t units = (ours ? size_a : size_b) / size;                   // of an element: one more axis
+    for (int64_t i = 0; i <= t->dim(); ++i) {
+      const int64_t n = i < t->dim() ? t->size(i) - 1 : units - 1, stride = i < t->dim() ? t->stride(i) * units : 1;
       if (n == 0 || stride == 0) continue;
-      const bool ours = t == &a;
       auto same = std::find_if(s.begin(), s.end(), [&](const Step& x) { return x.stride == stride; });
       if (same == s.end()) same = s.insert(s.end(), Step{stride, 0, 0});
       (ours ? same->hi : same->lo) += ours ? n : -n;
     }
+  }
   std::sort(s.begin(), s.end(), [](const Step& x, const Step& y) { return x.stride > y.stride; });
   int budget = 4096;
   return reaches(s.data(), s.size(), bytes / size, budget);
@@ -879,6 +881,12 @@ PyObject* rope(PyObject* const* a) {
     }
   }
   if (qo.given) check_in_place("q_out", qo.t, q);
+  for (int i = 2; i < 4; ++i) {
+    if (a[i] == Py_None) continue;
+    const at::Tensor& read = tensor(a[i], "freqs");
+    if (qo.given) check_apart("q_out", qo.t, {&read});
+    if (ko.given) check_apart("k_out", ko.t, {&read});
+  }
   const On on(q);
   init_device(on.device);
   call("ua_rope", [&] {
@@ -909,19 +917,20 @@ PyObject* rope_append(PyObject* const* a) {
   check_shape("v_cache", vc, kc.sizes());
   check_written("k_cache", kc);
   check_written("v_cache", vc);
-  const int32_t* lens = lengths(tensor(a[5], "lens"), q);
+  const at::Tensor &l = tensor(a[5], "lens"), &fr = tensor(a[6], "freqs");
+  const int32_t* lens = lengths(l, q);
   int64_t rotary;
-  const double* f = frequencies(tensor(a[6], "freqs"), q, rotary);
+  const double* f = frequencies(fr, q, rotary);
   const bool interleaved = truth(a[7]);
   const float scale = positive(a[8], "scale");
   Slot qo(a[9]);
   result(qo, "q_out", q);
   if (qo.given) {
-    check_apart("q_out", qo.t, {&k, &v, &kc, &vc});
+    check_apart("q_out", qo.t, {&k, &v, &kc, &vc, &l, &fr});
     check_in_place("q_out", qo.t, q);
   }
-  check_apart("k_cache", kc, {&q, &k, &v, &vc});
-  check_apart("v_cache", vc, {&q, &k, &v});
+  check_apart("k_cache", kc, {&q, &k, &v, &vc, &l, &fr});
+  check_apart("v_cache", vc, {&q, &k, &v, &l, &fr});
   const On on(q);
   init_device(on.device);
   call("ua_rope_append", [&] {
@@ -984,6 +993,7 @@ PyObject* swa_forward(PyObject* const* a) {
     check_apart("out", out.t, {&k, &v});
     check_in_place("out", out.t, q);
   }
+  if (lse.given) check_apart("lse", lse.t, {&q, &k, &v, &out.t});
   const On on(q);
   init_device(on.device);
   const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), sq = (int)q.size(1), sk = (int)k.size(1), D = (int)q.size(3);
@@ -1010,9 +1020,9 @@ PyObject* swa_backward(PyObject* const* a) {
   result(dq, "dq", q);
   result(dk, "dk", k);
   result(dv, "dv", v);
-  if (dq.given) check_apart("dq", dq.t, {&dout, &q, &k, &v, &dk.t, &dv.t});
-  if (dk.given) check_apart("dk", dk.t, {&dout, &q, &k, &v, &dv.t});
-  if (dv.given) check_apart("dv", dv.t, {&dout, &q, &k, &v});
+  if (dq.given) check_apart("dq", dq.t, {&dout, &q, &k, &v, &dk.t, &dv.t, &lse});
+  if (dk.given) check_apart("dk", dk.t, {&dout, &q, &k, &v, &dv.t, &lse});
+  if (dv.given) check_apart("dv", dv.t, {&dout, &q, &k, &v, &lse});
   const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), sq = (int)q.size(1), sk = (int)k.size(1), D = (int)q.size(3);
   const On on(q);
   init_device(on.device);
@@ -1020,6 +1030,9 @@ PyObject* swa_backward(PyObject* const* a) {
   if (a[9] != Py_None) {
     delta = tensor(a[9], "softmax_d");
     check_lse("softmax_d", delta, q);
+    if (dq.given) check_apart("dq", dq.t, {&delta});
+    if (dk.given) check_apart("dk", dk.t, {&delta});
+    if (dv.given) check_apart("dv", dv.t, {&delta});
   } else {
     if (a[4] == Py_None) fail(PyExc_ValueError, "either out or softmax_d is required");
     const at::Tensor& out = tensor(a[4], "out");
@@ -1047,7 +1060,8 @@ PyObject* swa_decode(PyObject* const* a) {
   const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k_cache"), &v = tensor(a[2], "v_cache");
   check_swa(q, k, v, "k_cache", "v_cache");
   const int dt = dtype_code("q", q, false);
-  const int32_t* lens = lengths(tensor(a[3], "lens"), q);
+  const at::Tensor& l = tensor(a[3], "lens");
+  const int32_t* lens = lengths(l, q);
   const int64_t left = integer(a[4]), sinks = integer(a[5]);
   if (left < -1) fail(PyExc_ValueError, "window must be -1 (no bound) or a number of keys");
   if (sinks < 0) fail(PyExc_ValueError, "sinks must be a number of keys");
@@ -1057,9 +1071,10 @@ PyObject* swa_decode(PyObject* const* a) {
   if (lse.given) check_lse("lse", lse.t = tensor(lse.given, "lse"), q);
   else lse.t = stat_of(q);
   if (out.given) {
-    check_apart("out", out.t, {&k, &v});
+    check_apart("out", out.t, {&k, &v, &l});
     check_in_place("out", out.t, q);
   }
+  if (lse.given) check_apart("lse", lse.t, {&q, &k, &v, &out.t, &l});
   const On on(q);
   init_device(on.device);
   const int B = (int)q.size(0), T = (int)q.size(1), H = (int)q.size(2), Hk = (int)k.size(2), room = (int)k.size(1), D = (int)q.size(3);
