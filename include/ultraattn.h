@@ -341,7 +341,7 @@ int ua_rope_append(const void *q, const void *k, const void *v, void *q_out, voi
  * shards: the chunk of keys that another rank holds, or queries that follow a cached prefix (q_start = k_start + seqlen_k - seqlen_q).
  * q, o [batch, seqlen_q, n_heads, head_dim]; k, v [batch, seqlen_k, n_kv_heads, head_dim]: key head h serves query heads
  * h * n_heads / n_kv_heads ...  Any lengths (0 too, up to 2^28), head_dim 64 or 128, dtype UA_BF16 or UA_FP16; pointers 16-byte
- * aligned, element strides multiples of 8 (inputs may have strides of 0: broadcast).  lse [batch, n_heads, seqlen_q] fp32, contiguous, natural log: rows
+ * aligned, element strides multiples of 8 (inputs may have strides of 0: broadcast); softmax_scale from 2^-64 to 2^64.  lse [batch, n_heads, seqlen_q] fp32, contiguous, natural log: rows
  * that see no key get o = 0, lse = -inf, and ua_rows_merge / ua_rows_update join shards (bf16 heads of 128 also ua_merge / ua_merge_update).  Scores, statistics and sums are 32 bits; P is rounded
  * to dtype for its product with V, as it is in ua_bsa_fwd.
  * Few long walks are cut into parts, whose fp32 results are merged in a second launch, if `workspace` (16-byte aligned,

@@ -973,7 +973,12 @@ struct Window {
     if (q_start > kMost || q_start < -kMost || k_start > kMost || k_start < -kMost) fail(PyExc_ValueError, "q_start and k_start must be positions");
   }
 };
-float swa_scale(PyObject* o, int64_t dim) { return o == Py_None ? (float)(1.0 / std::sqrt((double)dim)) : positive(o, "softmax_scale"); }
+float swa_scale(PyObject* o, int64_t dim) {
+  if (o == Py_None) return (float)(1.0 / std::sqrt((double)dim));
+  const float x = positive(o, "softmax_scale");
+  if (x < 0x1p-64f || x > 0x1p64f) fail(PyExc_ValueError, "softmax_scale must be between 2^-64 and 2^64");
+  return x;
+}
 at::Tensor scratch(int64_t bytes, const at::Tensor& like) { return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor(); }
 
 // swa_forward(q, k, v, left, right, sinks, q_start, k_start, softmax_scale, out, lse) -> (out, lse)

@@ -256,6 +256,8 @@ inline SwaSteps swa_row_steps(const SwaParams& p) {
 int swa_fill(SwaParams& p, int batch, int n_heads, int n_kv_heads, int seq_q, int seq_k, int head_dim, int dtype, int64_t q_start, int64_t k_start,
              int64_t left, int64_t right, int64_t sinks, float softmax_scale);
 bool swa_strides_ok(const int64_t* s, bool written);
+// The backward starts scores from -lse / scale, in 32 bits: both, and scale * log2(e), stay far from their ends.
+inline bool swa_scale_ok(float scale) { return scale >= 0x1p-64f && scale <= 0x1p64f; }
 // Merge of fp32 partial rows: see merge_rows_kernel.
 int swa_merge(const float* part_o, int64_t o_part, const float* part_lse, int64_t lse_part, int n_parts, void* o, const Strides3& os, float* lse,
               int batch, int n_heads, int seq, int head_dim, int dtype, hipStream_t st);

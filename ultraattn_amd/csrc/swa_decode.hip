@@ -267,7 +267,7 @@ static int dec_check(int batch, int n_tokens, int n_heads, int n_kv_heads, int r
   if (room > kSwaMaxLen || n_tokens > kSwaMaxLen || (int64_t)n_tokens * (n_heads / n_kv_heads) > kSwaMaxLen ||
       (int64_t)batch * n_tokens * n_heads > INT32_MAX / kDecMaxParts)
     return UA_ERR_SHAPE;
-  if ((head_dim != 64 && head_dim != 128) || (dtype != UA_BF16 && dtype != UA_FP16) || !(scale > 0.f)) return UA_ERR_UNSUPPORTED;
+  if ((head_dim != 64 && head_dim != 128) || (dtype != UA_BF16 && dtype != UA_FP16) || !swa_scale_ok(scale)) return UA_ERR_UNSUPPORTED;
   return UA_OK;
 }
 template <class T, int kD>

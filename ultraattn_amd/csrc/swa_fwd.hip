@@ -274,7 +274,7 @@ int swa_fill(SwaParams& p, int batch, int n_heads, int n_kv_heads, int seq_q, in
   if (q_start > kMost || q_start < -kMost || k_start > kMost || k_start < -kMost || left < -1 || right < -1 || left > kMost || right > kMost || sinks < 0 ||
       sinks > kMost)
     return UA_ERR_SHAPE;
-  if ((head_dim != 64 && head_dim != 128) || (dtype != UA_BF16 && dtype != UA_FP16) || !(softmax_scale > 0.f)) return UA_ERR_UNSUPPORTED;
+  if ((head_dim != 64 && head_dim != 128) || (dtype != UA_BF16 && dtype != UA_FP16) || !swa_scale_ok(softmax_scale)) return UA_ERR_UNSUPPORTED;
   auto clamp = [](int64_t x) { return (int)std::min<int64_t>(std::max<int64_t>(x, -kFar), kFar); };
   p.batch = batch; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.group = n_heads / n_kv_heads; p.seq_q = seq_q; p.seq_k = seq_k;
   p.hi = right < 0 ? kFar : clamp(q_start - k_start + right);
