@@ -59,6 +59,7 @@ extern "C" {
 #define UA_HEAD_DIM 128    /* the only supported head dimension */
 #define UA_MAX_PARTS 16    /* most partial outputs one ua_merge call combines */
 #define UA_ROPE_MAX_DIM 512 /* largest head_dim of the rotary entry points */
+#define UA_SWA_MAX_TOKEN_STRIDE 4194303   /* elements from token to token of what the sliding-window kernels walk */
 #define UA_NOALLOC_MAX_LINES 65532   /* most query tiles + key tiles of ua_tilelist_build_device_noalloc */
 
 /* Element types of the entry points that take more than bf16. */
@@ -341,7 +342,8 @@ int ua_rope_append(const void *q, const void *k, const void *v, void *q_out, voi
  * shards: the chunk of keys that another rank holds, or queries that follow a cached prefix (q_start = k_start + seqlen_k - seqlen_q).
  * q, o [batch, seqlen_q, n_heads, head_dim]; k, v [batch, seqlen_k, n_kv_heads, head_dim]: key head h serves query heads
  * h * n_heads / n_kv_heads ...  Any lengths (0 too, up to 2^28), head_dim 64 or 128, dtype UA_BF16 or UA_FP16; pointers 16-byte
- * aligned, element strides multiples of 8 (inputs may have strides of 0: broadcast); softmax_scale from 2^-64 to 2^64.  lse [batch, n_heads, seqlen_q] fp32, contiguous, natural log: rows
+ * aligned, element strides multiples of 8 (inputs may have strides of 0: broadcast); softmax_scale from 2^-64 to 2^64.
+ * What a kernel walks (k and v; in the backward q and dout too) has token strides up to UA_SWA_MAX_TOKEN_STRIDE, else UA_ERR_SHAPE.  lse [batch, n_heads, seqlen_q] fp32, contiguous, natural log: rows
  * that see no key get o = 0, lse = -inf, and ua_rows_merge / ua_rows_update join shards (bf16 heads of 128 also ua_merge / ua_merge_update).  Scores, statistics and sums are 32 bits; P is rounded
  * to dtype for its product with V, as it is in ua_bsa_fwd.
  * Few long walks are cut into parts, whose fp32 results are merged in a second launch, if `workspace` (16-byte aligned,

@@ -947,6 +947,12 @@ Strides used_strides(const at::Tensor& t) {
   auto of = [&](int i) { return t.size(i) > 1 ? t.stride(i) : kDim; };
   return Strides(of(0), of(1), of(2));
 }
+// The kernels copy blocks of 64 tokens of these at offsets in 32 bits.
+void check_token_stride(const char* name, const at::Tensor& t) {
+  if (t.size(1) > 1 && t.stride(1) > UA_SWA_MAX_TOKEN_STRIDE)
+    fail(PyExc_ValueError, std::string(name) + ": its tokens lie " + std::to_string(t.stride(1)) + " elements apart, at most " + std::to_string(UA_SWA_MAX_TOKEN_STRIDE) +
+                               " are supported");
+}
 void check_swa(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const char* k_name, const char* v_name) {
   dtype_code("q", q, false);
   check_rows4("q", q, q);
@@ -955,6 +961,8 @@ void check_swa(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, co
   if (q.size(3) != 64 && q.size(3) != 128) fail(PyExc_ValueError, "head_dim must be 64 or 128, got " + std::to_string(q.size(3)));
   check_shape(k_name, k, {q.size(0), k.size(1), k.size(2), q.size(3)});
   check_shape(v_name, v, k.sizes());
+  check_token_stride(k_name, k);
+  check_token_stride(v_name, v);
   if (q.size(2) < 1 || k.size(2) < 1 || q.size(2) % k.size(2))
     fail(PyExc_ValueError, std::to_string(q.size(2)) + " query heads cannot share " + std::to_string(k.size(2)) + " key heads evenly");
 }
@@ -1018,6 +1026,8 @@ PyObject* swa_backward(PyObject* const* a) {
   const int dt = dtype_code("q", q, false);
   check_rows4("dout", dout, q);
   check_shape("dout", dout, q.sizes());
+  check_token_stride("q", q);
+  check_token_stride("dout", dout);
   check_lse("lse", lse, q);
   const Window w(a + 10, q.size(1), k.size(1));
   const float scale = swa_scale(a[15], q.size(3));

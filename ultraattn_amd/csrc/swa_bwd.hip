@@ -664,7 +664,7 @@ extern "C" int ua_swa_bwd(const void* dout, const void* q, const void* k, const 
   for (const int64_t* s : {dq_strides, dk_strides, dv_strides})
     if (!swa_strides_ok(s, true)) return UA_ERR_ALIGN;
   for (const int64_t* s : {do_strides, q_strides, k_strides, v_strides})
-    if (s[1] > (INT32_MAX >> 9)) return UA_ERR_SHAPE;
+    if (s[1] > UA_SWA_MAX_TOKEN_STRIDE) return UA_ERR_SHAPE;
   rc = check_device();
   if (rc != UA_OK) return rc;
   auto three = [](const int64_t* s) { return Strides3{s[0], s[1], s[2]}; };

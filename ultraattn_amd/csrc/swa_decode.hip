@@ -298,7 +298,7 @@ extern "C" int ua_swa_decode(const void* q, const void* k_cache, const void* v_c
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o) || !aligned4(lens) || !swa_strides_ok(q_strides, false) ||
       !swa_strides_ok(k_strides, false) || !swa_strides_ok(v_strides, false) || !swa_strides_ok(o_strides, true))
     return UA_ERR_ALIGN;
-  if (k_strides[1] > (INT32_MAX >> 9) || v_strides[1] > (INT32_MAX >> 9)) return UA_ERR_SHAPE;
+  if (k_strides[1] > UA_SWA_MAX_TOKEN_STRIDE || v_strides[1] > UA_SWA_MAX_TOKEN_STRIDE) return UA_ERR_SHAPE;
   rc = check_device();
   if (rc != UA_OK) return rc;
   DecShape s = dec_shape(batch, n_tokens, n_heads, n_kv_heads, room, head_dim, left, sinks);

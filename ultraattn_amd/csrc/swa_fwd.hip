@@ -340,7 +340,7 @@ extern "C" int ua_swa_fwd(const void* q, const void* k, const void* v, void* o, 
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !swa_strides_ok(q_strides, false) || !swa_strides_ok(k_strides, false) ||
       !swa_strides_ok(v_strides, false) || !swa_strides_ok(o_strides, true))
     return UA_ERR_ALIGN;
-  if (k_strides[1] > (INT32_MAX >> 9) || v_strides[1] > (INT32_MAX >> 9)) return UA_ERR_SHAPE;
+  if (k_strides[1] > UA_SWA_MAX_TOKEN_STRIDE || v_strides[1] > UA_SWA_MAX_TOKEN_STRIDE) return UA_ERR_SHAPE;
   rc = check_device();
   if (rc != UA_OK) return rc;
   p.q = q; p.k = k; p.v = v; p.o = o; p.lse = lse;

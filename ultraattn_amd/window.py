@@ -1,7 +1,8 @@
 """Sliding-window attention with sinks on one MI355X: forward, backward, and new tokens against a cache.
 
 Host side of ``ua_swa_*`` in ``include/ultraattn.h``, beside the block-sparse operators of ``ops.py`` and in their manner: row tensors
-``[B, S, H, D]`` with any (batch, token, head) strides, ``lse`` ``[B, H, S]`` fp32 in natural logarithm, results written in place when
+``[B, S, H, D]`` with any (batch, token, head) strides (multiples of 8; from token to token of keys and values, in the backward of ``q`` and ``dout`` too,
+at most 4194303 elements), ``lse`` ``[B, H, S]`` fp32 in natural logarithm, results written in place when
 given (``out`` may be ``q`` itself; results overlap nothing else), everything on the current CUDA(HIP) stream, nothing synchronises.  Types are bf16 and fp16, D is 64 or 128, lengths are arbitrary, and keys
 may have fewer heads than queries (each serves ``Hq / Hk`` consecutive ones).
 
