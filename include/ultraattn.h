@@ -59,6 +59,7 @@ extern "C" {
 #define UA_HEAD_DIM 128    /* the only supported head dimension */
 #define UA_MAX_PARTS 16    /* most partial outputs one ua_merge call combines */
 #define UA_ROPE_MAX_DIM 512 /* largest head_dim of the rotary entry points */
+#define UA_ROPE_MAX_POSITION (INT64_C(1) << 53)   /* largest size of a position that is turned exactly */
 #define UA_SWA_MAX_TOKEN_STRIDE 4194303   /* elements from token to token of what the sliding-window kernels walk */
 #define UA_NOALLOC_MAX_LINES 65532   /* most query tiles + key tiles of ua_tilelist_build_device_noalloc */
 
@@ -314,8 +315,8 @@ int ua_copy_in(void *dst, const void *src, int64_t bytes, void *stream);
  * x [batch, seqlen, heads, head_dim] of `dtype` (UA_BF16, UA_FP16, UA_FP32) with (batch, token, head) element strides, any
  * of them; wide strides and pointers (16 bytes) make wide accesses.  q and k are turned in one launch; n_kv_heads = 0 (or n_heads = 0) leaves one
  * out.  Outputs may be exactly the inputs (same pointer and strides) or not overlap them.
- * freqs: DEVICE array of rotary_dim / 2 doubles, radians per position.  The angle is reduced in twice 64 bits: far positions lose
- * nothing.  positions: DEVICE array of int32 (positions_64 = 0) or int64, read at b * position_stride_b + s * position_stride_s; NULL:
+ * freqs: DEVICE array of rotary_dim / 2 doubles, radians per position.  The angle is reduced in twice 64 bits: positions up to
+ * UA_ROPE_MAX_POSITION in size lose nothing (a `start` beyond it is refused, a position on the device is the caller's to keep below).  positions: DEVICE array of int32 (positions_64 = 0) or int64, read at b * position_stride_b + s * position_stride_s; NULL:
  * token s is at start + s. */
 int ua_rope(const void *q, const void *k, void *q_out, void *k_out, const double *freqs,
             const void *positions, int positions_64, int64_t position_stride_b, int64_t position_stride_s, int64_t start,

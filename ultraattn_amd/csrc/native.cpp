@@ -867,6 +867,7 @@ PyObject* rope(PyObject* const* a) {
     pos_b = t.dim() == 2 ? t.stride(0) : 0;
   }
   const int64_t start = integer(a[4]);
+  if (!pos && (start > UA_ROPE_MAX_POSITION - q.size(1) || start < -UA_ROPE_MAX_POSITION)) fail(PyExc_ValueError, "positions from start on must be within 2^53");
   const bool interleaved = truth(a[5]), inverse = truth(a[6]);
   const float scale = positive(a[7], "scale");
   Slot qo(a[8]), ko(a[9]);

@@ -45,7 +45,7 @@ __device__ __forceinline__ int64_t rope_position(const RopeParams& p, int b, int
 }
 
 // cos and sin of position * freq.  The angle in turns is a product in twice 64 bits, of which only the part behind the point is
-// used: far positions lose nothing (position 2^31 with one rounding in 64 bits is 5e-7 off, as much as a cosine in 32 bits has).
+// used: far positions, up to UA_ROPE_MAX_POSITION where 64 bits hold them, lose nothing (position 2^31 with one rounding in 64 bits is 5e-7 off, as much as a cosine in 32 bits has).
 __device__ __forceinline__ void rope_angle(int64_t pos, double freq, float& c, float& s) {
 #pragma clang fp contract(off)         // (turns - rint(turns) as one fma would count `rest` twice)
   constexpr double kHi = 0.15915494309189535, kLo = -9.839338337591e-18;       // 1 / (2 pi) = kHi + kLo
@@ -269,6 +269,7 @@ extern "C" int ua_rope(const void* q, const void* k, void* q_out, void* k_out, c
   const RopeShape s{batch, seqlen, head_dim, rotary_dim, dtype};
   const int rc = rope_check(s, n_heads, n_kv_heads, scale);
   if (rc != UA_OK) return rc;
+  if (!positions && (start > UA_ROPE_MAX_POSITION - seqlen || start < -UA_ROPE_MAX_POSITION)) return UA_ERR_SHAPE;
   if ((int64_t)batch * seqlen == 0) return UA_OK;
   if (!freqs || (n_heads && (!q || !q_out || !q_strides || !q_out_strides)) || (n_kv_heads && (!k || !k_out || !k_strides || !k_out_strides)))
     return UA_ERR_NULL;

@@ -57,7 +57,7 @@ def rope_fwd(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, po
     Pair i is turned by ``position * freqs[i]`` and multiplied by ``scale``; pairs are ``(x[i], x[i + n])`` of the first ``2 n``
     entries, ``n = len(freqs)``, or with ``interleaved`` ``(x[2i], x[2i + 1])``; what is behind them passes through.  Token s is at
     ``start + s``, or at ``positions`` (int32 or int64, ``[S]`` or ``[B, S]``, in any order).  Angles are reduced in more than
-    64 bits, so far positions are as exact as near ones.  ``q_out=q`` works in place; an output may not overlap an input otherwise."""
+    64 bits, so far positions (up to 2^53 in size; ``start`` is checked) are as exact as near ones.  ``q_out=q`` works in place; an output may not overlap an input otherwise."""
     return native().rope(q, k, freqs, positions, start, interleaved, False, scale, q_out, k_out)
 
 
