@@ -30,7 +30,7 @@ extern "C" const char* ua_strerror(int rc) {
     case UA_OK: return "ok";
     case UA_ERR_NULL: return "a required pointer is NULL";
     case UA_ERR_SHAPE: return "non-positive or inconsistent sizes";
-    case UA_ERR_UNSUPPORTED: return "unsupported configuration (head_dim, softmax_scale > 0, 1..16 partials, element type)";
+    case UA_ERR_UNSUPPORTED: return "unsupported configuration (head_dim 128, of sliding windows and joined rows 64 too, softmax_scale > 0, 1..16 partials, element type)";
     case UA_ERR_ALIGN: return "pointer not 16-byte aligned or stride not a multiple of 8 elements";
     case UA_ERR_MASK: return "block mask holds a value other than 0 (EMPTY), 1 (FULL), 2 (CAUSAL)";
     case UA_ERR_LAUNCH: return "HIP kernel launch failed";
