@@ -8,6 +8,8 @@
 // one key (query), so that P and dS, rounded, are operands of the next products.  Both sides are one launch: neither leaves the device partly
 // empty at its end.
 //
+// P and dS are rounded to the operands' type for the products that sum them, as P is in the forward; everything else stays in fp32.
+//
 // A column of the sinks is seen by every later query: its walk is cut into parts of about the others' length, which leave fp32 dK and
 // dV that a last launch adds in their order.  So are all walks where there are few of them.
 #include <algorithm>
@@ -551,13 +553,18 @@ struct BwdCut {
   int row_parts, n_sink, col_parts[2];            // n_sink: tiles of the first run of columns
   int64_t dq_bytes, col_bytes[2], total;          // of a part; of a part's dK
 };
-// Walks are cut to about what a workgroup has on average with two of them on every CU, `each`, where the time that the longest take beyond that
-// is well above what the parts cost: their rows' way through memory and the launch that adds them.  Lengths are counted in products of 64 rows (0.8 us where
-// two workgroups share every CU, 0.5 where they hardly do); a column's step has four of them and a row's three.  us, whole and cut as taken here:
-//     128 columns   16 heads, 4096, window 1024, 4 sinks      155   120        64 columns   14 heads on 2, 3000, window 464        99    38
-//                   4, 2048 causal                           61.7  44.2                     2, 8192, window 2048, 70 sinks        184    54
-//                   32 on 8, 100 x 16384                      374   128                     2 x 10 on 5, 1333 x 2048, window 700  47.1  43.5
-//                   8 on 2, 16384, window 4096, 16 sinks     2085   728                     (the sinks' columns alone: 740)
+// Walks are cut to about what a workgroup has on average with two of them on every CU (of heads of 64 as well, of which three fit), `each`, where the time
+// that the longest take beyond that is well above what the parts cost: their rows' way through memory and the launch that adds them.  Lengths are counted in
+// products of 64 rows (0.8 us where two workgroups share every CU, 0.5 where they hardly do); a column's step has four of them and a row's three.
+// us, whole and cut as taken here:
+//     128 columns   16 heads, 4096, window 1024, 4 sinks      154   116        64 columns   14 heads on 2, 3000, window 464       102    39
+//                   4, 2048 causal                           62.0  44.3                     2, 8192, window 2048, 70 sinks        191    54
+//                   32 on 8, 100 x 16384                      380   131                     2 x 10 on 5, 1333 x 2048, window 700  49.5  44.7
+//                   8 on 2, 16384, window 4096, 16 sinks     2136   721
+// Against a cut of every walk of more than 1.5 each + 24 products, forward and backward in one, both rules in turn, 22 drawn shapes on which they differ (of
+// 147): 5 to 20 % faster in fourteen (16 heads on 2 of 64, 1332 and 1924 causal, 65 -> 59 and 91 -> 81; 8 on 2, 956, window 110, 60 -> 48), up to 3 % in three, slower
+// in five (4 x 32 on 8, 290 causal, 58 -> 66; 2 x 32 on 4 of 64, 3781, window 234, 139 -> 147).  Slower too where only a little is left beyond `each`, which
+// runs on alone faster than is counted here: 8 on 2, 16384, window 4096, 971 -> 981; 16 on 4, 8192, window 2048, 523 -> 529.
 static BwdCut bwd_cut(const SwaParams& p, int head_dim, bool cut) {
   BwdCut c{1, 0, {1, 1}, 0, {0, 0}, 0};
   const double cols = (double)p.batch * p.n_kv_heads, rows = (double)p.batch * p.n_heads * p.n_qtiles;

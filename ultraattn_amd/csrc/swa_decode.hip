@@ -5,7 +5,9 @@
 // waits for another before the end, where their rows are merged.  The keys of long caches are cut into parts, workgroups of their own, that leave fp32 rows
 // for a merge.
 //
-// Bound: HBM, the visible keys and values once per key head.  Two stages of 16 KiB a wave keep 64 to 128 KiB in flight on every CU.
+// Bound: HBM, the visible keys and values once per 32 rows of a key head: from 33 rows on (5 tokens of 7 heads, say) another workgroup reads them again, seldom
+// from a cache (64 x 8 key heads of 8000: 32 rows 375 us, 35 to 64 rows 600).  Two stages of 16 KiB a wave keep 64 to 128 KiB in flight on every CU.
+// P is rounded as in the forward.
 #include <algorithm>
 #include <cmath>
 #include "swa.h"
@@ -237,11 +239,11 @@ __global__ __launch_bounds__(64 * kDecWaves) void swa_decode_kernel(const DecPar
 struct DecShape { int tiles, row_tiles, parts; };        // 16-row tiles of a workgroup, workgroups of a key head's rows, parts of its keys
 // Parts of a key head's keys: what an estimate in microseconds says of the longest caches that the call allows (lengths are on the device).  A round of
 // workgroups on all CUs takes its start and its iterations, or what its keys take from memory; whole caches of a batch differ in length, and the longest
-// ones end alone (64 x 8 of 8192 to 16384 keys, whole 584 us, in four parts 552); parts cost the launch that merges them.
+// ones end alone (64 x 8 of 8192 to 16384 keys, whole 582 us, in two or four parts 565); parts cost the launch that merges them.
 // us in 1, 2, 4, 8, 16 and 32 parts (sequences x key heads, keys, columns):
-//     1 x 8, 1027, 128    11.7  11.3  10.3  10.3  10.1  10.3        8 x 8, 4000, 128      32.3  27.0  26.8  28.8  36.0  43.7
-//     1 x 8, 8000, 128    56.1  34.5  22.0  15.5  13.0  12.8        16 x 8, 1027, 128     15.6  17.5  22.4  30.0  38.5  63.6
-//     4 x 1, 16000, 128  106.3  59.8  34.3  22.0  16.0  14.5        32 x 8, 2000, 64      24.2  26.0  26.4  29.5  34.6  55.8
+//     1 x 8, 1027, 128    12.2  11.6  10.7  10.1   9.9  10.2        8 x 8, 4000, 128      33.3  27.1  26.9  29.2  36.6  45.5
+//     1 x 8, 8000, 128    57.9  35.7  22.9  16.0  13.3  13.1        16 x 8, 1027, 128     15.8  17.7  23.5  30.3  39.7  65.2
+//     4 x 1, 16000, 128  110.5  61.6  36.6  22.9  16.6  14.9        32 x 8, 2000, 64      24.1  26.0  27.0  29.3  35.8  55.4
 static DecShape dec_shape(int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int head_dim, int64_t left, int64_t sinks) {
   DecShape s;
   const int64_t rows = (int64_t)n_tokens * (n_heads / n_kv_heads);

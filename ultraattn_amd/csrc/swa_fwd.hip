@@ -6,6 +6,9 @@
 // are skipped by it.  K and V come in through two LDS stages, the next block's copies between this one's matrix instructions.
 //
 // The running maximum is raised only where a block's sums show a score far above it, or where a row has not seen a key yet.
+//
+// P is rounded to the operands' type, which the matrix instruction asks for: independent errors of half a step, which the sum over the keys averages,
+// beside the output's own (error against 64 bits: bf16 1.9e-3, with P in 32 bits 1.6e-3).  Scores, the row sums and O stay in fp32.
 #include <algorithm>
 #include <type_traits>
 #include "swa.h"
@@ -203,7 +206,6 @@ __global__ __launch_bounds__(256) void merge_rows_kernel(const float* part_o, in
   float total = w, acc[kPer] = {};
 #pragma unroll
   for (int d = kLanes / 2; d; d /= 2) total += __shfl_xor(total, d);
-#pragma unroll 4
   for (int i0 = 0; i0 < n_parts; i0 += kGroups) {
     const int i = i0 + (lane >> 4);
     const float f = __shfl(w, i % kLanes, kLanes);
@@ -292,12 +294,13 @@ int swa_fill(SwaParams& p, int batch, int n_heads, int n_kv_heads, int seq_q, in
 }
 
 // Parts that a forward's walks are cut into: what an estimate of the launch's time in microseconds says.  A step takes `alone` where a CU has one
-// workgroup and `shared` where it has two; parts cost a launch for their merge, and each its rows' way through the caches.  us, whole and in
-// 2, 4, 8 and 16 parts (heads, queries x keys, window):
-//     128 columns   4, 2048 causal     37.3   28.6   24.1   26.5   34.4          64 columns   8, 2048 causal       28.2  24.4  22.5  28.6  33.8
-//                   8, 128 x 4096      67.1   41.3   27.0   19.7   18.2                       2, 8192, 2047        32.8  26.0  26.0  32.5  40.0
-//                  32, 100 x 16384    255    135     73.9   48.8   47.2                       8, 512 causal        10.6  12.0  11.7  11.7  13.1
-//                   4, 8192, 2047      44.3   53.1   60.1   83.9  137                         2 x 10, 1333 x 2048, 700  19.5  25.4
+// workgroup and `shared` where it has two; parts cost a launch for their merge, and each its rows' way through the caches.  (Of heads of 64 three fit a
+// CU; the estimate counts two for them as well, and its constants were fitted that way.)  us, whole and in 2, 4, 8 and 16 parts (heads, queries x
+// keys, window):
+//     128 columns   4, 2048 causal     37.0   28.4   23.9   26.8   34.1          64 columns   8, 2048 causal       29.4  25.0  22.9  29.0  33.6
+//                   8, 128 x 4096      66.6   41.1   27.0   19.8   18.4                       2, 8192, 2047        34.3  26.8  26.2  32.4  39.8
+//                  32, 100 x 16384    255    135     74.1   46.5   45.5                       8, 512 causal        10.9  12.2  11.7  11.6  13.3
+//                   4, 8192, 2047      44.3   52.5   58.3   82.6  136                         2 x 10, 1333 x 2048, 700  20.3  25.4  28.4  37.3  49.8
 static int fwd_parts(const SwaParams& p, int head_dim) {
   const double lines = (double)p.batch * p.n_heads * p.n_qtiles;
   if (lines == 0 || lines >= 2 * kCus) return 1;
