@@ -198,3 +198,26 @@ def test_refusals():
         with pytest.raises((ValueError, TypeError, RuntimeError)):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_results_over_operands_are_refused():
+    (a, b), (la, lb) = random_parts(2, (1, 16, 2, 64), torch.float16)
+    run = la.transpose(1, 2).unsqueeze(-1).contiguous()
+    flat = torch.zeros(3 * a.numel(), dtype=torch.float16, device=DEV)
+    view = lambda at, like=a: flat[at:at + like.numel()].view(like.shape)  # noqa: E731
+    stat = lambda at: flat[at:at + 2 * la.numel()].view(torch.float32).view(la.shape)  # noqa: E731
+    wide = flat[:2 * a.numel()].view(torch.float32).view(a.shape)
+    bad = [lambda: ua.merge_partials([view(0), b], [la, lb], out=view(64)), lambda: ua.merge_partials([a, b], [la, lb], out=view(0), lse=stat(128)),
+           lambda: ua.merge_partials([a, b], [stat(0), lb], lse=stat(2)), lambda: ua.merge_partials([view(0), b], [la, lb], lse=stat(128)),
+           lambda: ua.merge_partials([a, b], [stat(0), lb], out=view(0)), lambda: ua.grad_sum([view(0), b], out=view(64)), lambda: ua.grad_sum([wide], out=view(0)),
+           lambda: ua.grad_sum([a, b], out=a[:, :1].expand_as(a)), lambda: ua.softmax_delta(view(0), b, stat(0)),
+           lambda: ua.update_out_and_lse(view(0), run, view(64), lb, slice_=(slice(None),)), lambda: ua.update_out_and_lse(a[:, :1].expand_as(a), run, b, lb, slice_=(slice(None),)),
+           lambda: ua.update_out_and_lse(a, run[:, :1].expand_as(run), b, lb, slice_=(slice(None),)), lambda: ua.update_out_and_lse(a, run, a, lb, slice_=(slice(None),))]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+            pytest.fail(f"call {i} was taken")
+    beside = ua.merge_partials([view(0), view(a.numel())], [la, lb], out=view(2 * a.numel()))
+    assert torch.equal(beside[0], ua.merge_partials([view(0).clone(), view(a.numel()).clone()], [la, lb])[0])
+    same = a.clone()
+    assert torch.equal(ua.grad_sum([same, b], out=same), ua.grad_sum([a, b]))

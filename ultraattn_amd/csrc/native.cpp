@@ -205,6 +205,9 @@ void check_rows_first(const char* name, const at::Tensor& t) {
     fail(PyExc_TypeError, std::string(name) + " must be bfloat16 or float16, got " + c10::toString(t.scalar_type()));
   check_rows_of(name, t, t.scalar_type(), t.dim() == 4 && t.size(3) == 64 ? 64 : kDim);
 }
+void check_written(const char* name, const at::Tensor& t);
+void check_apart(const char* name, const at::Tensor& written, std::initializer_list<const at::Tensor*> others);
+void check_in_place(const char* name, const at::Tensor& written, const at::Tensor& x);
 void check_beside(const char* name, const at::Tensor& t, const at::Tensor& first) {
   if (t.device() != first.device()) fail(PyExc_ValueError, std::string(name) + " is on another device than the first tensor");
 }
@@ -218,6 +221,7 @@ at::Tensor delta_of(const at::Tensor& out, const at::Tensor& dout, at::Tensor de
     if (!delta.defined()) delta = stat_of(out);
     check_stat("delta", delta, out);
     check_beside("delta", delta, out);
+    check_apart("delta", delta, {&out, &dout});
     const On on(out);
     call("ua_rows_delta", [&] {
       return ua_rows_delta(out.data_ptr(), dout.data_ptr(), (float*)delta.data_ptr(), (int)out.size(0), (int)out.size(1), (int)out.size(2), (int)out.size(3),
@@ -591,6 +595,16 @@ PyObject* merge(PyObject* const* a) {
   if (!plain) {
     check_beside("out", out.t, first);
     check_beside("lse", lse.t, first);
+    if (out.given || lse.given) {                          // each row is written by those that read it
+      check_apart("out", out.t, {&lse.t});
+      for (int64_t i = 0; i < n; ++i) {
+        const at::Tensor &o = outs.at(i, "partial out"), &l = lses.at(i, "partial lse");
+        check_in_place("out", out.t, o);
+        check_in_place("lse", lse.t, l);
+        check_apart("out", out.t, {&l});
+        check_apart("lse", lse.t, {&o});
+      }
+    }
     call("ua_rows_merge", [&] {
       return ua_rows_merge(op, lp, (int)n, out.t.data_ptr(), (float*)lse.t.data_ptr(), (int)first.size(0), (int)first.size(1), (int)first.size(2),
                            (int)first.size(3), rows_code(first), on.stream);
@@ -630,6 +644,13 @@ PyObject* grad_sum(PyObject* const* a) {
     check_rows_first("out", out.t);
     check_rows_of("out", out.t, dt == at::kFloat ? out.t.scalar_type() : dt, dim);
     for (int64_t i = 0; i < n; ++i) check_beside("partial gradient", parts.at(i, "partial gradient"), out.t);
+  }
+  if (!plain && out.given && out.t.sizes().equals(first.sizes())) {
+    check_written("out", out.t);
+    for (int64_t i = 0; i < n; ++i) {
+      const at::Tensor& t = parts.at(i, "partial gradient");
+      if (dt == at::kFloat) check_apart("out", out.t, {&t}); else check_in_place("out", out.t, t);
+    }
   }
   if (!out.t.sizes().equals(first.sizes())) fail(PyExc_ValueError, "out must have the partials' shape");
   const float scale = (float)number(a[2]);
@@ -682,6 +703,12 @@ PyObject* merge_update(PyObject* const* a) {
   if (half || out.size(3) != kDim) {
     if (half && (out.scalar_type() == at::kBFloat16 || blk.scalar_type() == at::kBFloat16)) fail(PyExc_TypeError, "out and block_out must be of one type, or float32");
     for (const at::Tensor* t : {&lse, &blk, &blk_lse}) check_beside("an operand", *t, out);
+    if (in_place) {
+      check_written("out", out);
+      check_written("lse", lse);
+      check_apart("out", out, {&blk, &lse, &blk_lse});
+      check_apart("lse", lse, {&blk, &blk_lse});
+    }
     call("ua_rows_update", [&] {
       return ua_rows_update(out.data_ptr(), (const float*)lse.data_ptr(), blk.data_ptr(), (const float*)blk_lse.data_ptr(), new_out.t.data_ptr(),
                             (float*)new_lse.t.data_ptr(), (int)out.size(0), (int)out.size(1), (int)out.size(2), (int)out.size(3), half ? UA_FP16 : UA_BF16,
