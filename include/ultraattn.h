@@ -61,6 +61,7 @@ extern "C" {
 #define UA_ROPE_MAX_DIM 512 /* largest head_dim of the rotary entry points */
 #define UA_ROPE_MAX_POSITION (INT64_C(1) << 53)   /* largest size of a position that is turned exactly */
 #define UA_SWA_MAX_TOKEN_STRIDE 4194303   /* elements from token to token of what the sliding-window kernels walk */
+#define UA_PAGED_MAX_TREE 256  /* most tokens of a sequence's tree */
 #define UA_NOALLOC_MAX_LINES 65532   /* most query tiles + key tiles of ua_tilelist_build_device_noalloc */
 
 /* Element types of the entry points that take more than bf16. */
@@ -70,8 +71,8 @@ extern "C" {
 
 /* 100 * major + minor.  102: `nnz` argument of the attention entry points, ua_merge_update, the
  * no-allocation builder, `work` of ua_tilelist_build_device grown to n_qtiles + n_ktiles + 7.  104: ua_bsa_bwd.
- * 105: ua_tilelist_build_device_scratch.  106: ua_copy_in.  107: ua_rope, ua_rope_append.  108: ua_swa_*.  109: ua_rows_*.  */
-#define UA_VERSION 109
+ * 105: ua_tilelist_build_device_scratch.  106: ua_copy_in.  107: ua_rope, ua_rope_append.  108: ua_swa_*.  109: ua_rows_*.  110: ua_paged_*.  */
+#define UA_VERSION 110
 int ua_version(void);
 const char *ua_strerror(int rc);
 
@@ -411,6 +412,48 @@ int ua_rows_sum(const void *const *parts, int n_parts, int parts_fp32, void *out
 int ua_rows_delta(const void *o, const void *dout, float *delta,
                   int batch, int seqlen_q, int n_heads, int head_dim, int dtype,
                   const int64_t *o_strides, const int64_t *do_strides, void *stream);
+
+/* ---- a paged cache --------------------------------------------------------------------------------------
+ * No counterpart in the reference.  Pools k_pages, v_pages [n_pages, page, n_kv_heads, head_dim], any page size, with (page, slot, head) element strides;
+ * table DEVICE int32 [batch, max_pages], rows table_stride apart: row r of sequence b is slot r % page of page table[b, r / page].  An entry outside
+ * [0, n_pages) is a page that is not there: nothing is written to it, and its rows are not seen; entries behind the last row are not used.  Sequences
+ * may share pages that none of them writes.  A contiguous cache [batch, room, ...] is one of batch pages of `room` rows.
+ * A call brings n_tokens tokens of every sequence, n_new[b] (DEVICE int32; NULL: all) of them real; lens[b] (DEVICE int32) is the length WITH the real ones,
+ * base = lens[b] - n_new[b], and token t's row is base + t.  The tokens are a chain, or a tree with parents (DEVICE int32 [batch, n_tokens], rows
+ * parents_stride apart, 0: one tree for all; n_tokens <= UA_PAGED_MAX_TREE): parents[b, t] is the token before token t, and any value but 0 .. t - 1 says
+ * that row base - 1 is.  A token's position is base plus the number of tokens before it in its branch (in a chain, its row).  Lengths count up to
+ * 2^29, below 0 they are 0.  Nothing here depends on lens, n_new, parents or table on the host: a captured call serves all of them. */
+
+/* The new tokens' Q turned into q_out (q_out may be q), K, turned, and V written to their rows; turns, types and widths as in ua_rope.  Rows outside the table
+ * or on a page that is not there are not written.  Of tokens that are not real K and V are not written and q_out is 0. */
+int ua_paged_append(const void *q, const void *k, const void *v, void *q_out, void *k_pages, void *v_pages, const double *freqs,
+                    const int32_t *table, const int32_t *lens, const int32_t *n_new, const int32_t *parents,
+                    int batch, int n_tokens, int n_heads, int n_kv_heads, int n_pages, int page, int max_pages, int head_dim, int rotary_dim,
+                    int dtype, int interleaved, float scale, int64_t table_stride, int64_t parents_stride,
+                    const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides, const int64_t *q_out_strides,
+                    const int64_t *k_page_strides, const int64_t *v_page_strides, void *stream);
+
+/* Their attention: q, o [batch, n_tokens, n_heads, head_dim], lse [batch, n_heads, n_tokens].  A token sees the rows before base and the tokens of its branch,
+ * itself among them; with left >= 0 of both only what is at most `left` positions before its own, and the first `sinks` positions.  Tokens that see nothing, and
+ * those that are not real, get o = 0, lse = -inf.  Types, alignment and strides (pools: non-negative multiples of 8 elements) and what may be NaN as in ua_swa_decode; of a
+ * tree's tokens NaN in a key or value may reach all of the sequence's new tokens.  o may be q itself.
+ * Long caches are cut into parts if `workspace` (16-byte aligned) holds ua_paged_decode_workspace_bytes(). */
+int64_t ua_paged_decode_workspace_bytes(int batch, int n_tokens, int n_heads, int n_kv_heads, int page, int max_pages, int head_dim, int64_t left, int64_t sinks);
+int ua_paged_decode(const void *q, const void *k_pages, const void *v_pages, void *o, float *lse,
+                    const int32_t *table, const int32_t *lens, const int32_t *n_new, const int32_t *parents,
+                    int batch, int n_tokens, int n_heads, int n_kv_heads, int n_pages, int page, int max_pages, int head_dim, int dtype,
+                    int64_t table_stride, int64_t parents_stride,
+                    const int64_t *q_strides, const int64_t *k_page_strides, const int64_t *v_page_strides, const int64_t *o_strides,
+                    int64_t left, int64_t sinks, float softmax_scale, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* After a tree's verification: row base + i takes what row base + path[b, i] holds, i < n_kept[b] (at most n_path), in place, for K and V of all `layers`, whose
+ * pools lie (layer, page, slot, head) strides apart under one table.  path DEVICE int32 [batch, n_path], rows path_stride apart, rising in each row as a branch's
+ * tokens are; entries below i or not of a real token, and rows on pages that are not there, leave row base + i as it is.  The caller then sets lens to base + n_kept.
+ * UA_BF16, UA_FP16 or UA_FP32, any head_dim and strides; 65535 layers and sequences at the most. */
+int ua_paged_keep(void *k_pages, void *v_pages, const int32_t *table, const int32_t *lens, const int32_t *n_new, const int32_t *path,
+                  const int32_t *n_kept, int layers, int batch, int n_tokens, int n_path, int n_kv_heads, int n_pages, int page, int max_pages,
+                  int head_dim, int dtype, int64_t table_stride, int64_t path_stride, const int64_t *k_page_strides, const int64_t *v_page_strides,
+                  void *stream);
 
 #ifdef __cplusplus
 }

@@ -16,6 +16,9 @@ def __getattr__(name):
     if name in ("rope_freqs", "rope_fwd", "rope_bwd", "rope_append"):
         from . import rope
         return getattr(rope, name)
+    if name in ("paged_append", "paged_decode", "paged_keep"):
+        from . import paged
+        return getattr(paged, name)
     if name in ("BlockSparseExecutor", "mask_from_comp_kernels", "comp_kernels_from_schedule"):
         from . import executor
         return getattr(executor, name)

@@ -51,6 +51,10 @@ SIGNATURES = {
     "ua_rows_update": (c_int, [c_void_p] * 6 + [c_int] * 8 + [_i64p] * 6 + [c_void_p]),
     "ua_rows_sum": (c_int, [POINTER(c_void_p), c_int, c_int, c_void_p] + [c_int] * 5 + [_i64p, c_float, c_void_p]),
     "ua_rows_delta": (c_int, [c_void_p] * 3 + [c_int] * 5 + [_i64p] * 2 + [c_void_p]),
+    "ua_paged_append": (c_int, [c_void_p] * 11 + [c_int] * 11 + [c_float] + [c_int64] * 2 + [_i64p] * 6 + [c_void_p]),
+    "ua_paged_decode_workspace_bytes": (c_int64, [c_int] * 7 + [c_int64] * 2),
+    "ua_paged_decode": (c_int, [c_void_p] * 9 + [c_int] * 9 + [c_int64] * 2 + [_i64p] * 4 + [c_int64] * 2 + [c_float, c_void_p, c_int64, c_void_p]),
+    "ua_paged_keep": (c_int, [c_void_p] * 7 + [c_int] * 10 + [c_int64] * 2 + [_i64p] * 2 + [c_void_p]),
     "ua_copy_in": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }
 

@@ -11,7 +11,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libultraattn_hip.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 NATIVE_PATH = os.path.join(PKG_DIR, "_native.so")
-SOURCES = ["api.hip", "tilelist.hip", "merge.hip", "glue.hip", "reduce.hip", "fwd.hip", "bwd.hip", "rope.hip", "swa_fwd.hip", "swa_bwd.hip", "swa_decode.hip", "rows.hip"]
+SOURCES = ["api.hip", "tilelist.hip", "merge.hip", "glue.hip", "reduce.hip", "fwd.hip", "bwd.hip", "rope.hip", "swa_fwd.hip", "swa_bwd.hip", "swa_decode.hip", "rows.hip", "paged_decode.hip",
+           "paged_keep.hip"]
 # benchmark-only probes (register-only MFMA loop, streaming-mix ceiling): built beside bench.py,
 # never linked into the product library
 BENCH_SRC = os.path.join(os.path.dirname(PKG_DIR), "bench_probe.hip")

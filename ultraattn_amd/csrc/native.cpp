@@ -1130,6 +1130,199 @@ PyObject* swa_decode(PyObject* const* a) {
   return tuple_of(out, lse);
 }
 
+// ---- a paged cache ----------------------------------------------------------------------------------------------
+// int32 on the tensors' device, the last axis contiguous; `shape` without its rows is one line for all of them.
+struct Whole {
+  const int32_t* data = nullptr;
+  int64_t stride = 0;
+  at::Tensor t;
+};
+Whole whole_numbers(const char* name, PyObject* o, const at::Tensor& x, int64_t rows, int64_t columns, bool shared) {
+  Whole w;
+  w.t = tensor(o, name);
+  const at::Tensor& t = w.t;
+  if (t.scalar_type() != at::kInt || t.device() != x.device())
+    fail(PyExc_ValueError, std::string(name) + " must be an int32 tensor on the tensors' device");
+  const bool one = shared && t.dim() == 1;
+  if ((!one && t.dim() != 2) || (!one && t.size(0) != rows) || (columns >= 0 && t.size(t.dim() - 1) != columns))
+    fail(PyExc_ValueError, std::string(name) + " has shape " + shape_str(t.sizes()) + ", expected (" + std::to_string(rows) + ", " +
+                               (columns >= 0 ? std::to_string(columns) : std::string("*")) + ")" + (shared ? " or one line of it" : ""));
+  if (t.size(t.dim() - 1) > 1 && t.stride(t.dim() - 1) != 1) fail(PyExc_ValueError, std::string(name) + ": the last axis must be contiguous");
+  if (t.size(t.dim() - 1) > INT32_MAX) fail(PyExc_ValueError, std::string(name) + " is too long");
+  w.data = (const int32_t*)t.data_ptr();
+  w.stride = one || t.size(0) <= 1 ? 0 : t.stride(0);
+  return w;
+}
+// What the calls on a paged cache have in common.
+struct Paged {
+  const at::Tensor &k, &v;
+  Whole table, parents;
+  at::Tensor lens, n_new;
+  int axis;                                    // of the pages: 0, or 1 behind the layers
+  Paged(const at::Tensor& first, PyObject* k_, PyObject* v_, PyObject* table_, PyObject* lens_, PyObject* n_new_, int64_t batch, int axes)
+      : k(tensor(k_, "k_pages")), v(tensor(v_, "v_pages")), axis(axes - 4) {
+    for (const at::Tensor* t : {&k, &v}) {
+      const std::string name = t == &k ? "k_pages" : "v_pages";
+      if (!t->is_cuda()) fail(PyExc_ValueError, name + " must be a CUDA (HIP) tensor");
+      if (t->device() != first.device()) fail(PyExc_ValueError, name + " is on another device than the first tensor");
+      if (t->scalar_type() != first.scalar_type())
+        fail(PyExc_TypeError, name + " must be " + c10::toString(first.scalar_type()) + ", got " + c10::toString(t->scalar_type()));
+      if (t->dim() != axes) fail(PyExc_ValueError, name + " must be " + (axis ? "[layers, " : "[") + "n_pages, page, H, D], got " + shape_str(t->sizes()));
+      if (t->stride(axis + 3) != 1 && t->size(axis + 3) != 1) fail(PyExc_ValueError, name + ": head_dim axis must be contiguous");
+      for (int i = 0; i < axes; ++i)
+        if (t->size(i) > INT32_MAX) fail(PyExc_ValueError, name + " is too long: " + shape_str(t->sizes()));
+      if (t->size(axis + 1) < 1 || t->size(axis + 1) > (1 << 29)) fail(PyExc_ValueError, name + ": a page holds 1 to 2^29 rows");
+    }
+    check_shape("v_pages", v, k.sizes());
+    if (k.size(axis + 2) < 1 || k.size(axis + 3) < 1) fail(PyExc_ValueError, "k_pages has no heads");
+    table = whole_numbers("table", table_, first, batch, -1, false);
+    lens = counts("lens", lens_, first, batch);
+    if (n_new_ != Py_None) n_new = counts("n_new", n_new_, first, batch);
+  }
+  static at::Tensor counts(const char* name, PyObject* o, const at::Tensor& x, int64_t batch) {
+    const at::Tensor& l = tensor(o, name);
+    if (l.scalar_type() != at::kInt || l.dim() != 1 || l.size(0) != batch || !l.is_contiguous() || l.device() != x.device())
+      fail(PyExc_ValueError, std::string(name) + " must be a contiguous int32 vector of one number per sequence on the tensors' device");
+    return l;
+  }
+  void of_tree(PyObject* o, const at::Tensor& q) {
+    if (o == Py_None) return;
+    parents = whole_numbers("parents", o, q, q.size(0), q.size(1), true);
+    if (q.size(1) > UA_PAGED_MAX_TREE)
+      fail(PyExc_ValueError, "a tree has at most " + std::to_string(UA_PAGED_MAX_TREE) + " tokens, got " + std::to_string(q.size(1)));
+  }
+  int n_pages() const { return (int)k.size(axis); }
+  int page() const { return (int)k.size(axis + 1); }
+  int heads() const { return (int)k.size(axis + 2); }
+  int most() const { return (int)table.t.size(1); }
+  const int32_t* len_data() const { return (const int32_t*)lens.data_ptr(); }
+  const int32_t* new_data() const { return n_new.defined() ? (const int32_t*)n_new.data_ptr() : nullptr; }
+  void check_apart_from(const char* name, const at::Tensor& written, bool pools) const {
+    check_apart(name, written, {&table.t, &lens});
+    if (n_new.defined()) check_apart(name, written, {&n_new});
+    if (parents.data) check_apart(name, written, {&parents.t});
+    if (pools) check_apart(name, written, {&k, &v});
+  }
+  void check_pools_written() const {
+    check_written("k_pages", k);
+    check_written("v_pages", v);
+    check_apart("k_pages", k, {&v});
+    check_apart_from("k_pages", k, false);
+    check_apart_from("v_pages", v, false);
+  }
+};
+
+// paged_append(q, k, v, k_pages, v_pages, table, lens, freqs, n_new, parents, interleaved, scale, q_out) -> q_out
+PyObject* paged_append(PyObject* const* a) {
+  const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v");
+  const int dt = dtype_code("q", q, true);
+  check_rows4("q", q, q);
+  check_rows4("k", k, q);
+  check_rows4("v", v, q);
+  check_shape("k", k, {q.size(0), q.size(1), k.size(2), q.size(3)});
+  check_shape("v", v, k.sizes());
+  Paged c(q, a[3], a[4], a[5], a[6], a[8], q.size(0), 4);
+  check_shape("k_pages", c.k, {c.k.size(0), c.k.size(1), k.size(2), k.size(3)});
+  c.of_tree(a[9], q);
+  const at::Tensor& fr = tensor(a[7], "freqs");
+  int64_t rotary;
+  const double* f = frequencies(fr, q, rotary);
+  const bool interleaved = truth(a[10]);
+  const float scale = positive(a[11], "scale");
+  Slot qo(a[12]);
+  result(qo, "q_out", q);
+  if (qo.given) {
+    check_apart("q_out", qo.t, {&k, &v, &fr});
+    c.check_apart_from("q_out", qo.t, true);
+    check_in_place("q_out", qo.t, q);
+  }
+  c.check_pools_written();
+  for (const at::Tensor* t : {&c.k, &c.v}) check_apart(t == &c.k ? "k_pages" : "v_pages", *t, {&q, &k, &v, &fr});
+  const On on(q);
+  init_device(on.device);
+  call("ua_paged_append", [&] {
+    return ua_paged_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), qo.t.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), f, c.table.data, c.len_data(),
+                           c.new_data(), c.parents.data, (int)q.size(0), (int)q.size(1), (int)q.size(2), c.heads(), c.n_pages(), c.page(), c.most(),
+                           (int)q.size(3), (int)rotary, dt, interleaved, scale, c.table.stride, c.parents.stride, Strides(q), Strides(k), Strides(v),
+                           Strides(qo.t), Strides(c.k), Strides(c.v), on.stream);
+  });
+  return qo.wrap();
+}
+
+// paged_decode(q, k_pages, v_pages, table, lens, n_new, parents, window, sinks, softmax_scale, out, lse) -> (out, lse)
+PyObject* paged_decode(PyObject* const* a) {
+  const at::Tensor& q = tensor(a[0], "q");
+  const int dt = dtype_code("q", q, false);
+  check_rows4("q", q, q);
+  if (q.size(3) != 64 && q.size(3) != 128) fail(PyExc_ValueError, "head_dim must be 64 or 128, got " + std::to_string(q.size(3)));
+  Paged c(q, a[1], a[2], a[3], a[4], a[5], q.size(0), 4);
+  check_shape("k_pages", c.k, {c.k.size(0), c.k.size(1), c.k.size(2), q.size(3)});
+  if (q.size(2) < 1 || q.size(2) % c.heads())
+    fail(PyExc_ValueError, std::to_string(q.size(2)) + " query heads cannot share " + std::to_string(c.heads()) + " key heads evenly");
+  c.of_tree(a[6], q);
+  const int64_t left = integer(a[7]), sinks = integer(a[8]);
+  if (left < -1) fail(PyExc_ValueError, "window must be -1 (no bound) or a number of keys");
+  if (sinks < 0) fail(PyExc_ValueError, "sinks must be a number of keys");
+  const float scale = swa_scale(a[9], q.size(3));
+  Slot out(a[10]), lse(a[11]);
+  result(out, "out", q);
+  if (lse.given) check_lse("lse", lse.t = tensor(lse.given, "lse"), q);
+  else lse.t = stat_of(q);
+  if (out.given) {
+    c.check_apart_from("out", out.t, true);
+    check_in_place("out", out.t, q);
+  }
+  if (lse.given) {
+    check_apart("lse", lse.t, {&q, &out.t});
+    c.check_apart_from("lse", lse.t, true);
+  }
+  const On on(q);
+  init_device(on.device);
+  const int B = (int)q.size(0), T = (int)q.size(1), H = (int)q.size(2), D = (int)q.size(3);
+  const at::Tensor ws = scratch(ua_paged_decode_workspace_bytes(B, T, H, c.heads(), c.page(), c.most(), D, left, sinks), q);
+  call("ua_paged_decode", [&] {
+    return ua_paged_decode(q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), out.t.data_ptr(), (float*)lse.t.data_ptr(), c.table.data, c.len_data(), c.new_data(),
+                           c.parents.data, B, T, H, c.heads(), c.n_pages(), c.page(), c.most(), D, dt, c.table.stride, c.parents.stride, used_strides(q),
+                           used_strides(c.k), used_strides(c.v), used_strides(out.t), left, sinks, scale, ws.defined() ? ws.data_ptr() : nullptr,
+                           ws.defined() ? ws.numel() : 0, on.stream);
+  });
+  return tuple_of(out, lse);
+}
+
+// paged_keep(k_pages, v_pages, table, lens, n_new, path, n_kept); n_new: a vector, or one number for all sequences
+PyObject* paged_keep(PyObject* const* a) {
+  const at::Tensor &k = tensor(a[0], "k_pages"), &lens = tensor(a[3], "lens");
+  const int dt = dtype_code("k_pages", k, true);
+  if (lens.dim() != 1) fail(PyExc_ValueError, "lens must be a contiguous int32 vector of one number per sequence on the tensors' device");
+  constexpr int64_t kMost = int64_t(1) << 28;
+  const bool same = PyLong_Check(a[4]);
+  const int64_t batch = lens.size(0), n_tokens = same ? integer(a[4]) : kMost;
+  if (n_tokens < 0 || n_tokens > kMost) fail(PyExc_ValueError, "n_new must be numbers of tokens");
+  if (a[4] == Py_None) fail(PyExc_ValueError, "n_new must be given: a vector or one number of tokens");
+  const Paged c(k, a[0], a[1], a[2], a[3], same ? Py_None : a[4], batch, k.dim() == 5 ? 5 : 4);
+  const Whole path = whole_numbers("path", a[5], k, batch, -1, false);
+  const at::Tensor kept = Paged::counts("n_kept", a[6], k, batch);
+  c.check_pools_written();
+  for (const at::Tensor* t : {&c.k, &c.v}) check_apart(t == &c.k ? "k_pages" : "v_pages", *t, {&path.t, &kept});
+  const int layers = c.axis ? (int)k.size(0) : 1;
+  if (layers > 65535 || batch > 65535) fail(PyExc_ValueError, "at most 65535 layers and sequences");
+  struct Strides4 {
+    int64_t s[4];
+    Strides4(const at::Tensor& t, int axis) : s{} {
+      for (int i = 0; i < 4; ++i)
+        if (i + axis >= 1 && t.size(i + axis - 1) > 1) s[i] = t.stride(i + axis - 1);
+    }
+  } const ks(c.k, c.axis), vs(c.v, c.axis);
+  const On on(k);
+  init_device(on.device);
+  call("ua_paged_keep", [&] {
+    return ua_paged_keep(c.k.data_ptr(), c.v.data_ptr(), c.table.data, c.len_data(), c.new_data(), path.data, (const int32_t*)kept.data_ptr(), layers,
+                         (int)batch, (int)n_tokens, (int)path.t.size(1), c.heads(), c.n_pages(), c.page(), c.most(), (int)k.size(c.axis + 3), dt, c.table.stride,
+                         path.stride, ks.s, vs.s, on.stream);
+  });
+  Py_RETURN_NONE;
+}
+
 // ---- module ---------------------------------------------------------------------------------------------
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -1156,6 +1349,7 @@ PyMethodDef methods[] = {
     UA_METHOD(delta, 3), UA_METHOD(grad_accumulate, 4), UA_METHOD(merge, 4), UA_METHOD(grad_sum, 3),
     UA_METHOD(merge_update, 5), UA_METHOD(permute_cols, 6), UA_METHOD(lists_from_mask, 5),
     UA_METHOD(build_lists_device, 3), UA_METHOD(rope, 10), UA_METHOD(rope_append, 10), UA_METHOD(swa_forward, 11), UA_METHOD(swa_backward, 16), UA_METHOD(swa_decode, 9),
+    UA_METHOD(paged_append, 13), UA_METHOD(paged_decode, 12), UA_METHOD(paged_keep, 7),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "Native host side of the attention operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,748 @@
+// Attention of the new tokens of every sequence, a chain or a tree, against a paged cache that holds them already.
+//
+// The rows of a key head are the new tokens of each of the query heads that share it, row = token * group + head of the group.  Two kernels:
+//   few rows (up to 32 of a key head): as against a contiguous cache, four waves of a workgroup go through blocks of 32 keys of their own, rows are the columns
+//     of 16x16x32 products, and the waves' rows are merged at the end.  Bound: HBM, the visible keys and values once.
+//   many rows: tiles of 128, 32 a wave, go through blocks of 64 keys together, as in the sliding-window forward (32x32x16 products, two LDS stages).  Bound: the
+//     products, or HBM where the tiles are few.
+// The keys of long caches are cut into parts, workgroups of their own, that leave fp32 rows for a merge.
+//
+// Pages: a lane's copy names its own address, so a block's keys may lie on any pages and start anywhere.  The table's entries come into LDS two blocks ahead, by
+// the same asynchronous copies; one lane a key turns them into addresses of its key and its value, which the copies' lanes take from LDS.  Keys
+// that nothing in the workgroup sees (behind the last, on a page that is not there) are read from a row of zeros.
+//
+// What a row sees of 32 keys is one word: up to its own position, from its window's first key on or among the sinks, on pages that are there, and of
+// the new tokens those of its branch.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+#include "paged.h"
+#include "swa.h"
+
+namespace ua {
+
+constexpr int kPagedWaves = 4, kPagedMaxParts = 64;
+__device__ __attribute__((aligned(256))) const uint32_t kZeroRow[64] = {};
+
+// P is held times 2^bits of the largest score's (as in the other kernels of these types).
+template <class T> constexpr float kFewBits = 0.f;
+template <> constexpr float kFewBits<fp16> = 14.f;
+template <class T> struct ManyRaise;
+template <> struct ManyRaise<bf16> { static constexpr float kSum = 16777216.f, kBits = 0.f; };
+template <> struct ManyRaise<fp16> { static constexpr float kSum = 32768.f, kBits = 7.f; };
+
+struct PagedRows { const char* rows; int64_t page, slot, head; };       // strides in bytes
+struct PagedParams {
+  const void* q;
+  PagedRows k, v;
+  void* o;
+  float* lse;
+  PagedSteps steps;
+  PagedTable pages;
+  Strides3 qs, os;
+  int n_heads, n_kv_heads, group, left, sinks, rows, n_tiles, n_parts, least;       // left: kFar = no bound; rows: of a key head; least: blocks of a part
+  float scale_log2;
+  float *part_o, *part_lse;
+  int64_t o_part, lse_part;
+  Div by_kv_heads, by_group, by_tiles, by_parts;
+  BlockMap map;
+};
+
+// A lane's 16 bytes (4 bytes) from its own address into LDS, lane l at +16 l (+4 l) of the wave-uniform `lds`; see dma16_abs.
+__device__ __forceinline__ void dma16_at(uint64_t from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(from) : "m0");
+}
+__device__ __forceinline__ void dma4_at(uint64_t from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" :: "s"(lds), "v"(from) : "m0");
+}
+
+// Blocks of kKeys keys that a tile's tokens t0 .. t1 see: the sinks before the window, then the window's first key on.
+template <int kKeys>
+struct PagedWalk {
+  int n_sink, n, start, sinks_end, last;              // keys that a row sees: before sinks_end, and start .. last
+  __device__ __forceinline__ PagedWalk(const PagedParams& p, const StepOf& of, int t0, int t1) {
+    const bool any = t0 < of.n;
+    last = any ? min(of.base + min(t1, of.n - 1), p.pages.room - 1) : -1;
+    start = max(of.base + (p.steps.parents ? 0 : t0) - p.left, 0);
+    sinks_end = max(min(min(p.sinks, start), last + 1), 0);
+    n_sink = (sinks_end + kKeys - 1) / kKeys;
+    n = n_sink + (last >= start ? (last - start) / kKeys + 1 : 0);
+  }
+  __device__ __forceinline__ int at(int i) const { return i < n_sink ? i * kKeys : start + (i - n_sink) * kKeys; }
+  __device__ __forceinline__ int end_of(int i) const { return i < n_sink ? sinks_end : last + 1; }
+};
+
+// How a wave gets at kRows keys of a block: lane l stands for key row_of(l % kRows), its K (l / kRows even) or its V.
+template <int kRows>
+struct PagedLane {
+  uint64_t base;
+  int64_t page, slot;
+  __device__ __forceinline__ PagedLane(const PagedParams& p, int hk, int lane) {
+    const bool second = (lane / kRows) & 1;
+    base = reinterpret_cast<uint64_t>(second ? p.v.rows + hk * p.v.head : p.k.rows + hk * p.k.head);
+    page = second ? p.v.page : p.k.page;
+    slot = second ? p.v.slot : p.k.slot;
+  }
+  // The key's entry on its way into LDS (of keys behind the last: the last one's).
+  static __device__ __forceinline__ void fetch(const PagedParams& p, const int32_t* line, int key, int last, uint32_t lds) {
+    dma4_at(reinterpret_cast<uint64_t>(line + quotient(min(max(key, 0), last), p.pages.by_page)), lds);
+  }
+  // The key's address, or zeros', from its entry; whether it is there.
+  __device__ __forceinline__ uint64_t address(const PagedParams& p, int key, int end, int entry, bool& there) const {
+    const int k = min(key, end - 1), i = quotient(max(k, 0), p.pages.by_page), in_page = k - i * p.pages.page;
+    there = key < end && (uint32_t)entry < (uint32_t)p.pages.n_pages;
+    return there ? base + (uint64_t)((int64_t)entry * page) + (uint64_t)((int64_t)in_page * slot) : reinterpret_cast<uint64_t>(kZeroRow);
+  }
+};
+
+// The branches of a sequence's tokens: bit j of a token's 256 is set if it is token j or comes behind it.  Words 1 .. 8 of a token's line hold them, word 0
+// stands for the cache's rows before (all seen); word 9, which is shifted in behind the last bit, no row gets to.
+constexpr int kDepth = 9, kBefore = 10, kBranchPitch = 11;       // (words; odd, so that 32 tokens' lines meet 32 banks)
+struct Branches { uint32_t line[kTreeMost * kBranchPitch]; };
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+// By a workgroup of kTreeThreads: distances double, as in tree_depths.  A window cuts what is further behind and not among the sinks.
+__device__ __forceinline__ void tree_branches(const PagedParams& p, const StepOf& of, int b, Branches& out) {
+  constexpr int kWords = kTreeMost / 32;
+  const int t = threadIdx.x, words = (p.steps.n_tokens + 31) / 32;
+  uint32_t mine[kWords];
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) mine[w] = t >> 5 == w ? 1u << (t & 31) : 0u;
+  uint32_t* const line = out.line + t * kBranchPitch;
+  line[0] = ~0u;
+  int parent = parent_of(p.steps, b, t);
+  while (true) {
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) line[1 + w] = mine[w];
+    line[kBefore] = parent;
+    if (!__syncthreads_or(parent >= 0)) break;
+    if (parent >= 0) {
+      const uint32_t* const theirs = out.line + parent * kBranchPitch;
+#pragma unroll
+      for (int w = 0; w < kWords; ++w)
+        if (w < words) mine[w] |= theirs[1 + w];
+      parent = (int)theirs[kBefore];
+    }
+    __syncthreads();
+  }
+  int depth = -1;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) depth += __popc(mine[w]);
+  line[kDepth] = depth;
+  __syncthreads();
+  if (p.left < p.steps.n_tokens) {
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      for (uint32_t rest = mine[w]; rest; rest &= rest - 1) {
+        const int theirs = (int)out.line[(32 * w + __ffs(rest) - 1) * kBranchPitch + kDepth];
+        if (depth - theirs > p.left && of.base + theirs >= p.sinks) mine[w] &= ~(rest & -rest);
+      }
+      line[1 + w] = mine[w];
+    }
+    __syncthreads();
+  }
+}
+
+// What a row sees.
+struct RowSees {
+  int hi, lo, sinks, base;                              // keys lo .. hi and those before `sinks`, up to hi
+  const uint32_t* bits;                                 // its token's branch
+  template <bool kTree>
+  __device__ __forceinline__ void of(const PagedParams& p, const StepOf& step, int token, const Branches& branches) {
+    const bool real = token < step.n;
+    const int pos = step.base + (kTree ? (int)branches.line[token * kBranchPitch + kDepth] : token);
+    hi = real ? min(step.base + token, p.pages.room - 1) : -1;
+    lo = kTree ? min(pos - p.left, step.base) : pos - p.left;
+    sinks = p.sinks;
+    base = step.base;
+    bits = branches.line + token * kBranchPitch;
+  }
+  // of keys key .. key + 31
+  template <bool kTree>
+  __device__ __forceinline__ uint32_t word(int key) const {
+    uint32_t w = below(hi + 1 - key) & (~below(lo - key) | below(sinks - key));
+    if (kTree) {
+      const int s = min(max(key - base, -32), 255), i = (s >> 5) + 1;
+      w &= __builtin_amdgcn_alignbit(bits[i + 1], bits[i], s & 31);
+    }
+    return w;
+  }
+};
+
+template <int kD>
+struct FewHead {
+  static constexpr int kKeys = 32, kRow = 2 * kD, kChunks = kD / 8, kCopyRows = 1024 / kRow, kUnits = kKeys / kCopyRows, kTile = kUnits * 1024;
+  static constexpr int kStage = 2 * kTile, kWave = 2 * kStage, kSteps = kD / 32, kBlocks = kD / 16;
+  static constexpr int kEntries = 256, kTable = 2 * kEntries + 512;       // of a wave: two blocks' entries, a block's addresses
+  // K: 16 rows are read at one chunk.  V is read transposed: 8 rows at two chunks that start at a multiple of two.
+  static __device__ __forceinline__ int slot_k(int r, int c) { return kD == 128 ? c ^ (r & 15) : c ^ (r >> 1 & 7); }
+  static __device__ __forceinline__ int slot_v(int r, int c) { return kD == 128 ? c ^ ((r & 3) << 2) ^ ((r >> 2 & 1) << 1) : c ^ ((r >> 1 & 3) << 1); }
+};
+struct NoBranches { uint32_t line[1]; };
+
+template <class T, int kD, int kTiles, bool kTree>
+__global__ __launch_bounds__(64 * kPagedWaves) void paged_few_kernel(const PagedParams p) {
+  using H = FewHead<kD>;
+  using V = SwaVec<T>;
+  typedef typename V::x8 x8;
+  constexpr int kRows = 16 * kTiles, kOutPitch = 4 * kD + 16;             // (bytes of a row of fp32 at the merge)
+  static_assert(kRows * kOutPitch + 8 * kRows <= H::kWave, "a wave's rows and statistics fit its stages");
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[kPagedWaves * H::kWave];
+  __shared__ __attribute__((aligned(256))) unsigned char tables[kPagedWaves * H::kTable];
+  __shared__ std::conditional_t<kTree, Branches, NoBranches> branch_store;
+  Branches& branches = reinterpret_cast<Branches&>(branch_store);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
+  const int rest = quotient(blockIdx.x, p.by_parts), part = blockIdx.x - rest * p.n_parts;
+  const int bh = quotient(rest, p.by_tiles), tile = rest - bh * p.n_tiles, b = quotient(bh, p.by_kv_heads), hk = bh - b * p.n_kv_heads;
+  const StepOf step = step_of(p.steps, b);
+  const int row0 = tile * kRows, row1 = min(row0 + kRows, p.rows) - 1;
+  const PagedWalk<H::kKeys> walk(p, step, quotient(row0, p.by_group), quotient(row1, p.by_group));
+  const int part_len = max((walk.n + p.n_parts - 1) / p.n_parts, p.least), i0 = min(part * part_len, walk.n), i1 = min(i0 + part_len, walk.n);
+
+  const int32_t* const line = p.pages.table + b * p.pages.stride;
+  const PagedLane<32> from(p, hk, lane);
+  const uint32_t mine = lds0 + wave * H::kWave, entries = (uint32_t)(uintptr_t)(lds_byte*)tables + wave * H::kTable, places = entries + 2 * H::kEntries;
+  const int key_row = lane & 31, copy_row = lane / H::kChunks, chunk = lane % H::kChunks;
+  auto fetch = [&](int i, uint32_t to) { from.fetch(p, line, walk.at(i) + key_row, walk.last, to); };
+  // The block's addresses into LDS; which of its keys are there.
+  auto locate = [&](int i, uint32_t entry_at) {
+    bool there;
+    const uint64_t a = from.address(p, walk.at(i) + key_row, i < i1 ? walk.end_of(i) : 0, lds_get<int>(entry_at + 4 * lane), there);
+    lds_put(places + 8 * lane, a);
+    return (uint32_t)__builtin_amdgcn_ballot_w64(there);
+  };
+  auto copy_in = [&](uint32_t stage) {
+#pragma unroll
+    for (int u = 0; u < H::kUnits; ++u) {
+      const int r = H::kCopyRows * u + copy_row;
+      dma16_at(lds_get<uint64_t>(places + 8 * r) + 16 * H::slot_k(r, chunk), stage + 1024 * u);
+      dma16_at(lds_get<uint64_t>(places + 256 + 8 * r) + 16 * H::slot_v(r, chunk), stage + H::kTile + 1024 * u);
+    }
+  };
+  int i = i0 + wave;
+  uint32_t there = 0, there_next = 0;
+  if (i < i1) {
+    fetch(i, entries);
+    fetch(i + kPagedWaves, entries + H::kEntries);
+    wait_vmem_all();
+    there = locate(i, entries);
+    copy_in(mine);
+    there_next = locate(i + kPagedWaves, entries + H::kEntries);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    fetch(i + 2 * kPagedWaves, entries);
+    copy_in(mine + H::kStage);
+  }
+  if (kTree && i0 < i1) tree_branches(p, step, b, branches);
+
+  // Q as B operands: row col of the tile, columns 32 s + 8 quad ..
+  x8 qf[kTiles][H::kSteps];
+  RowSees sees[kTiles];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    const int row = min(row0 + 16 * t + col, p.rows - 1), token = quotient(row, p.by_group), h = hk * p.group + row - token * p.group;
+    const T* q = (const T*)p.q + b * p.qs.b + token * p.qs.s + h * p.qs.h + 8 * quad;
+#pragma unroll
+    for (int s = 0; s < H::kSteps; ++s) qf[t][s] = *reinterpret_cast<const x8*>(q + 32 * s);
+    sees[t].template of<kTree>(p, step, token, branches);
+  }
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int s = 0; s < H::kSteps; ++s) asm volatile("" : "+v"(qf[t][s]));     // arrived before the walk counts its copies
+  f32x4 o[kTiles][H::kBlocks];
+  float m_run[kTiles], m_use[kTiles], l_run[kTiles];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    m_run[t] = -INFINITY;
+    m_use[t] = l_run[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < H::kBlocks; ++d) o[t][d] = f32x4{0};
+  }
+  uint32_t stage = mine, other = mine + H::kStage, entry_now = entries, entry_next = entries + H::kEntries;
+  constexpr int kCopies = 2 * H::kUnits;
+  for (; i < i1; i += kPagedWaves) {
+    // (in flight: this block, the entries two blocks on, the next block)
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kCopies) : "memory");
+    const uint32_t there_after = locate(i + 2 * kPagedWaves, entry_now);
+    const int key0 = walk.at(i);
+    x8 kf[2][H::kSteps];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int s = 0; s < H::kSteps; ++s) {
+        const int r = 16 * n + col;
+        kf[n][s] = lds_get<x8>(stage + r * H::kRow + (H::slot_k(r, 4 * s + quad) << 4));
+      }
+    x8 vf[H::kBlocks];
+#pragma unroll
+    for (int d = 0; d < H::kBlocks; ++d) {
+      const int r = 4 * quad + (col >> 2), c = 2 * d + ((col & 3) >> 1);
+      const uint32_t at = stage + H::kTile + r * H::kRow + (H::slot_v(r, c) << 4) + (col & 1) * 8;        // (row + 16: the same slot)
+      vf[d] = lds_tr_pair<T>(at, at + 16 * H::kRow);
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      f32x4 s[2] = {f32x4{0}, f32x4{0}};
+#pragma unroll
+      for (int k = 0; k < H::kSteps; ++k)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) s[n] = V::mfma16(kf[n][k], qf[t][k], s[n]);
+      const uint32_t seen = (sees[t].template word<kTree>(key0) & there) >> (4 * quad);
+      float mx = -INFINITY, a, c;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (!(seen >> (16 * n + j) & 1)) s[n][j] = -INFINITY;
+          mx = fmaxf(mx, s[n][j]);
+        }
+      swap_lanes<16>(mx, a, c);
+      swap_lanes<32>(fmaxf(a, c), a, c);
+      mx = fmaxf(a, c) * p.scale_log2;
+      if (__builtin_amdgcn_ballot_w64(mx > m_run[t]) != 0) {
+        const float m_new = fmaxf(m_run[t], mx);
+        m_use[t] = m_new == -INFINITY ? 0.f : m_new - kFewBits<T>;
+        const float alpha = m_new == m_run[t] ? 1.f : fast_exp2(m_run[t] - m_new);
+        m_run[t] = m_new;
+        l_run[t] *= alpha;
+#pragma unroll
+        for (int d = 0; d < H::kBlocks; ++d) o[t][d] *= alpha;
+      }
+      x8 pf;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float e = fast_exp2(fmaf(s[n][j], p.scale_log2, -m_use[t]));
+          l_run[t] += e;
+          pf[4 * n + j] = (T)e;
+        }
+#pragma unroll
+      for (int d = 0; d < H::kBlocks; ++d) o[t][d] = V::mfma16(vf[d], pf, o[t][d]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // everything of this stage is in registers
+    fetch(i + 3 * kPagedWaves, entry_next);
+    copy_in(stage);
+    there = there_next;
+    there_next = there_after;
+    const uint32_t x = stage, y = entry_now;
+    stage = other;
+    other = x;
+    entry_now = entry_next;
+    entry_next = y;
+  }
+  wait_vmem_all();
+  // ---- the waves' rows: O as fp32, then the reference and the sum of each
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    float a, c;
+    swap_lanes<16>(l_run[t], a, c);
+    swap_lanes<32>(a + c, a, c);
+#pragma unroll
+    for (int d = 0; d < H::kBlocks; ++d) lds_put(mine + (16 * t + col) * kOutPitch + (16 * d + 4 * quad) * 4, o[t][d]);
+    if (quad == 0) {
+      lds_put(mine + kRows * kOutPitch + 8 * (16 * t + col), m_run[t]);
+      lds_put(mine + kRows * kOutPitch + 8 * (16 * t + col) + 4, a + c);
+    }
+  }
+  __syncthreads();
+  constexpr int kPer = kD / 16;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    const int r = 16 * t + (threadIdx.x >> 4), c = threadIdx.x & 15, row = row0 + r;
+    if (row >= p.rows) continue;
+    float m = -INFINITY, l = 0.f, acc[kPer] = {};
+#pragma unroll
+    for (int w = 0; w < kPagedWaves; ++w) m = fmaxf(m, lds_get<float>(lds0 + w * H::kWave + kRows * kOutPitch + 8 * r));
+    const float at = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < kPagedWaves; ++w) {
+      const uint32_t rows = lds0 + w * H::kWave;
+      const float f = fast_exp2(lds_get<float>(rows + kRows * kOutPitch + 8 * r) - at);
+      l += f * lds_get<float>(rows + kRows * kOutPitch + 8 * r + 4);
+#pragma unroll
+      for (int j = 0; j < kPer; j += 4) {
+        const f32x4 x = lds_get<f32x4>(rows + r * kOutPitch + (c * kPer + j) * 4);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[j + n] += f * x[n];
+      }
+    }
+    const bool any = l > 0.f || l != l;                                  // (NaN stays)
+    const float inv = any ? 1.f / l : 0.f, lse = any ? (m - kFewBits<T> + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+    const int token = quotient(row, p.by_group), h = hk * p.group + row - token * p.group;
+    const int64_t out_row = ((int64_t)b * p.n_heads + h) * p.steps.n_tokens + token;
+    if (p.n_parts > 1) {
+      if (c == 0) p.part_lse[part * p.lse_part + out_row] = lse;
+      if (any) {
+        float* to = p.part_o + part * p.o_part + out_row * kD + c * kPer;
+#pragma unroll
+        for (int j = 0; j < kPer; j += 4) *reinterpret_cast<f32x4*>(to + j) = f32x4{acc[j] * inv, acc[j + 1] * inv, acc[j + 2] * inv, acc[j + 3] * inv};
+      }
+    } else {
+      typedef __attribute__((ext_vector_type(kPer))) T vec;
+      vec w;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) w[j] = any ? (T)(acc[j] * inv) : (T)0.f;
+      *reinterpret_cast<vec*>((T*)p.o + b * p.os.b + token * p.os.s + h * p.os.h + c * kPer) = w;
+      if (c == 0) p.lse[out_row] = lse;
+    }
+  }
+}
+
+// ---- many rows ------------------------------------------------------------------------------------------------------------
+// Row of a tile's wave (of 32) -> token, query head.
+struct RowPlace { int token, head; };
+__device__ __forceinline__ RowPlace row_place(const PagedParams& p, int hk, int row) {
+  const int token = quotient(row, p.by_group);
+  return {token, hk * p.group + row - token * p.group};
+}
+
+template <class T, int kD, bool kTree>
+__global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p) {
+  using H = SwaHead<kD>;
+  using V = SwaVec<T>;
+  typedef typename V::x8 x8;
+  constexpr int kPieces = 2 * H::kCopies, kSecond = H::kTile, kMine = kSwaBlock / kPagedWaves;        // kMine: keys of a block that a wave copies
+  static_assert(kMine == 16 && H::kCopies * H::kCopyRows == kMine, "a wave's keys");
+  __shared__ __attribute__((aligned(1024))) unsigned char stage_a[2 * H::kTile];
+  __shared__ __attribute__((aligned(1024))) unsigned char stage_b[2 * H::kTile];
+  __shared__ __attribute__((aligned(256))) unsigned char tables[kPagedWaves * 768];                   // of a wave: two blocks' entries, a block's addresses
+  __shared__ std::conditional_t<kTree, Branches, NoBranches> branch_store;
+  Branches& branches = reinterpret_cast<Branches&>(branch_store);
+  const uint32_t lds[2] = {(uint32_t)(uintptr_t)(lds_byte*)stage_a, (uint32_t)(uintptr_t)(lds_byte*)stage_b};
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int pos, bh;
+  map_block(blockIdx.x, p.map, pos, bh);
+  const int part = quotient(pos, p.by_tiles), tile = pos - part * p.n_tiles;       // (tiles that read the same keys beside each other)
+  const int b = quotient(bh, p.by_kv_heads), hk = bh - b * p.n_kv_heads;
+  const StepOf step = step_of(p.steps, b);
+  const int r0 = tile * kSwaRows, row0 = r0 + 32 * wave, n_rows = p.rows - row0;      // rows of this wave that exist (may be <= 0)
+  const PagedWalk<kSwaBlock> walk(p, step, quotient(r0, p.by_group), quotient(min(r0 + kSwaRows, p.rows) - 1, p.by_group));
+  const int part_len = max((walk.n + p.n_parts - 1) / p.n_parts, p.least), i0 = min(part * part_len, walk.n), i1 = min(i0 + part_len, walk.n);
+
+  const int32_t* const line = p.pages.table + b * p.pages.stride;
+  const PagedLane<kMine> from(p, hk, lane);
+  const uint32_t entries = (uint32_t)(uintptr_t)(lds_byte*)tables + wave * 768, places = entries + 512;
+  const int m = lane & (kMine - 1), key_row = H::kCopyRows * (kPagedWaves * (m / H::kCopyRows) + wave) + m % H::kCopyRows;
+  const int copy_row = lane / H::kChunks, slot_row = H::kCopyRows * wave + copy_row, chunk = lane % H::kChunks;
+  const uint32_t k_chunk = 16 * H::slot_n(slot_row, chunk), v_chunk = 16 * H::slot_t(slot_row, chunk);
+  auto fetch = [&](int i, int parity) { from.fetch(p, line, walk.at(i) + lane, walk.last, entries + 256 * parity); };
+  uint64_t there = 0, there_next = 0;      // keys of this block and the next that are there
+  auto locate = [&](int i, int parity) {
+    bool is;
+    const int key0 = walk.at(i), end = i < i1 ? walk.end_of(i) : 0;
+    const uint64_t a = from.address(p, key0 + key_row, end, lds_get<int>(entries + 256 * parity + 4 * key_row), is);
+    if (lane < 2 * kMine) lds_put(places + 8 * lane, a);
+    there_next = __builtin_amdgcn_ballot_w64(key0 + lane < end && (uint32_t)lds_get<int>(entries + 256 * parity + 4 * lane) < (uint32_t)p.pages.n_pages);
+  };
+  auto place = [&](int n) { return lds_get<uint64_t>(places + 128 * (n & 1) + 8 * (H::kCopyRows * (n >> 1) + copy_row)) + (n & 1 ? v_chunk : k_chunk); };
+  auto copy = [&](int n, uint64_t a, uint32_t stage) {
+    dma16_at(a, stage + (n & 1 ? kSecond : 0) + (kPagedWaves * (n >> 1) + wave) * 1024);
+  };
+  if (i0 < i1) {
+    fetch(i0, 0);
+    fetch(i0 + 1, 1);
+    wait_vmem_all();
+    locate(i0, 0);
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) copy(n, place(n), lds[0]);
+  }
+  if (kTree && i0 < i1) tree_branches(p, step, b, branches);
+  x8 qf[H::kSteps];
+  {
+    u32x4 raw[H::kSteps];
+    const int l = fresh_lane(), c = l % H::kChunks;
+#pragma unroll
+    for (int i = 0; i < H::kSteps; ++i) {
+      const RowPlace r = row_place(p, hk, min(row0 + H::kCopyRows * i + l / H::kChunks, p.rows - 1));
+      raw[i] = *reinterpret_cast<const u32x4*>((const T*)p.q + b * p.qs.b + r.token * p.qs.s + r.head * p.qs.h + c * 8);
+    }
+    const uint32_t turn = lds[1] + wave * 32 * H::kRow;   // the stage that the first step fills
+    swa_put_rows<kD>(raw, turn);
+    swa_frags<T, kD>(qf, turn);
+#pragma unroll
+    for (int i = 0; i < H::kSteps; ++i) asm volatile("" : "+v"(qf[i]));      // read before the walk
+  }
+  RowSees sees;
+  const int token = quotient(min(row0 + (lane & 31), p.rows - 1), p.by_group);
+  sees.template of<kTree>(p, step, token, branches);
+  // Keys that every real row of the wave sees: from .. to - 1, and those before `sinks` up to there.
+  const int t_first = quotient(min(row0, p.rows - 1), p.by_group), t_last = min(quotient(min(row0 + 31, p.rows - 1), p.by_group), step.n - 1);
+  const int all_to = min(kTree ? step.base : step.base + t_first + 1, p.pages.room), all_from = step.base + (kTree ? step.n - 1 : t_last) - p.left;
+  const int some_to = t_first >= step.n ? 0 : kTree ? walk.last + 1 : step.base + t_last + 1, some_from = step.base + (kTree ? 0 : t_first) - p.left;
+  f32x16 o[H::kBlocks];
+#pragma unroll
+  for (int x = 0; x < H::kBlocks; ++x) o[x] = f32x16{0};
+  float m_run = -INFINITY, m_use = 0.f, l_run = 0.f;
+  uint32_t nat[H::kSteps], tr[H::kBlocks];
+#pragma unroll
+  for (int i = 0; i < H::kSteps; ++i) nat[i] = H::at_n(lane & 31, 2 * i + (lane >> 5));
+#pragma unroll
+  for (int x = 0; x < H::kBlocks; ++x) tr[x] = kSecond + H::tr_offset(lane, x);
+
+  auto walk_step = [&](int i, auto stage_tag) {
+    constexpr int kStage = decltype(stage_tag)::value;
+    const uint32_t here = lds[kStage], other = lds[kStage ^ 1];
+    const int key0 = walk.at(i);
+    wait_vmem_all();
+    __syncthreads();                        // this block and the next one's entries have landed, and everyone has left the other stage
+    there = there_next;
+    locate(i + 1, (i - i0 + 1) & 1);
+    fetch(i + 2, (i - i0) & 1);
+    uint64_t at[kPieces];
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) at[n] = place(n);
+    const bool hidden = n_rows <= 0 || key0 >= some_to || (key0 + kSwaBlock <= some_from && key0 >= p.sinks);
+    if (hidden) {
+#pragma unroll
+      for (int n = 0; n < kPieces; ++n) copy(n, at[n], other);
+      return;
+    }
+    // S^T: two blocks of 32 keys in turn
+    f32x16 s[2] = {f32x16{0}, f32x16{0}};
+    {
+      constexpr int kAhead = 4, kAll = 2 * H::kSteps;
+      x8 kf[kAll];
+      auto rd = [&](int n) { return lds_get<x8>(here + nat[n >> 1] + 32 * H::kRow * (n & 1)); };
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) kf[n] = rd(n);
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+      for (int n = 0; n < kAll; ++n) {
+        if (n + kAhead < kAll) kf[n + kAhead] = rd(n + kAhead);
+        s[n & 1] = V::mfma(kf[n], qf[n >> 1], s[n & 1]);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (n & 1) copy(n >> 1, at[n >> 1], other);
+      }
+      static_assert(kAll / 2 == kPieces, "a copy after every other product");
+    }
+    const bool whole = key0 + kSwaBlock <= all_to && (key0 >= all_from || key0 + kSwaBlock <= p.sinks) && there == ~0ull;
+    if (!whole) {
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) {
+        const uint32_t seen = (sees.template word<kTree>(key0 + 32 * mb) & (uint32_t)(there >> (32 * mb))) >> (4 * (lane >> 5));
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (!(seen >> (8 * (j >> 2) + (j & 3)) & 1)) s[mb][j] = -INFINITY;
+      }
+    }
+    constexpr int kVAhead = 3, kVAll = 4 * H::kBlocks;
+    x8 vf[4];
+    auto rd_v = [&](int n) {                // fragment n % kBlocks of 16 keys
+      const uint32_t a = here + tr[n % H::kBlocks] + 16 * H::kRow * (n / H::kBlocks);
+      return lds_tr_pair<T>(a, a + 8 * H::kRow);
+    };
+#pragma unroll
+    for (int n = 0; n < kVAhead; ++n) vf[n] = rd_v(n);
+    float rs = 0.f;
+    x8 pf[4];
+    auto exponentials = [&]() {
+      rs = 0.f;
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float e = fast_exp2(fmaf(s[mb][j], p.scale_log2, -m_use));
+          rs += e;
+          pf[2 * mb + (j >> 3)][j & 7] = (T)e;
+        }
+    };
+    exponentials();
+    if (__builtin_amdgcn_ballot_w64(!(rs < ManyRaise<T>::kSum) || m_run == -INFINITY) != 0) {        // wave-uniform, rare
+      float mx = s[0][0], a, c;
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[mb][j]);
+      swap_lanes<32>(mx, a, c);
+      const float m_new = fmaxf(m_run, fmaxf(a, c) * p.scale_log2);
+      m_use = m_new == -INFINITY ? 0.f : m_new - ManyRaise<T>::kBits;
+      const float alpha = m_new == m_run ? 1.f : fast_exp2(m_run - m_new);      // m_run = -inf -> 0
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int x = 0; x < H::kBlocks; ++x)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[x][j] *= alpha;
+      exponentials();
+    }
+    l_run += rs;
+#pragma unroll
+    for (int n = 0; n < kVAll; ++n) {
+      if (n + kVAhead < kVAll) vf[(n + kVAhead) & 3] = rd_v(n + kVAhead);
+      o[n % H::kBlocks] = V::mfma(vf[n & 3], pf[n / H::kBlocks], o[n % H::kBlocks]);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+  };
+  for (int i = i0; i < i1; i += 2) {
+    walk_step(i, std::integral_constant<int, 0>{});
+    if (i + 1 < i1) walk_step(i + 1, std::integral_constant<int, 1>{});
+  }
+  wait_vmem_all();                          // the last step's copies filled a stage with zeros
+  __syncthreads();
+  if (n_rows <= 0) return;
+  float a, c;
+  swap_lanes<32>(l_run, a, c);
+  const float l = a + c;
+  const bool any = (l > 0.f || l != l) && token < step.n;              // (NaN stays; a token that is none saw keys beside the others)
+  const float inv = any ? 1.f / l : 0.f, lse = any ? (m_use + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+#pragma unroll
+  for (int x = 0; x < H::kBlocks; ++x)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[x][j] = any ? o[x][j] : 0.f;
+  const int out_lane = fresh_lane(), my_row = row0 + (out_lane & 31);
+  const RowPlace mine = row_place(p, hk, min(my_row, p.rows - 1));
+  const int64_t out_row = ((int64_t)b * p.n_heads + mine.head) * p.steps.n_tokens + mine.token;
+  if (p.n_parts > 1) {
+    if (my_row < p.rows && any) {
+      float* to = p.part_o + part * p.o_part + out_row * kD + 4 * (out_lane >> 5);
+#pragma unroll
+      for (int x = 0; x < H::kBlocks; ++x)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(to + 32 * x + 8 * g) = f32x4{o[x][4 * g] * inv, o[x][4 * g + 1] * inv, o[x][4 * g + 2] * inv, o[x][4 * g + 3] * inv};
+    }
+    if (my_row < p.rows && out_lane < 32) p.part_lse[part * p.lse_part + out_row] = lse;
+    return;
+  }
+  if (my_row < p.rows && out_lane < 32) p.lse[out_row] = lse;
+  const uint32_t turn = lds[0] + wave * 32 * H::kRow;
+#pragma unroll
+  for (int x = 0; x < H::kBlocks; ++x)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      typename V::x4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = (T)(o[x][4 * g + j] * inv);
+      lds_put(turn + H::at_n(out_lane & 31, 4 * x + g) + 8 * (out_lane >> 5), w);
+    }
+#pragma unroll
+  for (int i = 0; i < H::kSteps; ++i) {
+    const int r = H::kCopyRows * i + out_lane / H::kChunks, ch = out_lane % H::kChunks;
+    const u32x4 x = lds_get<u32x4>(turn + H::at_n(r, ch));
+    if (row0 + r < p.rows) {
+      const RowPlace at = row_place(p, hk, row0 + r);
+      *reinterpret_cast<u32x4*>((T*)p.o + b * p.os.b + at.token * p.os.s + at.head * p.os.h + ch * 8) = x;
+    }
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------
+struct PagedShape { bool many; int tiles, row_tiles, parts, least; };     // tiles: 16-row tiles of a workgroup of few rows; row_tiles: workgroups of a key head's rows
+static PagedShape paged_shape(int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int head_dim, int64_t left, int64_t sinks) {
+  PagedShape s;
+  const int64_t rows = (int64_t)n_tokens * (n_heads / n_kv_heads);
+  s.many = rows > 32;
+  s.tiles = rows <= 16 ? 1 : 2;
+  const int tile_rows = s.many ? kSwaRows : 16 * s.tiles, keys = s.many ? kSwaBlock : 32, waves = s.many ? 1 : kPagedWaves;
+  s.row_tiles = (int)((rows + tile_rows - 1) / tile_rows);
+  s.least = s.many ? 2 : 2 * kPagedWaves;
+  const int64_t blocks = ((int64_t)room + keys - 1) / keys;
+  const int64_t seen = left < 0 ? blocks : std::min(blocks, (std::min<int64_t>(left, kFar) + n_tokens + 2 * keys - 2) / keys + (std::min<int64_t>(sinks, room) + keys - 1) / keys);
+  const double groups = (double)batch * n_kv_heads * s.row_tiles, slots = s.many || head_dim == 64 ? 2 * kCus : kCus;
+  const double memory_us = (double)batch * n_kv_heads * seen * keys * head_dim * 4 / 7e6;
+  s.parts = 1;
+  double best_us = 1e30;
+  for (int parts = 1; parts <= kPagedMaxParts && (parts == 1 || waves * (parts - 1) < seen); ++parts) {
+    const double rounds = std::ceil(groups * parts / slots), iterations = std::ceil((double)seen / (waves * parts));
+    const double tail = batch > 1 && left < 0 ? 0.4 * iterations : 0;
+    const double us = 2 * rounds + std::max((s.many ? 1.3 : 0.8) * rounds * iterations, memory_us) + tail + (parts > 1 ? 3.5 + 0.03 * parts + groups * tile_rows * parts * head_dim * 8e-7 : 0);
+    if (us < 0.99 * best_us) { best_us = us; s.parts = parts; }
+  }
+  return s;
+}
+static int paged_decode_check(int batch, int n_tokens, int n_heads, int n_kv_heads, int n_pages, int page, int max_pages, int head_dim, int dtype,
+                              int64_t table_stride, const int32_t* parents, int64_t parents_stride, int64_t left, int64_t sinks, float scale) {
+  const int rc = paged_check(batch, n_tokens, n_kv_heads, n_pages, page, max_pages, table_stride, parents, parents_stride);
+  if (rc != UA_OK) return rc;
+  if (n_heads <= 0 || n_heads % n_kv_heads || left < -1 || sinks < 0) return UA_ERR_SHAPE;
+  if (n_tokens > kSwaMaxLen || (int64_t)n_tokens * (n_heads / n_kv_heads) > kSwaMaxLen || (int64_t)batch * n_tokens * n_heads > INT32_MAX / kPagedMaxParts)
+    return UA_ERR_SHAPE;
+  if ((head_dim != 64 && head_dim != 128) || (dtype != UA_BF16 && dtype != UA_FP16) || !swa_scale_ok(scale)) return UA_ERR_UNSUPPORTED;
+  return UA_OK;
+}
+template <class T, int kD, bool kTree>
+static void paged_launch(const PagedParams& p, const PagedShape& s, unsigned n, hipStream_t st) {
+  if (s.many)            paged_many_kernel<T, kD, kTree><<<n, 256, 0, st>>>(p);
+  else if (s.tiles == 1) paged_few_kernel<T, kD, 1, kTree><<<n, 64 * kPagedWaves, 0, st>>>(p);
+  else                   paged_few_kernel<T, kD, 2, kTree><<<n, 64 * kPagedWaves, 0, st>>>(p);
+}
+
+}  // namespace ua
+
+extern "C" int64_t ua_paged_decode_workspace_bytes(int batch, int n_tokens, int n_heads, int n_kv_heads, int page, int max_pages, int head_dim, int64_t left,
+                                                   int64_t sinks) {
+  using namespace ua;
+  if (paged_decode_check(batch, n_tokens, n_heads, n_kv_heads, 1, page, max_pages, head_dim, UA_BF16, 0, nullptr, 0, left, sinks, 1.f) != UA_OK) return 0;
+  const int parts = paged_shape(batch, n_tokens, n_heads, n_kv_heads, paged_room(page, max_pages), head_dim, left, sinks).parts;
+  const int64_t rows = (int64_t)batch * n_tokens * n_heads;
+  return parts > 1 ? parts * (align256(rows * head_dim * 4) + align256(rows * 4)) : 0;
+}
+
+extern "C" int ua_paged_decode(const void* q, const void* k_pages, const void* v_pages, void* o, float* lse, const int32_t* table, const int32_t* lens,
+                               const int32_t* n_new, const int32_t* parents, int batch, int n_tokens, int n_heads, int n_kv_heads, int n_pages, int page,
+                               int max_pages, int head_dim, int dtype, int64_t table_stride, int64_t parents_stride, const int64_t* q_strides,
+                               const int64_t* k_page_strides, const int64_t* v_page_strides, const int64_t* o_strides, int64_t left, int64_t sinks,
+                               float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace ua;
+  int rc = paged_decode_check(batch, n_tokens, n_heads, n_kv_heads, n_pages, page, max_pages, head_dim, dtype, table_stride, parents, parents_stride, left,
+                              sinks, softmax_scale);
+  if (rc != UA_OK) return rc;
+  if ((int64_t)batch * n_tokens == 0) return UA_OK;
+  const bool none = n_pages == 0 || max_pages == 0;        // (the pools and the table may be NULL)
+  if (!q || !o || !lse || !lens || !q_strides || !k_page_strides || !v_page_strides || !o_strides || (!none && (!k_pages || !v_pages || !table)))
+    return UA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned4(table) || !aligned4(lens) || !aligned4(n_new) ||
+      !aligned4(parents) || !swa_strides_ok(q_strides, false) || !swa_strides_ok(k_page_strides, false) || !swa_strides_ok(v_page_strides, false) ||
+      !swa_strides_ok(o_strides, true))
+    return UA_ERR_ALIGN;
+  rc = check_device();
+  if (rc != UA_OK) return rc;
+  PagedParams p{};
+  p.pages = {table, table_stride, n_pages, page, none ? 0 : paged_room(page, max_pages), make_div(page)};
+  const PagedShape s = paged_shape(batch, n_tokens, n_heads, n_kv_heads, paged_room(page, max_pages), head_dim, left, sinks);
+  p.q = q; p.o = o; p.lse = lse;
+  p.k = {(const char*)k_pages, 2 * k_page_strides[0], 2 * k_page_strides[1], 2 * k_page_strides[2]};
+  p.v = {(const char*)v_pages, 2 * v_page_strides[0], 2 * v_page_strides[1], 2 * v_page_strides[2]};
+  p.steps = {lens, n_new, parents, parents_stride, n_tokens};
+  p.qs = {q_strides[0], q_strides[1], q_strides[2]};
+  p.os = {o_strides[0], o_strides[1], o_strides[2]};
+  p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.group = n_heads / n_kv_heads;
+  p.left = left < 0 ? kFar : (int)std::min<int64_t>(left, kFar);
+  p.sinks = left < 0 ? 0 : (int)std::min<int64_t>(sinks, kFar);
+  p.rows = n_tokens * p.group;
+  p.n_tiles = s.row_tiles;
+  p.least = s.least;
+  p.scale_log2 = softmax_scale * kLog2e;
+  p.n_parts = 1;
+  const int64_t rows = (int64_t)batch * n_tokens * n_heads, o_bytes = align256(rows * head_dim * 4), lse_bytes = align256(rows * 4);
+  if (s.parts > 1 && workspace && aligned16(workspace) && workspace_bytes >= s.parts * (o_bytes + lse_bytes)) {
+    p.n_parts = s.parts;
+    p.part_o = (float*)workspace;
+    p.part_lse = (float*)((char*)workspace + s.parts * o_bytes);
+    p.o_part = o_bytes / 4;
+    p.lse_part = lse_bytes / 4;
+  }
+  p.by_kv_heads = make_div(n_kv_heads);
+  p.by_group = make_div(p.group);
+  p.by_tiles = make_div(p.n_tiles);
+  p.by_parts = make_div(p.n_parts);
+  const hipStream_t st = (hipStream_t)stream;
+  const int64_t n = (int64_t)batch * n_kv_heads * p.n_tiles * p.n_parts;
+  if (n > kSwaMaxGroups) return UA_ERR_SHAPE;
+  p.map = block_map(batch * n_kv_heads, p.n_tiles * p.n_parts);
+  auto by_tree = [&](auto element, auto dim) {
+    typedef decltype(element) T;
+    constexpr int kD = decltype(dim)::value;
+    if (parents) paged_launch<T, kD, true>(p, s, (unsigned)n, st); else paged_launch<T, kD, false>(p, s, (unsigned)n, st);
+  };
+  auto by_dim = [&](auto element) {
+    if (head_dim == 64) by_tree(element, std::integral_constant<int, 64>{}); else by_tree(element, std::integral_constant<int, 128>{});
+  };
+  if (dtype == UA_FP16) by_dim(fp16(0)); else by_dim(bf16(0.f));
+  if (hipGetLastError() != hipSuccess) return UA_ERR_LAUNCH;
+  if (p.n_parts == 1) return UA_OK;
+  return swa_merge(p.part_o, p.o_part, p.part_lse, p.lse_part, p.n_parts, o, p.os, lse, batch, n_heads, n_tokens, head_dim, dtype, st);
+}

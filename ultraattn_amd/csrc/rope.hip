@@ -1,13 +1,14 @@
 // Rotary positions: pair i of the first `rotary_dim` entries of every head is turned by the angle position * freqs[i],
 //   (a, b) -> scale * (a cos - b sin, b cos + a sin),
 // with pairs (x[i], x[i + rotary_dim / 2]) or, interleaved, (x[2i], x[2i + 1]); the rest of the head passes through.  The
-// gradient is the turn by the negative angle with the same scale.  The appending form also sends K, rotated, and V to
-// their places in a cache.
+// gradient is the turn by the negative angle with the same scale.  The appending forms also send K, rotated, and V to
+// their places in a cache, contiguous or in pages.
 //
 // Bound: HBM, each row in and out once.  The angles are not read from a table: a workgroup makes the cosines and sines of its tokens once, in
 // LDS, and all heads of a token, of Q and of K, use them.
 #include <algorithm>
-#include "ua_common.h"
+#include <type_traits>
+#include "paged.h"
 
 namespace ua {
 
@@ -23,7 +24,7 @@ constexpr int kRopeAhead = 4;              // items of a thread whose loads are 
 struct RopeTensor {
   const void* x; void* y;
   Strides3 xs, ys;
-  int rotate, cached;        // cached: y's row is the token's position, [0, room), not its index
+  int rotate, cached;        // cached: y's row is the token's position, [0, room), not its index (in pages: ys are the strides of page, slot and head)
   int items;                 // of a token, all heads
   Div by_head, by_token;     // items of a head, of a token
 };
@@ -35,6 +36,11 @@ struct RopeParams {
   int n_tokens, seqlen, tokens_per_group, n_half, head_vecs, room;
   float scale, sign;         // of the angle: -1 turns back
   Div by_seq;
+};
+struct PagedRopeParams : RopeParams {
+  PagedSteps steps;
+  PagedTable pages;
+  Div by_lines;              // of trees: workgroups of a sequence
 };
 
 __device__ __forceinline__ int64_t rope_position(const RopeParams& p, int b, int s) {
@@ -84,12 +90,21 @@ template <class T, int kV, bool kStream> __device__ __forceinline__ void rope_st
 enum RopeWay { kPairs, kBeside };
 // A workgroup goes through the tensors one after the other, or, where there are few tokens, takes one of them (blockIdx.y): which one is
 // then a scalar either way.
-template <class T, int kV, RopeWay kWay, bool kInterleaved, bool kStream>
-__global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) {
+template <class T, int kV, RopeWay kWay, bool kInterleaved, bool kStream, class Params>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(const Params p) {
   static_assert(kWay == kPairs ? !kInterleaved || kV == 1 : kInterleaved && kV > 1, "ways");
+  constexpr bool kPaged = std::is_same_v<Params, PagedRopeParams>;
   __shared__ __attribute__((aligned(16))) float cosine[kRopeAngles], sine[kRopeAngles];
-  __shared__ int64_t position[kRopeMaxTokens];
-  const int first = blockIdx.x * p.tokens_per_group, n_here = min(p.tokens_per_group, p.n_tokens - first);
+  __shared__ int64_t position[kRopeMaxTokens];             // in pages: of the cache's row, page * 2^32 + slot; -1 none, -2 no token
+  __shared__ int depth[kPaged ? kTreeMost : 1], before[kPaged ? kTreeMost : 1];
+  int first = blockIdx.x * p.tokens_per_group, n_here = min(p.tokens_per_group, p.n_tokens - first);
+  if constexpr (kPaged) {
+    if (p.steps.parents) {                                 // a workgroup's tokens are of one sequence
+      const int b = quotient(blockIdx.x, p.by_lines), s = (blockIdx.x - b * p.by_lines.d) * p.tokens_per_group;
+      first = b * p.seqlen + s;
+      n_here = min(p.tokens_per_group, p.seqlen - s);
+    }
+  }
   const int begin = gridDim.y > 1 ? blockIdx.y : 0, end = gridDim.y > 1 ? begin + 1 : 3;
   bool made = false;
   for (int which = begin; which < end; ++which) {
@@ -122,22 +137,39 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
         } else {
           angle[u] = at * kV;                               // the first entry
         }
-        to[u] = static_cast<T*>(x.y) + b * x.ys.b + (x.cached ? 0 : s * x.ys.s) + h * x.ys.h + at * kV;
+        to[u] = static_cast<T*>(x.y) + (kPaged && x.cached ? 0 : b * x.ys.b) + (x.cached ? 0 : s * x.ys.s) + h * x.ys.h + at * kV;
         rope_load<T, kV>(a[u], head + at * kV);
         if (kWay == kPairs && second[u]) rope_load<T, kV>(b2[u], head + at * kV + second[u]);
       }
       if (!made) {                                        // workgroup-uniform; the first loads are on their way meanwhile
         made = true;
+        if constexpr (kPaged) {
+          static_assert(kRopeThreads == kTreeThreads, "a token a thread");
+          if (p.steps.parents) tree_depths(p.steps, quotient(blockIdx.x, p.by_lines), depth, before);
+        }
         for (int i = threadIdx.x; i < n_here * p.n_half; i += kRopeThreads) {
           const int t = i / p.n_half, b = quotient(first + t, p.by_seq), s = first + t - b * p.seqlen;
           float c, sn;
-          rope_angle(rope_position(p, b, s), p.freqs[i - t * p.n_half], c, sn);
+          int64_t pos;
+          if constexpr (kPaged) pos = step_of(p.steps, b).base + (p.steps.parents ? depth[s] : s); else pos = rope_position(p, b, s);
+          rope_angle(pos, p.freqs[i - t * p.n_half], c, sn);
           cosine[i] = c * p.scale;
           sine[i] = sn * p.scale * p.sign;
         }
         if (threadIdx.x < n_here) {
-          const int b = quotient(first + threadIdx.x, p.by_seq);
-          position[threadIdx.x] = rope_position(p, b, first + threadIdx.x - b * p.seqlen);
+          const int b = quotient(first + threadIdx.x, p.by_seq), s = first + threadIdx.x - b * p.seqlen;
+          if constexpr (kPaged) {
+            const StepOf of = step_of(p.steps, b);
+            const int row = of.base + s;
+            int64_t at = s < of.n ? -1 : -2;
+            if (s < of.n && row >= 0 && row < p.pages.room) {
+              const int i = quotient(row, p.pages.by_page), page = p.pages.table[b * p.pages.stride + i];
+              if (page >= 0 && page < p.pages.n_pages) at = (int64_t)page << 32 | (row - i * p.pages.page);
+            }
+            position[threadIdx.x] = at;
+          } else {
+            position[threadIdx.x] = rope_position(p, b, s);
+          }
         }
         __syncthreads();
       }
@@ -146,8 +178,13 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
         if (!to[u]) continue;
         if (x.cached) {
           const int64_t row = position[token[u]];
-          if (row < 0 || row >= p.room) continue;
-          to[u] += row * x.ys.s;
+          if constexpr (kPaged) {
+            if (row < 0) continue;
+            to[u] += (row >> 32) * x.ys.b + (uint32_t)row * x.ys.s;
+          } else {
+            if (row < 0 || row >= p.room) continue;
+            to[u] += row * x.ys.s;
+          }
         }
         if constexpr (kWay == kPairs) {
           if (angle[u] >= 0)
@@ -167,6 +204,12 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
             a[u][2 * j + 1] = (T)(e * c + g * s);
           }
         }
+        if constexpr (kPaged) {
+          if (!x.cached && position[token[u]] == -2) {
+#pragma unroll
+            for (int j = 0; j < kV; ++j) a[u][j] = b2[u][j] = (T)0.f;
+          }
+        }
         rope_store<T, kV, kStream>(to[u], a[u]);
         if (kWay == kPairs && second[u]) rope_store<T, kV, kStream>(to[u] + second[u], b2[u]);
       }
@@ -174,13 +217,13 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
   }
 }
 
-template <class T, int kV>
-static void rope_launch(const RopeParams& p, bool interleaved, bool stream, dim3 groups, hipStream_t st) {
+template <class T, int kV, class P>
+static void rope_launch(const P& p, bool interleaved, bool stream, dim3 groups, hipStream_t st) {
   constexpr bool kWide = kV * sizeof(T) == 16;
   auto run = [&](auto kernel) { kernel<<<groups, kRopeThreads, 0, st>>>(p); };
-  if constexpr (kV == 1) interleaved ? run(rope_kernel<T, 1, kPairs, true, false>) : run(rope_kernel<T, 1, kPairs, false, false>);
-  else if (interleaved)  kWide && stream ? run(rope_kernel<T, kV, kBeside, true, kWide>) : run(rope_kernel<T, kV, kBeside, true, false>);
-  else                   kWide && stream ? run(rope_kernel<T, kV, kPairs, false, kWide>) : run(rope_kernel<T, kV, kPairs, false, false>);
+  if constexpr (kV == 1) interleaved ? run(rope_kernel<T, 1, kPairs, true, false, P>) : run(rope_kernel<T, 1, kPairs, false, false, P>);
+  else if (interleaved)  kWide && stream ? run(rope_kernel<T, kV, kBeside, true, kWide, P>) : run(rope_kernel<T, kV, kBeside, true, false, P>);
+  else                   kWide && stream ? run(rope_kernel<T, kV, kPairs, false, kWide, P>) : run(rope_kernel<T, kV, kPairs, false, false, P>);
 }
 
 struct RopeShape { int batch, seqlen, head_dim, rotary_dim, dtype; };
@@ -201,7 +244,8 @@ static int rope_vector(const RopeShape& s, const RopeTensor* t, const int* heads
   return 1;
 }
 
-static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_tensors, int interleaved, hipStream_t st) {
+template <class P>
+static int rope_run(P& p, const RopeShape& s, const int* heads, int n_tensors, int interleaved, hipStream_t st) {
   const int size = s.dtype == UA_FP32 ? 4 : 2;
   p.n_half = s.rotary_dim / 2;
   const int v = rope_vector(s, p.t, heads, n_tensors, interleaved ? s.head_dim : p.n_half);
@@ -212,8 +256,10 @@ static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_t
   for (int i = 0; i < 3; ++i) {
     RopeTensor& t = p.t[i];
     if (i >= n_tensors || !heads[i]) { t.items = 0; t.by_head = t.by_token = make_div(1); continue; }
-    // what passes through is there already
-    const bool same = t.rotate && !t.cached && t.x == t.y && t.xs.b == t.ys.b && t.xs.s == t.ys.s && t.xs.h == t.ys.h;
+    // what passes through is there already (but not the zeros of tokens that are none)
+    bool zeros = false;
+    if constexpr (std::is_same_v<P, PagedRopeParams>) zeros = p.steps.n_new != nullptr;
+    const bool same = !zeros && t.rotate && !t.cached && t.x == t.y && t.xs.b == t.ys.b && t.xs.s == t.ys.s && t.xs.h == t.ys.h;
     const int turned = t.rotate ? p.n_half / v : 0;
     const int per_head = way == kPairs ? turned + (same ? 0 : (p.head_vecs - 2 * turned + 1) / 2) : same ? (s.rotary_dim + v - 1) / v : p.head_vecs;
     if ((int64_t)per_head * heads[i] * kRopeMaxTokens > INT32_MAX) return UA_ERR_SHAPE;
@@ -230,7 +276,15 @@ static int rope_run(RopeParams& p, const RopeShape& s, const int* heads, int n_t
   p.by_seq = make_div(s.seqlen);
   // Tokens of a workgroup: as many as give each thread an angle, while that leaves four workgroups a CU.
   p.tokens_per_group = std::max(1, std::min({kRopeAngles / p.n_half, kRopeMaxTokens, (kRopeThreads + p.n_half - 1) / p.n_half, p.n_tokens / (4 * kCus)}));
-  const uint32_t lines = (uint32_t)(((int64_t)p.n_tokens + p.tokens_per_group - 1) / p.tokens_per_group);
+  uint32_t lines = (uint32_t)(((int64_t)p.n_tokens + p.tokens_per_group - 1) / p.tokens_per_group);
+  if constexpr (std::is_same_v<P, PagedRopeParams>) {
+    if (p.steps.parents) {
+      const int of_one = (s.seqlen + p.tokens_per_group - 1) / p.tokens_per_group;
+      if ((int64_t)s.batch * of_one > INT32_MAX) return UA_ERR_SHAPE;
+      p.by_lines = make_div(of_one);
+      lines = (uint32_t)(s.batch * of_one);
+    }
+  }
   if (lines > UINT32_MAX / kRopeThreads) return UA_ERR_SHAPE;              // (a launch counts its threads in 32 bits)
   const dim3 groups(lines, lines <= 4 * kCus ? n_tensors : 1);
   const int rc = check_device();
@@ -313,5 +367,37 @@ extern "C" int ua_rope_append(const void* q, const void* k, const void* v, void*
   p.room = room;
   p.scale = scale;
   p.sign = 1.f;
+  return rope_run(p, s, heads, 3, interleaved, (hipStream_t)stream);
+}
+
+extern "C" int ua_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages, const double* freqs,
+                               const int32_t* table, const int32_t* lens, const int32_t* n_new, const int32_t* parents, int batch, int n_tokens, int n_heads,
+                               int n_kv_heads, int n_pages, int page, int max_pages, int head_dim, int rotary_dim, int dtype, int interleaved, float scale,
+                               int64_t table_stride, int64_t parents_stride, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                               const int64_t* q_out_strides, const int64_t* k_page_strides, const int64_t* v_page_strides, void* stream) {
+  using namespace ua;
+  const RopeShape s{batch, n_tokens, head_dim, rotary_dim, dtype};
+  int rc = rope_check(s, n_heads, n_kv_heads, scale);
+  if (rc != UA_OK) return rc;
+  rc = paged_check(batch, n_tokens, n_kv_heads, n_pages, page, max_pages, table_stride, parents, parents_stride);
+  if (rc != UA_OK) return rc;
+  if ((int64_t)batch * n_tokens == 0) return UA_OK;
+  if (n_pages == 0 || max_pages == 0) n_kv_heads = 0;      // (no row to write: the pools may be NULL)
+  if (!freqs || !lens || (n_heads && (!q || !q_out || !q_strides || !q_out_strides)) ||
+      (n_kv_heads && (!table || !k || !v || !k_pages || !v_pages || !k_strides || !v_strides || !k_page_strides || !v_page_strides)))
+    return UA_ERR_NULL;
+  if (!aligned4(table) || !aligned4(lens) || !aligned4(n_new) || !aligned4(parents)) return UA_ERR_ALIGN;
+  PagedRopeParams p{};
+  const int heads[3] = {n_heads, n_kv_heads, n_kv_heads};
+  if (n_heads) p.t[0] = {q, q_out, strides_of(q_strides), strides_of(q_out_strides), 1, 0, 0, {}, {}};
+  if (n_kv_heads) {
+    p.t[1] = {k, k_pages, strides_of(k_strides), strides_of(k_page_strides), 1, 1, 0, {}, {}};
+    p.t[2] = {v, v_pages, strides_of(v_strides), strides_of(v_page_strides), 0, 1, 0, {}, {}};
+  }
+  p.freqs = freqs;
+  p.scale = scale;
+  p.sign = 1.f;
+  p.steps = {lens, n_new, parents, parents_stride, n_tokens};
+  p.pages = {table, table_stride, n_pages, page, n_kv_heads ? paged_room(page, max_pages) : 0, make_div(page)};
   return rope_run(p, s, heads, 3, interleaved, (hipStream_t)stream);
 }
