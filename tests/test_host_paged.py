@@ -62,7 +62,7 @@ def test_workspaces(lib):
     few = f(1, 1, 32, 8, 16, 512, 128, -1, 0)
     assert few > 0 and few % 256 == 0 and few % (32 * 128 * 4 + 256) == 0
     assert f(4096, 1, 8, 8, 16, 256, 128, -1, 0) == 0 and f(1, 1, 32, 8, 16, 1, 128, -1, 0) == 0            # fills the device; one block
-    assert f(1, 1, 32, 8, 16, 512, 96, -1, 0) == 0 and f(1, 1, 32, 5, 16, 512, 128, -1, 0) == 0 and f(0, 1, 1, 1, 1, 1, 64, -1, 0) == 0
+    assert f(1, 1, 32, 8, 16, 512, 96, -1, 0) == 0 and f(1, 1, 32, 5, 16, 512, 128, -1, 0) == 0 and f(0, 1, 1, 1, 1, 1, 64, -1, 0) == f(1, 0, 1, 1, 1, 1, 64, -1, 0) == 0
     assert f(1, 40, 32, 8, 16, 4096, 128, -1, 0) > 0
     assert 0 <= f(1, 1, 1, 1, 2 ** 29, 2 ** 31 - 1, 128, 2 ** 62, 2 ** 62) < 2 ** 30
     assert 0 <= f(2 ** 20, 16, 1, 1, 1, 2 ** 31 - 1, 128, 2 ** 62, 2 ** 62) < 2 ** 44

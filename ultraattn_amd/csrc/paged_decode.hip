@@ -44,9 +44,17 @@ struct PagedParams {
   float scale_log2;
   float *part_o, *part_lse;
   int64_t o_part, lse_part;
-  Div by_kv_heads, by_group, by_tiles, by_parts;
-  BlockMap map;
+  Div by_kv_heads, by_group, by_tiles, by_walks;      // by_walks: parts and key heads of a sequence
+  int batch, n_groups, sorted, eight_shift;
 };
+
+// The kernel's parameters read again: those that only a walk's end needs do not occupy scalar registers during the walk.
+__device__ __forceinline__ const PagedParams& parameters() {
+  typedef const __attribute__((address_space(4))) PagedParams* kernarg;
+  kernarg at = (kernarg)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  return *(const PagedParams*)at;
+}
 
 // A lane's 16 bytes (4 bytes) from its own address into LDS, lane l at +16 l (+4 l) of the wave-uniform `lds`; see dma16_abs.
 __device__ __forceinline__ void dma16_at(uint64_t from, uint32_t lds) {
@@ -54,6 +62,20 @@ __device__ __forceinline__ void dma16_at(uint64_t from, uint32_t lds) {
 }
 __device__ __forceinline__ void dma4_at(uint64_t from, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" :: "s"(lds), "v"(from) : "m0");
+}
+
+// The r-th longest of up to 64 sequences (the first of equal ones first), a lane a sequence: launches of many workgroups take the longest walks first, so that
+// they do not end alone.
+__device__ __forceinline__ StepOf ranked(const PagedParams& p, int r, int& b) {
+  const int lane = fresh_lane();
+  const StepOf mine = step_of(p.steps, min(lane, p.batch - 1));
+  int rank = 0;
+  for (int i = 0; i < p.batch; ++i) {
+    const int len = __builtin_amdgcn_readlane(mine.len, i);
+    rank += len > mine.len || (len == mine.len && i < lane);
+  }
+  b = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(rank == r && lane < p.batch)) - 1;
+  return {__builtin_amdgcn_readlane(mine.len, b), __builtin_amdgcn_readlane(mine.n, b), __builtin_amdgcn_readlane(mine.base, b)};
 }
 
 // Blocks of kKeys keys that a tile's tokens t0 .. t1 see: the sinks before the window, then the window's first key on.
@@ -68,6 +90,8 @@ struct PagedWalk {
     n_sink = (sinks_end + kKeys - 1) / kKeys;
     n = n_sink + (last >= start ? (last - start) / kKeys + 1 : 0);
   }
+  // Parts that the walk is cut into: all of p.n_parts, but none of fewer blocks than p.least.  A part takes every so many-th block.
+  __device__ __forceinline__ int parts(const PagedParams& p) const { return min(p.n_parts, max((n + p.least - 1) / p.least, 1)); }
   __device__ __forceinline__ int at(int i) const { return i < n_sink ? i * kKeys : start + (i - n_sink) * kKeys; }
   __device__ __forceinline__ int end_of(int i) const { return i < n_sink ? sinks_end : last + 1; }
 };
@@ -100,19 +124,67 @@ struct PagedLane {
 constexpr int kDepth = 9, kBefore = 10, kBranchPitch = 11;       // (words; odd, so that 32 tokens' lines meet 32 banks)
 struct Branches { uint32_t line[kTreeMost * kBranchPitch]; };
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
-// By a workgroup of kTreeThreads: distances double, as in tree_depths.  A window cuts what is further behind and not among the sinks.
-__device__ __forceinline__ void tree_branches(const PagedParams& p, const StepOf& of, int b, Branches& out) {
+// Distances double, as in tree_depths: a token's branch takes up that of the token 2^k before it, round by round.  Up to 64 tokens every wave does this for itself,
+// a lane a token, and writes the same lines as the others; more take kTreeThreads threads and two barriers a round (26 tokens that way: 2 us).  A window cuts
+// what is further behind and not among the sinks.
+__device__ __forceinline__ int tree_token(const PagedSteps& p) { return p.n_tokens <= 64 ? fresh_lane() : (int)threadIdx.x; }
+template <int kWords>
+__device__ __forceinline__ void tree_lines(const PagedParams& p, const StepOf& of, int t, const uint32_t (&branch)[kWords], Branches& out) {
+  uint32_t mine[kWords];
+  int depth = -1;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) {
+    mine[w] = branch[w];
+    depth += __popc(mine[w]);
+  }
+  uint32_t* const line = out.line + t * kBranchPitch;
+  line[0] = ~0u;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) line[1 + w] = mine[w];
+  if (kWords < kTreeMost / 32) line[1 + kWords] = 0;
+  line[kDepth] = depth;
+  if (kWords > 2) __syncthreads();
+  if (p.left < p.steps.n_tokens) {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      for (uint32_t rest = mine[w]; rest; rest &= rest - 1) {
+        const int theirs = (int)out.line[(32 * w + __ffs(rest) - 1) * kBranchPitch + kDepth];
+        if (depth - theirs > p.left && of.base + theirs >= p.sinks) mine[w] &= ~(rest & -rest);
+      }
+      line[1 + w] = mine[w];
+    }
+    if (kWords > 2) __syncthreads();
+  }
+}
+__device__ __forceinline__ void tree_branches(const PagedParams& p, const StepOf& of, int parent, Branches& out) {
+  const int t = tree_token(p.steps);
+  if (p.steps.n_tokens <= 64) {
+    uint32_t mine[2] = {t < 32 ? 1u << t : 0u, t < 32 ? 0u : 1u << (t & 31)};
+    while (__builtin_amdgcn_ballot_w64(parent >= 0) != 0) {
+      const int from = max(parent, 0);
+      const uint32_t lo = __shfl(mine[0], from), hi = __shfl(mine[1], from);
+      const int before = __shfl(parent, from);
+      if (parent >= 0) {
+        mine[0] |= lo;
+        mine[1] |= hi;
+        parent = before;
+      }
+    }
+    tree_lines(p, of, t, mine, out);
+    asm volatile("" ::: "memory");
+    return;
+  }
   constexpr int kWords = kTreeMost / 32;
-  const int t = threadIdx.x, words = (p.steps.n_tokens + 31) / 32;
+  const int words = (p.steps.n_tokens + 31) / 32;
   uint32_t mine[kWords];
 #pragma unroll
   for (int w = 0; w < kWords; ++w) mine[w] = t >> 5 == w ? 1u << (t & 31) : 0u;
   uint32_t* const line = out.line + t * kBranchPitch;
-  line[0] = ~0u;
-  int parent = parent_of(p.steps, b, t);
   while (true) {
 #pragma unroll
-    for (int w = 0; w < kWords; ++w) line[1 + w] = mine[w];
+    for (int w = 0; w < kWords; ++w)
+      if (w < words) line[1 + w] = mine[w];
     line[kBefore] = parent;
     if (!__syncthreads_or(parent >= 0)) break;
     if (parent >= 0) {
@@ -124,22 +196,7 @@ __device__ __forceinline__ void tree_branches(const PagedParams& p, const StepOf
     }
     __syncthreads();
   }
-  int depth = -1;
-#pragma unroll
-  for (int w = 0; w < kWords; ++w) depth += __popc(mine[w]);
-  line[kDepth] = depth;
-  __syncthreads();
-  if (p.left < p.steps.n_tokens) {
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-      for (uint32_t rest = mine[w]; rest; rest &= rest - 1) {
-        const int theirs = (int)out.line[(32 * w + __ffs(rest) - 1) * kBranchPitch + kDepth];
-        if (depth - theirs > p.left && of.base + theirs >= p.sinks) mine[w] &= ~(rest & -rest);
-      }
-      line[1 + w] = mine[w];
-    }
-    __syncthreads();
-  }
+  tree_lines(p, of, t, mine, out);
 }
 
 // What a row sees.
@@ -168,6 +225,15 @@ struct RowSees {
   }
 };
 
+// A workgroup of a part that a short walk does not have: rows that saw nothing.  (No copy may still be on its way into LDS.)
+__device__ __forceinline__ void leave_part(const PagedParams& p, int part, int b, int hk, int row0, int row1) {
+  for (int row = row0 + threadIdx.x; row <= row1; row += blockDim.x) {
+    const int token = quotient(row, p.by_group);
+    p.part_lse[part * p.lse_part + ((int64_t)b * p.n_heads + hk * p.group + row - token * p.group) * p.steps.n_tokens + token] = -INFINITY;
+  }
+  wait_vmem_all();
+}
+
 template <int kD>
 struct FewHead {
   static constexpr int kKeys = 32, kRow = 2 * kD, kChunks = kD / 8, kCopyRows = 1024 / kRow, kUnits = kKeys / kCopyRows, kTile = kUnits * 1024;
@@ -180,7 +246,7 @@ struct FewHead {
 struct NoBranches { uint32_t line[1]; };
 
 template <class T, int kD, int kTiles, bool kTree>
-__global__ __launch_bounds__(64 * kPagedWaves) void paged_few_kernel(const PagedParams p) {
+__global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_few_kernel(const PagedParams p) {
   using H = FewHead<kD>;
   using V = SwaVec<T>;
   typedef typename V::x8 x8;
@@ -192,63 +258,87 @@ __global__ __launch_bounds__(64 * kPagedWaves) void paged_few_kernel(const Paged
   Branches& branches = reinterpret_cast<Branches&>(branch_store);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
-  const int rest = quotient(blockIdx.x, p.by_parts), part = blockIdx.x - rest * p.n_parts;
-  const int bh = quotient(rest, p.by_tiles), tile = rest - bh * p.n_tiles, b = quotient(bh, p.by_kv_heads), hk = bh - b * p.n_kv_heads;
-  const StepOf step = step_of(p.steps, b);
-  const int row0 = tile * kRows, row1 = min(row0 + kRows, p.rows) - 1;
-  const PagedWalk<H::kKeys> walk(p, step, quotient(row0, p.by_group), quotient(row1, p.by_group));
-  const int part_len = max((walk.n + p.n_parts - 1) / p.n_parts, p.least), i0 = min(part * part_len, walk.n), i1 = min(i0 + part_len, walk.n);
-
+  const int r = quotient(blockIdx.x, p.by_walks), of_r = blockIdx.x - r * p.by_walks.d, part = quotient(of_r, p.by_kv_heads), hk = of_r - part * p.n_kv_heads;
+  int b = r;
+  const StepOf step = p.sorted ? ranked(p, r, b) : step_of(p.steps, r);
+  constexpr int row0 = 0;
+  const int row1 = p.rows - 1;
   const int32_t* const line = p.pages.table + b * p.pages.stride;
-  const PagedLane<32> from(p, hk, lane);
   const uint32_t mine = lds0 + wave * H::kWave, entries = (uint32_t)(uintptr_t)(lds_byte*)tables + wave * H::kTable, places = entries + 2 * H::kEntries;
   const int key_row = lane & 31, copy_row = lane / H::kChunks, chunk = lane % H::kChunks;
-  auto fetch = [&](int i, uint32_t to) { from.fetch(p, line, walk.at(i) + key_row, walk.last, to); };
-  // The block's addresses into LDS; which of its keys are there.
-  auto locate = [&](int i, uint32_t entry_at) {
-    bool there;
-    const uint64_t a = from.address(p, walk.at(i) + key_row, i < i1 ? walk.end_of(i) : 0, lds_get<int>(entry_at + 4 * lane), there);
-    lds_put(places + 8 * lane, a);
-    return (uint32_t)__builtin_amdgcn_ballot_w64(there);
-  };
-  auto copy_in = [&](uint32_t stage) {
-#pragma unroll
-    for (int u = 0; u < H::kUnits; ++u) {
-      const int r = H::kCopyRows * u + copy_row;
-      dma16_at(lds_get<uint64_t>(places + 8 * r) + 16 * H::slot_k(r, chunk), stage + 1024 * u);
-      dma16_at(lds_get<uint64_t>(places + 256 + 8 * r) + 16 * H::slot_v(r, chunk), stage + H::kTile + 1024 * u);
-    }
-  };
-  int i = i0 + wave;
-  uint32_t there = 0, there_next = 0;
-  if (i < i1) {
-    fetch(i, entries);
-    fetch(i + kPagedWaves, entries + H::kEntries);
-    wait_vmem_all();
-    there = locate(i, entries);
-    copy_in(mine);
-    there_next = locate(i + kPagedWaves, entries + H::kEntries);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    fetch(i + 2 * kPagedWaves, entries);
-    copy_in(mine + H::kStage);
+  // What does not depend on the length is on its way before it has come: the first two blocks' entries where there is no window (if the walk then turns out to
+  // be cut into fewer parts, the second's again), the tree, Q.
+  int i = part * kPagedWaves + wave;
+  const bool early = p.left == kFar && p.pages.room > 0;
+  if (early) {
+    PagedLane<32>::fetch(p, line, 32 * i + key_row, p.pages.room - 1, entries);
+    PagedLane<32>::fetch(p, line, 32 * (i + kPagedWaves * p.n_parts) + key_row, p.pages.room - 1, entries + H::kEntries);
   }
-  if (kTree && i0 < i1) tree_branches(p, step, b, branches);
-
+  int parent = kTree ? parent_of(p.steps, b, tree_token(p.steps)) : -1;
   // Q as B operands: row col of the tile, columns 32 s + 8 quad ..
   x8 qf[kTiles][H::kSteps];
-  RowSees sees[kTiles];
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
     const int row = min(row0 + 16 * t + col, p.rows - 1), token = quotient(row, p.by_group), h = hk * p.group + row - token * p.group;
     const T* q = (const T*)p.q + b * p.qs.b + token * p.qs.s + h * p.qs.h + 8 * quad;
 #pragma unroll
     for (int s = 0; s < H::kSteps; ++s) qf[t][s] = *reinterpret_cast<const x8*>(q + 32 * s);
-    sees[t].template of<kTree>(p, step, token, branches);
   }
+  const PagedLane<32> from(p, hk, lane);
+  const PagedWalk<H::kKeys> walk(p, step, quotient(row0, p.by_group), quotient(row1, p.by_group));
+  const int parts = walk.parts(p), stride = kPagedWaves * parts, i1 = walk.n;
+  auto fetch = [&](int i, uint32_t to) { from.fetch(p, line, walk.at(i) + key_row, walk.last, to); };
+  // The block's addresses into LDS; which of its keys are there.
+  auto locate = [&](int i, uint32_t entry_at) {
+    bool there;
+    const uint64_t a = from.address(p, walk.at(i) + key_row, walk.end_of(i), lds_get<int>(entry_at + 4 * lane), there);
+    lds_put(places + 8 * lane, a);
+    return (uint32_t)__builtin_amdgcn_ballot_w64(there);
+  };
+  // (all addresses are read before the first copy: read one by one, with a wait each, 16 copies took 2000 cycles)
+  auto copy_in = [&](uint32_t stage) {
+    uint64_t k[H::kUnits], v[H::kUnits];
+#pragma unroll
+    for (int u = 0; u < H::kUnits; ++u) {
+      k[u] = lds_get<uint64_t>(places + 8 * (H::kCopyRows * u + copy_row));
+      v[u] = lds_get<uint64_t>(places + 256 + 8 * (H::kCopyRows * u + copy_row));
+    }
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < H::kUnits; ++u) {
+      const int r = H::kCopyRows * u + copy_row;
+      dma16_at(k[u] + 16 * H::slot_k(r, chunk), stage + 1024 * u);
+      dma16_at(v[u] + 16 * H::slot_v(r, chunk), stage + H::kTile + 1024 * u);
+    }
+  };
+  constexpr int kCopies = 2 * H::kUnits;
+  if (part >= parts) {
+    leave_part(p, part, b, hk, row0, row1);
+    return;
+  }
+  if (!early && i < i1) fetch(i, entries);
+  if ((!early || parts != p.n_parts) && i + stride < i1) fetch(i + stride, entries + H::kEntries);
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
     for (int s = 0; s < H::kSteps; ++s) asm volatile("" : "+v"(qf[t][s]));     // arrived before the walk counts its copies
+  asm volatile("" : "+v"(parent));
+  wait_vmem_all();
+  uint32_t there = 0, there_next = 0;
+  // (Nothing is copied of blocks that are none: a CU's four waves bring 64 bytes a cycle, so a block of each is 1000 cycles.)
+  if (i < i1) {
+    there = locate(i, entries);
+    copy_in(mine);
+    if (i + stride < i1) {
+      there_next = locate(i + stride, entries + H::kEntries);
+      if (i + 2 * stride < i1) fetch(i + 2 * stride, entries);
+      copy_in(mine + H::kStage);
+    }
+  }
+  if constexpr (kTree) tree_branches(p, step, parent, branches);
+  RowSees sees[kTiles];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) sees[t].template of<kTree>(p, step, quotient(min(row0 + 16 * t + col, p.rows - 1), p.by_group), branches);
   f32x4 o[kTiles][H::kBlocks];
   float m_run[kTiles], m_use[kTiles], l_run[kTiles];
 #pragma unroll
@@ -259,11 +349,12 @@ __global__ __launch_bounds__(64 * kPagedWaves) void paged_few_kernel(const Paged
     for (int d = 0; d < H::kBlocks; ++d) o[t][d] = f32x4{0};
   }
   uint32_t stage = mine, other = mine + H::kStage, entry_now = entries, entry_next = entries + H::kEntries;
-  constexpr int kCopies = 2 * H::kUnits;
-  for (; i < i1; i += kPagedWaves) {
+  for (; i < i1; i += stride) {
     // (in flight: this block, the entries two blocks on, the next block)
-    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kCopies) : "memory");
-    const uint32_t there_after = locate(i + 2 * kPagedWaves, entry_now);
+    if (i + stride < i1) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kCopies) : "memory");
+    else                 wait_vmem_all();
+    const bool copies = i + 2 * stride < i1;
+    const uint32_t there_after = copies ? locate(i + 2 * stride, entry_now) : 0;
     const int key0 = walk.at(i);
     x8 kf[2][H::kSteps];
 #pragma unroll
@@ -321,8 +412,10 @@ __global__ __launch_bounds__(64 * kPagedWaves) void paged_few_kernel(const Paged
       for (int d = 0; d < H::kBlocks; ++d) o[t][d] = V::mfma16(vf[d], pf, o[t][d]);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // everything of this stage is in registers
-    fetch(i + 3 * kPagedWaves, entry_next);
-    copy_in(stage);
+    if (copies) {
+      if (i + 3 * stride < i1) fetch(i + 3 * stride, entry_next);
+      copy_in(stage);
+    }
     there = there_next;
     there_next = there_after;
     const uint32_t x = stage, y = entry_now;
@@ -406,57 +499,89 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
   static_assert(kMine == 16 && H::kCopies * H::kCopyRows == kMine, "a wave's keys");
   __shared__ __attribute__((aligned(1024))) unsigned char stage_a[2 * H::kTile];
   __shared__ __attribute__((aligned(1024))) unsigned char stage_b[2 * H::kTile];
-  __shared__ __attribute__((aligned(256))) unsigned char tables[kPagedWaves * 768];                   // of a wave: two blocks' entries, a block's addresses
+  __shared__ __attribute__((aligned(256))) unsigned char tables[kPagedWaves * 1024];                  // of a wave: three blocks' entries, a block's addresses
   __shared__ std::conditional_t<kTree, Branches, NoBranches> branch_store;
   Branches& branches = reinterpret_cast<Branches&>(branch_store);
   const uint32_t lds[2] = {(uint32_t)(uintptr_t)(lds_byte*)stage_a, (uint32_t)(uintptr_t)(lds_byte*)stage_b};
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int pos, bh;
-  map_block(blockIdx.x, p.map, pos, bh);
-  const int part = quotient(pos, p.by_tiles), tile = pos - part * p.n_tiles;       // (tiles that read the same keys beside each other)
-  const int b = quotient(bh, p.by_kv_heads), hk = bh - b * p.n_kv_heads;
-  const StepOf step = step_of(p.steps, b);
+  // Tiles that read the same keys beside each other, on one XCD if there are whole eights of parts and key heads; then key heads, parts, sequences.  Of one to two
+  // workgroups a CU the second ones in reverse, so that long and short walks share a CU.
+  const int at = p.n_groups > kCus && p.n_groups <= 2 * kCus && (int)blockIdx.x >= kCus ? p.n_groups - 1 - ((int)blockIdx.x - kCus) : (int)blockIdx.x;
+  const int eighth = at >> p.eight_shift, rest = quotient(eighth, p.by_tiles), tile = eighth - rest * p.n_tiles;
+  const int walk_at = (rest << p.eight_shift) + (at & ((1 << p.eight_shift) - 1));
+  const int r = quotient(walk_at, p.by_walks), of_r = walk_at - r * p.by_walks.d, part = quotient(of_r, p.by_kv_heads), hk = of_r - part * p.n_kv_heads;
+  int b = r;
+  const StepOf step = p.sorted ? ranked(p, r, b) : step_of(p.steps, r);
   const int r0 = tile * kSwaRows, row0 = r0 + 32 * wave, n_rows = p.rows - row0;      // rows of this wave that exist (may be <= 0)
-  const PagedWalk<kSwaBlock> walk(p, step, quotient(r0, p.by_group), quotient(min(r0 + kSwaRows, p.rows) - 1, p.by_group));
-  const int part_len = max((walk.n + p.n_parts - 1) / p.n_parts, p.least), i0 = min(part * part_len, walk.n), i1 = min(i0 + part_len, walk.n);
-
   const int32_t* const line = p.pages.table + b * p.pages.stride;
-  const PagedLane<kMine> from(p, hk, lane);
-  const uint32_t entries = (uint32_t)(uintptr_t)(lds_byte*)tables + wave * 768, places = entries + 512;
+  const uint32_t entries = (uint32_t)(uintptr_t)(lds_byte*)tables + wave * 1024, entries_first = entries + 512, places = entries + 768;
   const int m = lane & (kMine - 1), key_row = H::kCopyRows * (kPagedWaves * (m / H::kCopyRows) + wave) + m % H::kCopyRows;
   const int copy_row = lane / H::kChunks, slot_row = H::kCopyRows * wave + copy_row, chunk = lane % H::kChunks;
   const uint32_t k_chunk = 16 * H::slot_n(slot_row, chunk), v_chunk = 16 * H::slot_t(slot_row, chunk);
-  auto fetch = [&](int i, int parity) { from.fetch(p, line, walk.at(i) + lane, walk.last, entries + 256 * parity); };
-  uint64_t there = 0, there_next = 0;      // keys of this block and the next that are there
-  auto locate = [&](int i, int parity) {
-    bool is;
-    const int key0 = walk.at(i), end = i < i1 ? walk.end_of(i) : 0;
-    const uint64_t a = from.address(p, key0 + key_row, end, lds_get<int>(entries + 256 * parity + 4 * key_row), is);
-    if (lane < 2 * kMine) lds_put(places + 8 * lane, a);
-    there_next = __builtin_amdgcn_ballot_w64(key0 + lane < end && (uint32_t)lds_get<int>(entries + 256 * parity + 4 * lane) < (uint32_t)p.pages.n_pages);
-  };
-  auto place = [&](int n) { return lds_get<uint64_t>(places + 128 * (n & 1) + 8 * (H::kCopyRows * (n >> 1) + copy_row)) + (n & 1 ? v_chunk : k_chunk); };
-  auto copy = [&](int n, uint64_t a, uint32_t stage) {
-    dma16_at(a, stage + (n & 1 ? kSecond : 0) + (kPagedWaves * (n >> 1) + wave) * 1024);
-  };
-  if (i0 < i1) {
-    fetch(i0, 0);
-    fetch(i0 + 1, 1);
-    wait_vmem_all();
-    locate(i0, 0);
-#pragma unroll
-    for (int n = 0; n < kPieces; ++n) copy(n, place(n), lds[0]);
+  // (as with few rows: what does not depend on the length first)
+  const bool early = p.left == kFar && p.pages.room > 0;
+  if (early) {
+    PagedLane<kMine>::fetch(p, line, kSwaBlock * part + lane, p.pages.room - 1, entries_first);
+    PagedLane<kMine>::fetch(p, line, kSwaBlock * (part + p.n_parts) + lane, p.pages.room - 1, entries + 256);
+    PagedLane<kMine>::fetch(p, line, kSwaBlock * (part + 2 * p.n_parts) + lane, p.pages.room - 1, entries);
   }
-  if (kTree && i0 < i1) tree_branches(p, step, b, branches);
-  x8 qf[H::kSteps];
+  int parent = kTree ? parent_of(p.steps, b, tree_token(p.steps)) : -1;
+  u32x4 raw[H::kSteps];
   {
-    u32x4 raw[H::kSteps];
     const int l = fresh_lane(), c = l % H::kChunks;
 #pragma unroll
     for (int i = 0; i < H::kSteps; ++i) {
       const RowPlace r = row_place(p, hk, min(row0 + H::kCopyRows * i + l / H::kChunks, p.rows - 1));
       raw[i] = *reinterpret_cast<const u32x4*>((const T*)p.q + b * p.qs.b + r.token * p.qs.s + r.head * p.qs.h + c * 8);
     }
+  }
+  const PagedLane<kMine> from(p, hk, lane);
+  const PagedWalk<kSwaBlock> walk(p, step, quotient(r0, p.by_group), quotient(min(r0 + kSwaRows, p.rows) - 1, p.by_group));
+  const int parts = walk.parts(p), i0 = part, i1 = walk.n;
+  auto fetch = [&](int i, uint32_t at) { from.fetch(p, line, walk.at(i) + lane, walk.last, at); };
+  // Of the block after the next: the addresses into LDS, and which keys are there.
+  uint64_t there = 0, there_next = 0, there_after = 0;
+  auto locate = [&](int i, int entry_mine, int entry_lane) {
+    bool is;
+    const int key0 = walk.at(i), end = i < i1 ? walk.end_of(i) : 0;
+    const uint64_t a = from.address(p, key0 + key_row, end, entry_mine, is);
+    if (lane < 2 * kMine) lds_put(places + 8 * lane, a);
+    there_after = __builtin_amdgcn_ballot_w64(key0 + lane < end && (uint32_t)entry_lane < (uint32_t)p.pages.n_pages);
+  };
+  auto entry_mine = [&](uint32_t at) { return lds_get<int>(at + 4 * key_row); };
+  auto entry_lane = [&](uint32_t at) { return lds_get<int>(at + 4 * lane); };
+  auto place = [&](int n) { return lds_get<uint64_t>(places + 128 * (n & 1) + 8 * (H::kCopyRows * (n >> 1) + copy_row)) + (n & 1 ? v_chunk : k_chunk); };
+  auto copy = [&](int n, uint64_t a, uint32_t stage) {
+    dma16_at(a, stage + (n & 1 ? kSecond : 0) + (kPagedWaves * (n >> 1) + wave) * 1024);
+  };
+  if (part >= parts) {
+    leave_part(p, part, b, hk, r0, min(r0 + kSwaRows, p.rows) - 1);
+    return;
+  }
+  if (i0 < i1 && (!early || parts != p.n_parts)) {
+    if (!early) fetch(i0, entries_first);
+    fetch(i0 + parts, entries + 256);
+    fetch(i0 + 2 * parts, entries);
+  }
+#pragma unroll
+  for (int i = 0; i < H::kSteps; ++i) asm volatile("" : "+v"(raw[i]));
+  asm volatile("" : "+v"(parent));
+  wait_vmem_all();
+  if (i0 < i1) {
+    locate(i0, entry_mine(entries_first), entry_lane(entries_first));
+    there = there_after;
+    uint64_t at[kPieces];
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) at[n] = place(n);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) copy(n, at[n], lds[0]);
+    locate(i0 + parts, entry_mine(entries + 256), entry_lane(entries + 256));
+    there_next = there_after;
+  }
+  if (kTree && i0 < i1) tree_branches(p, step, parent, branches);
+  x8 qf[H::kSteps];
+  {
     const uint32_t turn = lds[1] + wave * 32 * H::kRow;   // the stage that the first step fills
     swa_put_rows<kD>(raw, turn);
     swa_frags<T, kD>(qf, turn);
@@ -485,17 +610,25 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
     const uint32_t here = lds[kStage], other = lds[kStage ^ 1];
     const int key0 = walk.at(i);
     wait_vmem_all();
-    __syncthreads();                        // this block and the next one's entries have landed, and everyone has left the other stage
-    there = there_next;
-    locate(i + 1, (i - i0 + 1) & 1);
-    fetch(i + 2, (i - i0) & 1);
+    __syncthreads();                        // this block and the entries two blocks on have landed, and everyone has left the other stage
+    // Addresses of the next block, made a step ago; entries of the one after it, to make its addresses of beside the products.
     uint64_t at[kPieces];
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) at[n] = place(n);
+    asm volatile("" ::: "memory");          // (read at once, not one by one before its copy)
+    const uint32_t entries_after = entries + 256 * kStage;
+    const int mine_after = entry_mine(entries_after), lane_after = entry_lane(entries_after);
+    fetch(i + 3 * parts, entries + 256 * (kStage ^ 1));
+    auto turn_over = [&]() {
+      locate(i + 2 * parts, mine_after, lane_after);
+      there = there_next;
+      there_next = there_after;
+    };
     const bool hidden = n_rows <= 0 || key0 >= some_to || (key0 + kSwaBlock <= some_from && key0 >= p.sinks);
     if (hidden) {
 #pragma unroll
       for (int n = 0; n < kPieces; ++n) copy(n, at[n], other);
+      turn_over();
       return;
     }
     // S^T: two blocks of 32 keys in turn
@@ -568,6 +701,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
       exponentials();
     }
     l_run += rs;
+    turn_over();
 #pragma unroll
     for (int n = 0; n < kVAll; ++n) {
       if (n + kVAhead < kVAll) vf[(n + kVAhead) & 3] = rd_v(n + kVAhead);
@@ -576,9 +710,9 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
   };
-  for (int i = i0; i < i1; i += 2) {
+  for (int i = i0; i < i1; i += 2 * parts) {
     walk_step(i, std::integral_constant<int, 0>{});
-    if (i + 1 < i1) walk_step(i + 1, std::integral_constant<int, 1>{});
+    if (i + parts < i1) walk_step(i + parts, std::integral_constant<int, 1>{});
   }
   wait_vmem_all();                          // the last step's copies filled a stage with zeros
   __syncthreads();
@@ -586,6 +720,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
   float a, c;
   swap_lanes<32>(l_run, a, c);
   const float l = a + c;
+  const PagedParams& e = parameters();
   const bool any = (l > 0.f || l != l) && token < step.n;              // (NaN stays; a token that is none saw keys beside the others)
   const float inv = any ? 1.f / l : 0.f, lse = any ? (m_use + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 #pragma unroll
@@ -593,21 +728,21 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[x][j] = any ? o[x][j] : 0.f;
   const int out_lane = fresh_lane(), my_row = row0 + (out_lane & 31);
-  const RowPlace mine = row_place(p, hk, min(my_row, p.rows - 1));
-  const int64_t out_row = ((int64_t)b * p.n_heads + mine.head) * p.steps.n_tokens + mine.token;
-  if (p.n_parts > 1) {
-    if (my_row < p.rows && any) {
-      float* to = p.part_o + part * p.o_part + out_row * kD + 4 * (out_lane >> 5);
+  const RowPlace mine = row_place(e, hk, min(my_row, e.rows - 1));
+  const int64_t out_row = ((int64_t)b * e.n_heads + mine.head) * e.steps.n_tokens + mine.token;
+  if (e.n_parts > 1) {
+    if (my_row < e.rows && any) {
+      float* to = e.part_o + part * e.o_part + out_row * kD + 4 * (out_lane >> 5);
 #pragma unroll
       for (int x = 0; x < H::kBlocks; ++x)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<f32x4*>(to + 32 * x + 8 * g) = f32x4{o[x][4 * g] * inv, o[x][4 * g + 1] * inv, o[x][4 * g + 2] * inv, o[x][4 * g + 3] * inv};
     }
-    if (my_row < p.rows && out_lane < 32) p.part_lse[part * p.lse_part + out_row] = lse;
+    if (my_row < e.rows && out_lane < 32) e.part_lse[part * e.lse_part + out_row] = lse;
     return;
   }
-  if (my_row < p.rows && out_lane < 32) p.lse[out_row] = lse;
+  if (my_row < e.rows && out_lane < 32) e.lse[out_row] = lse;
   const uint32_t turn = lds[0] + wave * 32 * H::kRow;
 #pragma unroll
   for (int x = 0; x < H::kBlocks; ++x)
@@ -622,15 +757,69 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
   for (int i = 0; i < H::kSteps; ++i) {
     const int r = H::kCopyRows * i + out_lane / H::kChunks, ch = out_lane % H::kChunks;
     const u32x4 x = lds_get<u32x4>(turn + H::at_n(r, ch));
-    if (row0 + r < p.rows) {
-      const RowPlace at = row_place(p, hk, row0 + r);
-      *reinterpret_cast<u32x4*>((T*)p.o + b * p.os.b + at.token * p.os.s + at.head * p.os.h + ch * 8) = x;
+    if (row0 + r < e.rows) {
+      const RowPlace at = row_place(e, hk, row0 + r);
+      *reinterpret_cast<u32x4*>((T*)e.o + b * e.os.b + at.token * e.os.s + at.head * e.os.h + ch * 8) = x;
     }
   }
 }
 
+// ---- parts joined, few rows --------------------------------------------------------------------------------------------------
+// As in swa_merge, by a workgroup a row: 16 groups of 16 lanes take the parts' rows side by side, so that all of them are on their way at once and are added
+// up through LDS (32 rows of 128 in 32 parts: 5.4 us with the 64 lanes a row of swa_merge, and 3.7 this way).
+template <class T, int kD>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams p, Div by_heads, Div by_tokens) {
+  constexpr int kPer = kD / 16, kMost = kPagedMaxParts / 16;
+  __shared__ __attribute__((aligned(16))) float sums[16][kD + 4];
+  const int row = blockIdx.x, group = threadIdx.x >> 4, c = threadIdx.x & 15, lane = threadIdx.x & 63;
+  const float l = lane < p.n_parts ? p.part_lse[lane * p.lse_part + row] : -INFINITY;
+  float top = l;
+#pragma unroll
+  for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+  const float ref = top == -INFINITY ? 0.f : top, w = l == -INFINITY ? 0.f : fast_exp2((l - ref) * kLog2e);
+  float total = w, acc[kPer] = {};
+#pragma unroll
+  for (int d = 32; d; d /= 2) total += __shfl_xor(total, d);
+#pragma unroll
+  for (int n = 0; n < kMost; ++n) {
+    const int i = 16 * n + group;
+    const float f = __shfl(w, i);
+    if (i < p.n_parts && f != 0.f) {                     // (a part that saw nothing left no row)
+      const float* x = p.part_o + i * p.o_part + (int64_t)row * kD + c * kPer;
+#pragma unroll
+      for (int j = 0; j < kPer; j += 4) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(x + j);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) acc[j + m] += f * y[m];
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kPer; j += 4) *reinterpret_cast<f32x4*>(&sums[group][c * kPer + j]) = f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]};
+  __syncthreads();
+  const bool any = total > 0.f || total != total;        // (NaN stays)
+  const int bh = quotient(row, by_tokens), token = row - bh * p.steps.n_tokens, b = quotient(bh, by_heads), h = bh - b * p.n_heads;
+  if (threadIdx.x < kD) {
+    float x = 0.f;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) x += sums[g][threadIdx.x];
+    ((T*)p.o)[b * p.os.b + token * p.os.s + h * p.os.h + threadIdx.x] = any ? (T)(x / total) : (T)0.f;
+  }
+  if (threadIdx.x == 0) p.lse[row] = any ? ref + __builtin_amdgcn_logf(total) * kLn2 : -INFINITY;
+}
+
 // ---- host -----------------------------------------------------------------------------------------------------------------
-struct PagedShape { bool many; int tiles, row_tiles, parts, least; };     // tiles: 16-row tiles of a workgroup of few rows; row_tiles: workgroups of a key head's rows
+// tiles: 16-row tiles of a workgroup of few rows; row_tiles: workgroups of a key head's rows; least: blocks of a part
+struct PagedShape { bool many; int tiles, row_tiles, parts, least; };
+// Parts of a key head's keys: what an estimate in microseconds says of the longest walks that the call allows (lengths are on the device; shorter walks make fewer
+// parts).  Fitted to 4026 drawn calls of 1 to 64 sequences, 1 to 256 tokens, 60 to 33000 rows, each timed in up to 12 numbers of parts: what it takes is
+// 1.3 % (few rows) and 1.5 % (many) slower than the best of them on average, 8 and 9 % at the 95th percentile.  us in 1, 2, 4, 8, 16 and 32 parts:
+//     few    1 x 8, 4000 rows, 128 columns             38.7   25.0   17.3   13.2   11.3   11.2
+//            3 x 8, 6007 to 21353                     237    127     72.3   45.9   36.7   40.6
+//            64 x 8, 8192 to 16384                    549    560    571    594
+//     many   1 x 8, 2777 rows, 26 tokens of 4 heads    54.5   35.6   24.1   19.0   17.5   19.4
+//            16 x 8, 2048 to 8192, 64 tokens of 4     172    124    128    161
+//            3 x 8, 700 to 6000, 256 tokens           114     66.3   42.5   33.0   44
 static PagedShape paged_shape(int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int head_dim, int64_t left, int64_t sinks) {
   PagedShape s;
   const int64_t rows = (int64_t)n_tokens * (n_heads / n_kv_heads);
@@ -638,21 +827,33 @@ static PagedShape paged_shape(int batch, int n_tokens, int n_heads, int n_kv_hea
   s.tiles = rows <= 16 ? 1 : 2;
   const int tile_rows = s.many ? kSwaRows : 16 * s.tiles, keys = s.many ? kSwaBlock : 32, waves = s.many ? 1 : kPagedWaves;
   s.row_tiles = (int)((rows + tile_rows - 1) / tile_rows);
-  s.least = s.many ? 2 : 2 * kPagedWaves;
-  const int64_t blocks = ((int64_t)room + keys - 1) / keys;
-  const int64_t seen = left < 0 ? blocks : std::min(blocks, (std::min<int64_t>(left, kFar) + n_tokens + 2 * keys - 2) / keys + (std::min<int64_t>(sinks, room) + keys - 1) / keys);
-  const double groups = (double)batch * n_kv_heads * s.row_tiles, slots = s.many || head_dim == 64 ? 2 * kCus : kCus;
-  const double memory_us = (double)batch * n_kv_heads * seen * keys * head_dim * 4 / 7e6;
+  s.least = waves;
+  int64_t seen = ((int64_t)room + keys - 1) / keys;
+  if (left >= 0)
+    seen = std::min(seen, (std::min<int64_t>(left, kFar) + n_tokens + 2 * keys - 2) / keys + (std::min<int64_t>(sinks, room) + keys - 1) / keys);
+  const double walks = (double)batch * n_kv_heads, groups = walks * s.row_tiles, entries = (double)batch * n_tokens * n_heads * head_dim;
+  auto few_us = [&](int parts) {
+    const double step = head_dim == 64 ? 0.83 : 1.41, slots = head_dim == 64 ? 2 * kCus : kCus;         // a block of 32 keys a wave
+    const double n = groups * parts, steps = std::ceil((double)seen / (waves * parts)), rounds = n <= slots ? 1 : n / slots + 0.66;
+    const double memory = walks * seen * keys * head_dim * 4 / 8.1e6 + (batch > 1 ? 0.11 * steps : 0);
+    return 2.4 + std::max(rounds * steps * step, memory) + (parts > 1 ? 4.1 + 0.024 * parts + entries * parts * 6e-7 : 0);
+  };
+  auto many_us = [&](int parts) {
+    const double alone = head_dim == 64 ? 0.9 : 1.35, shared = head_dim == 64 ? 1.05 : 1.78;            // a block of 64 keys; of two workgroups of a CU
+    const double n = groups * parts, steps = std::ceil((double)seen / parts), beside = std::min(std::max((n - kCus) / kCus, 0.0), 1.0);
+    double walk = std::max(steps * (alone + (shared - alone) * beside), groups * seen / (2 * kCus) * shared);
+    if (n > 2 * kCus) walk = std::max(walk, (n / (2 * kCus) + 0.18) * steps * shared);
+    return 13.4 + walk + (parts > 1 ? 5 + entries * parts * 1.67e-6 : 0);
+  };
   s.parts = 1;
   double best_us = 1e30;
   for (int parts = 1; parts <= kPagedMaxParts && (parts == 1 || waves * (parts - 1) < seen); ++parts) {
-    const double rounds = std::ceil(groups * parts / slots), iterations = std::ceil((double)seen / (waves * parts));
-    const double tail = batch > 1 && left < 0 ? 0.4 * iterations : 0;
-    const double us = 2 * rounds + std::max((s.many ? 1.3 : 0.8) * rounds * iterations, memory_us) + tail + (parts > 1 ? 3.5 + 0.03 * parts + groups * tile_rows * parts * head_dim * 8e-7 : 0);
-    if (us < 0.99 * best_us) { best_us = us; s.parts = parts; }
+    const double us = s.many ? many_us(parts) : few_us(parts);
+    if (us < 0.98 * best_us) { best_us = us; s.parts = parts; }
   }
   return s;
 }
+constexpr int kJoinRows = 2048;                       // rows up to which a workgroup joins one
 static int paged_decode_check(int batch, int n_tokens, int n_heads, int n_kv_heads, int n_pages, int page, int max_pages, int head_dim, int dtype,
                               int64_t table_stride, const int32_t* parents, int64_t parents_stride, int64_t left, int64_t sinks, float scale) {
   const int rc = paged_check(batch, n_tokens, n_kv_heads, n_pages, page, max_pages, table_stride, parents, parents_stride);
@@ -728,11 +929,14 @@ extern "C" int ua_paged_decode(const void* q, const void* k_pages, const void* v
   p.by_kv_heads = make_div(n_kv_heads);
   p.by_group = make_div(p.group);
   p.by_tiles = make_div(p.n_tiles);
-  p.by_parts = make_div(p.n_parts);
+  p.by_walks = make_div(p.n_parts * n_kv_heads);
   const hipStream_t st = (hipStream_t)stream;
   const int64_t n = (int64_t)batch * n_kv_heads * p.n_tiles * p.n_parts;
   if (n > kSwaMaxGroups) return UA_ERR_SHAPE;
-  p.map = block_map(batch * n_kv_heads, p.n_tiles * p.n_parts);
+  p.batch = batch;
+  p.n_groups = (int)n;
+  p.sorted = batch > 1 && batch <= 64 && n > kCus;
+  p.eight_shift = n / p.n_tiles % 8 ? 0 : 3;
   auto by_tree = [&](auto element, auto dim) {
     typedef decltype(element) T;
     constexpr int kD = decltype(dim)::value;
@@ -744,5 +948,15 @@ extern "C" int ua_paged_decode(const void* q, const void* k_pages, const void* v
   if (dtype == UA_FP16) by_dim(fp16(0)); else by_dim(bf16(0.f));
   if (hipGetLastError() != hipSuccess) return UA_ERR_LAUNCH;
   if (p.n_parts == 1) return UA_OK;
+  if (rows <= kJoinRows && p.n_parts > 4) {
+    auto join = [&](auto element, auto dim) {
+      paged_join_kernel<decltype(element), decltype(dim)::value><<<(unsigned)rows, 256, 0, st>>>(p, make_div(n_heads), make_div(n_tokens));
+    };
+    auto join_dim = [&](auto element) {
+      if (head_dim == 64) join(element, std::integral_constant<int, 64>{}); else join(element, std::integral_constant<int, 128>{});
+    };
+    if (dtype == UA_FP16) join_dim(fp16(0)); else join_dim(bf16(0.f));
+    return hipGetLastError() == hipSuccess ? UA_OK : UA_ERR_LAUNCH;
+  }
   return swa_merge(p.part_o, p.o_part, p.part_lse, p.lse_part, p.n_parts, o, p.os, lse, batch, n_heads, n_tokens, head_dim, dtype, st);
 }
