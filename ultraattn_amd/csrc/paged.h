@@ -14,7 +14,7 @@ namespace ua {
 constexpr int kPagedMost = 1 << 29;                   // lengths are clamped to it: no sum of two rows leaves 32 bits
 constexpr int kTreeMost = UA_PAGED_MAX_TREE;
 constexpr int kTreeThreads = 256;                     // of the workgroups that walk trees
-static_assert(kTreeMost <= kTreeThreads, "a token a thread");
+static_assert(kTreeMost == kTreeThreads, "a token a thread");
 
 struct PagedSteps {                                   // the new tokens of all sequences
   const int32_t *lens, *n_new, *parents;
@@ -38,15 +38,26 @@ __device__ __forceinline__ int parent_of(const PagedSteps& p, int b, int t) {
 }
 
 // Depths of a sequence's tokens, by a workgroup of kTreeThreads: every token's distance to a token before it, and that one, doubled until all have
-// reached the first of their branch, as many times as the deepest branch's logarithm (as one thread a branch, 64 deep: 64 reads in a row).
-__device__ __forceinline__ void tree_depths(const PagedSteps& p, int b, int (&depth)[kTreeMost], int (&before)[kTreeMost]) {
-  const int t = threadIdx.x;
-  int parent = parent_of(p, b, t), d = parent >= 0;
-  while (true) {
-    if (t < kTreeMost) {
-      depth[t] = d;
-      before[t] = parent;
+// reached the first of their branch, as many times as the deepest branch's logarithm.  Up to 64 tokens every wave does this for itself, a lane a token, and
+// writes what the others write; more meet at two barriers a round.  `parent`: of the token that tree_token names.
+__device__ __forceinline__ int tree_token(const PagedSteps& p) { return p.n_tokens <= 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x; }
+__device__ __forceinline__ void tree_depths(const PagedSteps& p, int parent, int (&depth)[kTreeMost], int (&before)[kTreeMost]) {
+  const int t = tree_token(p);
+  int d = parent >= 0;
+  if (p.n_tokens <= 64) {
+    while (__builtin_amdgcn_ballot_w64(parent >= 0) != 0) {
+      const int from = max(parent, 0), far = __shfl(d, from), next = __shfl(parent, from);
+      if (parent >= 0) {
+        d += far;
+        parent = next;
+      }
     }
+    depth[t] = d;
+    return;
+  }
+  while (true) {
+    depth[t] = d;
+    before[t] = parent;
     if (!__syncthreads_or(parent >= 0)) return;
     if (parent >= 0) {
       d += depth[parent];

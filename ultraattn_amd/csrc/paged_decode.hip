@@ -127,7 +127,6 @@ __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 
 // Distances double, as in tree_depths: a token's branch takes up that of the token 2^k before it, round by round.  Up to 64 tokens every wave does this for itself,
 // a lane a token, and writes the same lines as the others; more take kTreeThreads threads and two barriers a round (26 tokens that way: 2 us).  A window cuts
 // what is further behind and not among the sinks.
-__device__ __forceinline__ int tree_token(const PagedSteps& p) { return p.n_tokens <= 64 ? fresh_lane() : (int)threadIdx.x; }
 template <int kWords>
 __device__ __forceinline__ void tree_lines(const PagedParams& p, const StepOf& of, int t, const uint32_t (&branch)[kWords], Branches& out) {
   uint32_t mine[kWords];
@@ -847,7 +846,8 @@ static PagedShape paged_shape(int batch, int n_tokens, int n_heads, int n_kv_hea
   };
   s.parts = 1;
   double best_us = 1e30;
-  for (int parts = 1; parts <= kPagedMaxParts && (parts == 1 || waves * (parts - 1) < seen); ++parts) {
+  // (every number up to 8, then every second, fourth and eighth one: 20 of them, twice a call)
+  for (int parts = 1; parts <= kPagedMaxParts && (parts == 1 || waves * (parts - 1) < seen); parts += parts < 8 ? 1 : parts < 16 ? 2 : parts < 32 ? 4 : 8) {
     const double us = s.many ? many_us(parts) : few_us(parts);
     if (us < 0.98 * best_us) { best_us = us; s.parts = parts; }
   }

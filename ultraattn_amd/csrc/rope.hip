@@ -97,12 +97,13 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const Params p) {
   __shared__ __attribute__((aligned(16))) float cosine[kRopeAngles], sine[kRopeAngles];
   __shared__ int64_t position[kRopeMaxTokens];             // in pages: of the cache's row, page * 2^32 + slot; -1 none, -2 no token
   __shared__ int depth[kPaged ? kTreeMost : 1], before[kPaged ? kTreeMost : 1];
-  int first = blockIdx.x * p.tokens_per_group, n_here = min(p.tokens_per_group, p.n_tokens - first);
+  int first = blockIdx.x * p.tokens_per_group, n_here = min(p.tokens_per_group, p.n_tokens - first), parent = -1;
   if constexpr (kPaged) {
     if (p.steps.parents) {                                 // a workgroup's tokens are of one sequence
       const int b = quotient(blockIdx.x, p.by_lines), s = (blockIdx.x - b * p.by_lines.d) * p.tokens_per_group;
       first = b * p.seqlen + s;
       n_here = min(p.tokens_per_group, p.seqlen - s);
+      parent = parent_of(p.steps, b, tree_token(p.steps));
     }
   }
   const int begin = gridDim.y > 1 ? blockIdx.y : 0, end = gridDim.y > 1 ? begin + 1 : 3;
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const Params p) {
         made = true;
         if constexpr (kPaged) {
           static_assert(kRopeThreads == kTreeThreads, "a token a thread");
-          if (p.steps.parents) tree_depths(p.steps, quotient(blockIdx.x, p.by_lines), depth, before);
+          if (p.steps.parents) tree_depths(p.steps, parent, depth, before);
         }
         for (int i = threadIdx.x; i < n_here * p.n_half; i += kRopeThreads) {
           const int t = i / p.n_half, b = quotient(first + t, p.by_seq), s = first + t - b * p.seqlen;
@@ -246,6 +247,7 @@ static int rope_vector(const RopeShape& s, const RopeTensor* t, const int* heads
 
 template <class P>
 static int rope_run(P& p, const RopeShape& s, const int* heads, int n_tensors, int interleaved, hipStream_t st) {
+  constexpr bool kPaged = std::is_same_v<P, PagedRopeParams>;
   const int size = s.dtype == UA_FP32 ? 4 : 2;
   p.n_half = s.rotary_dim / 2;
   const int v = rope_vector(s, p.t, heads, n_tensors, interleaved ? s.head_dim : p.n_half);
@@ -258,7 +260,7 @@ static int rope_run(P& p, const RopeShape& s, const int* heads, int n_tensors, i
     if (i >= n_tensors || !heads[i]) { t.items = 0; t.by_head = t.by_token = make_div(1); continue; }
     // what passes through is there already (but not the zeros of tokens that are none)
     bool zeros = false;
-    if constexpr (std::is_same_v<P, PagedRopeParams>) zeros = p.steps.n_new != nullptr;
+    if constexpr (kPaged) zeros = p.steps.n_new != nullptr;
     const bool same = !zeros && t.rotate && !t.cached && t.x == t.y && t.xs.b == t.ys.b && t.xs.s == t.ys.s && t.xs.h == t.ys.h;
     const int turned = t.rotate ? p.n_half / v : 0;
     const int per_head = way == kPairs ? turned + (same ? 0 : (p.head_vecs - 2 * turned + 1) / 2) : same ? (s.rotary_dim + v - 1) / v : p.head_vecs;
@@ -274,10 +276,13 @@ static int rope_run(P& p, const RopeShape& s, const int* heads, int n_tensors, i
   if (p.n_tokens == 0 || n_items == 0) return UA_OK;
   const bool stream = bytes > kRopeStreamBytes;
   p.by_seq = make_div(s.seqlen);
-  // Tokens of a workgroup: as many as give each thread an angle, while that leaves four workgroups a CU.
-  p.tokens_per_group = std::max(1, std::min({kRopeAngles / p.n_half, kRopeMaxTokens, (kRopeThreads + p.n_half - 1) / p.n_half, p.n_tokens / (4 * kCus)}));
+  // Tokens of a workgroup: as many as give each thread an angle, while that leaves four workgroups a CU; in pages, whose tokens' lengths, trees and table entries each
+  // workgroup reads first, one, times the tensors (one token a workgroup and three or four, us: 32 trees of 25 tokens, 14 + 4 heads of 64, 8.2 and 6.4; 3
+  // of 256, 8 + 16 of 128, 13.4 and 7.2; 16 chains of 64, 32 + 16 of 128, 11.4 and 8.8; 64 trees of 64 by tensors 21.8, all three 20.1).
+  p.tokens_per_group = std::max(1, std::min({kRopeAngles / p.n_half, kRopeMaxTokens, (kRopeThreads + p.n_half - 1) / p.n_half,
+                                             p.n_tokens / ((kPaged ? 1 : 4) * kCus)}));
   uint32_t lines = (uint32_t)(((int64_t)p.n_tokens + p.tokens_per_group - 1) / p.tokens_per_group);
-  if constexpr (std::is_same_v<P, PagedRopeParams>) {
+  if constexpr (kPaged) {
     if (p.steps.parents) {
       const int of_one = (s.seqlen + p.tokens_per_group - 1) / p.tokens_per_group;
       if ((int64_t)s.batch * of_one > INT32_MAX) return UA_ERR_SHAPE;
@@ -286,7 +291,7 @@ static int rope_run(P& p, const RopeShape& s, const int* heads, int n_tensors, i
     }
   }
   if (lines > UINT32_MAX / kRopeThreads) return UA_ERR_SHAPE;              // (a launch counts its threads in 32 bits)
-  const dim3 groups(lines, lines <= 4 * kCus ? n_tensors : 1);
+  const dim3 groups(lines, lines <= (kPaged ? 2 : 4) * kCus ? n_tensors : 1);
   const int rc = check_device();
   if (rc != UA_OK) return rc;
   auto launch = [&](auto element) {
