@@ -418,7 +418,7 @@ int ua_rows_delta(const void *o, const void *dout, float *delta,
  * table DEVICE int32 [batch, max_pages], rows table_stride apart: row r of sequence b is slot r % page of page table[b, r / page].  An entry outside
  * [0, n_pages) is a page that is not there: nothing is written to it, and its rows are not seen; entries behind the last row are not used.  Sequences
  * may share pages that none of them writes.  A contiguous cache [batch, room, ...] is one of batch pages of `room` rows.
- * A call brings n_tokens tokens of every sequence, n_new[b] (DEVICE int32; NULL: all) of them real; lens[b] (DEVICE int32) is the length WITH the real ones,
+ * A call brings n_tokens tokens of every sequence, n_new[b] (DEVICE int32, 0 .. n_tokens, to which others are clamped; NULL: all) of them real; lens[b] (DEVICE int32) is the length WITH the real ones,
  * base = lens[b] - n_new[b], and token t's row is base + t.  The tokens are a chain, or a tree with parents (DEVICE int32 [batch, n_tokens], rows
  * parents_stride apart, 0: one tree for all; n_tokens <= UA_PAGED_MAX_TREE): parents[b, t] is the token before token t, and any value but 0 .. t - 1 says
  * that row base - 1 is.  A token's position is base plus the number of tokens before it in its branch (in a chain, its row).  Lengths count up to

@@ -183,6 +183,17 @@ def test_long_caches_in_parts():
         check(q, kp, vp, table, ints([320, 41]), None, None, -1, 0, out, lse)
 
 
+@pytest.mark.parametrize("batch", [40, 64, 70])
+@pytest.mark.parametrize("tokens,heads,kv_heads,tree", [(1, 8, 8, False), (5, 12, 6, True), (20, 16, 8, True), (70, 8, 4, False)])
+def test_large_launches_take_the_longest_first(batch, tokens, heads, kv_heads, tree):
+    """More workgroups than CUs: sequences are ranked by length up to 64 of them; equal and empty ones among them."""
+    kp, vp, table = pools(batch, 330, 16, kv_heads, 64, torch.bfloat16)
+    lens = spread(batch, 0, 330, batch)
+    lens[5:15] = 200
+    n_new = torch.minimum(torch.full_like(lens, tokens), lens)
+    run(queries(batch, tokens, heads, 64, torch.bfloat16), kp, vp, table, lens, n_new, trees(batch, tokens) if tree else None)
+
+
 def test_pools_beyond_two_gigabytes():
     pages, page = 70_000, 16
     kp = torch.zeros(pages, page, 16, 128, dtype=torch.bfloat16, device=DEV)
@@ -194,6 +205,12 @@ def test_pools_beyond_two_gigabytes():
         for i in range(13):
             kp[pages - 1 - i], vp[pages - 1 - i] = k[0, 16 * i:16 * i + 16], v[0, 16 * i:16 * i + 16]
         run(q, kp, vp, table, ints([208]))
+    rows = pages * page                                         # one page of all rows
+    long_k, long_v = kp.view(1, rows, 16, 128), vp.view(1, rows, 16, 128)
+    long_k[:, -208:], long_v[:, -208:] = k, v
+    out, lse = ua.paged_decode(q, long_k, long_v, ints([[0]]), ints([rows]), window=207 - 19, sinks=0)
+    seen = torch.ones(20, 208, dtype=torch.bool, device=DEV).tril(188) & ~torch.ones(20, 208, dtype=torch.bool, device=DEV).tril(-1)
+    Reference(q, k, v, seen).check(out=out, lse=lse)
 
 
 def test_two_calls_at_once_and_on_another_stream():

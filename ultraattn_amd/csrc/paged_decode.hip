@@ -316,7 +316,10 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_few_kernel(const Pa
     return;
   }
   if (!early && i < i1) fetch(i, entries);
-  if ((!early || parts != p.n_parts) && i + stride < i1) fetch(i + stride, entries + H::kEntries);
+  if ((!early || parts != p.n_parts) && i + stride < i1) {
+    if (early) wait_vmem_all();                            // (the same place in LDS)
+    fetch(i + stride, entries + H::kEntries);
+  }
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -558,7 +561,8 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
     return;
   }
   if (i0 < i1 && (!early || parts != p.n_parts)) {
-    if (!early) fetch(i0, entries_first);
+    if (early) wait_vmem_all();                            // (the same places in LDS)
+    else       fetch(i0, entries_first);
     fetch(i0 + parts, entries + 256);
     fetch(i0 + 2 * parts, entries);
   }

@@ -34,7 +34,7 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(const KeepPara
     const int rows = min(kKeepRows, n - i0);
     if (i0) __syncthreads();
     if (threadIdx.x < rows) {
-      const int i = i0 + threadIdx.x, token = p.path[b * p.path_stride + i], to = of.base + i, from = of.base + token;
+      const int i = i0 + threadIdx.x, token = p.path[b * p.path_stride + i], to = of.base + i, from = of.base + min(max(token, 0), of.n);
       int page = -1, source = -1, slot = 0, source_slot = 0;
       if (token > i && token < of.n && to >= 0 && from < p.pages.room) {          // (token == i: it is there)
         const int32_t* const line = p.pages.table + b * p.pages.stride;
