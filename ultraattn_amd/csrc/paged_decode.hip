@@ -121,81 +121,53 @@ struct PagedLane {
 
 // The branches of a sequence's tokens: bit j of a token's 256 is set if it is token j or comes behind it.  Words 1 .. 8 of a token's line hold them, word 0
 // stands for the cache's rows before (all seen); word 9, which is shifted in behind the last bit, no row gets to.
-constexpr int kDepth = 9, kBefore = 10, kBranchPitch = 11;       // (words; odd, so that 32 tokens' lines meet 32 banks)
+constexpr int kDepth = 9, kExit = 10, kBranchPitch = 11;       // (words; odd, so that 32 tokens' lines meet 32 banks)
 struct Branches { uint32_t line[kTreeMost * kBranchPitch]; };
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
-// Distances double, as in tree_depths: a token's branch takes up that of the token 2^k before it, round by round.  Up to 64 tokens every wave does this for itself,
-// a lane a token, and writes the same lines as the others; more take kTreeThreads threads and two barriers a round (26 tokens that way: 2 us).  A window cuts
-// what is further behind and not among the sinks.
-template <int kWords>
-__device__ __forceinline__ void tree_lines(const PagedParams& p, const StepOf& of, int t, const uint32_t (&branch)[kWords], Branches& out) {
-  uint32_t mine[kWords];
-  int depth = -1;
-#pragma unroll
-  for (int w = 0; w < kWords; ++w) {
-    mine[w] = branch[w];
-    depth += __popc(mine[w]);
-  }
-  uint32_t* const line = out.line + t * kBranchPitch;
-  line[0] = ~0u;
-#pragma unroll
-  for (int w = 0; w < kWords; ++w) line[1 + w] = mine[w];
-  if (kWords < kTreeMost / 32) line[1 + kWords] = 0;
-  line[kDepth] = depth;
-  if (kWords > 2) __syncthreads();
-  if (p.left < p.steps.n_tokens) {
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-      for (uint32_t rest = mine[w]; rest; rest &= rest - 1) {
-        const int theirs = (int)out.line[(32 * w + __ffs(rest) - 1) * kBranchPitch + kDepth];
-        if (depth - theirs > p.left && of.base + theirs >= p.sinks) mine[w] &= ~(rest & -rest);
-      }
-      line[1 + w] = mine[w];
-    }
-    if (kWords > 2) __syncthreads();
-  }
-}
+// (see tree_part.)  A window cuts what is further behind and not among the sinks.
 __device__ __forceinline__ void tree_branches(const PagedParams& p, const StepOf& of, int parent, Branches& out) {
-  const int t = tree_token(p.steps);
-  if (p.steps.n_tokens <= 64) {
-    uint32_t mine[2] = {t < 32 ? 1u << t : 0u, t < 32 ? 0u : 1u << (t & 31)};
-    while (__builtin_amdgcn_ballot_w64(parent >= 0) != 0) {
-      const int from = max(parent, 0);
-      const uint32_t lo = __shfl(mine[0], from), hi = __shfl(mine[1], from);
-      const int before = __shfl(parent, from);
-      if (parent >= 0) {
-        mine[0] |= lo;
-        mine[1] |= hi;
-        parent = before;
-      }
-    }
-    tree_lines(p, of, t, mine, out);
-    asm volatile("" ::: "memory");
-    return;
-  }
-  constexpr int kWords = kTreeMost / 32;
-  const int words = (p.steps.n_tokens + 31) / 32;
-  uint32_t mine[kWords];
-#pragma unroll
-  for (int w = 0; w < kWords; ++w) mine[w] = t >> 5 == w ? 1u << (t & 31) : 0u;
+  const int t = tree_token(p.steps), words = 2 * (t >> 6);
+  const bool alone = p.steps.n_tokens <= 64;
+  const TreePart x = tree_part(t, parent);
   uint32_t* const line = out.line + t * kBranchPitch;
-  while (true) {
-#pragma unroll
-    for (int w = 0; w < kWords; ++w)
-      if (w < words) line[1 + w] = mine[w];
-    line[kBefore] = parent;
-    if (!__syncthreads_or(parent >= 0)) break;
-    if (parent >= 0) {
-      const uint32_t* const theirs = out.line + parent * kBranchPitch;
-#pragma unroll
-      for (int w = 0; w < kWords; ++w)
-        if (w < words) mine[w] |= theirs[1 + w];
-      parent = (int)theirs[kBefore];
+  int depth = __popc(x.bits[0]) + __popc(x.bits[1]) - 1;
+  line[0] = ~0u;
+  line[1 + words] = x.bits[0];
+  line[2 + words] = x.bits[1];
+  if (alone) {
+    line[3] = 0u;
+    line[kDepth] = depth;
+  } else {
+    line[kExit] = x.exit;
+    for (int w = 0; w < kTreeMost / 32; ++w)
+      if (w < words || w > words + 1) line[1 + w] = 0u;
+    __syncthreads();
+    for (int at = x.exit; at >= 0;) {                     // (of another token's line only what it wrote before the barrier is read)
+      const uint32_t* const theirs = out.line + at * kBranchPitch;
+      const int there = 2 * (at >> 6);
+      const uint32_t lo = theirs[1 + there], hi = theirs[2 + there];
+      line[1 + there] = lo;
+      line[2 + there] = hi;
+      depth += __popc(lo) + __popc(hi);
+      at = (int)theirs[kExit];
     }
+    line[kDepth] = depth;
     __syncthreads();
   }
-  tree_lines(p, of, t, mine, out);
+  if (p.left < p.steps.n_tokens) {
+    asm volatile("" ::: "memory");
+    for (int w = 0; w <= words + 1; ++w) {
+      const uint32_t all = line[1 + w];
+      uint32_t kept = all;
+      for (uint32_t rest = all; rest; rest &= rest - 1) {
+        const int theirs = (int)out.line[(32 * w + __ffs(rest) - 1) * kBranchPitch + kDepth];
+        if (depth - theirs > p.left && of.base + theirs >= p.sinks) kept &= ~(rest & -rest);
+      }
+      line[1 + w] = kept;
+    }
+    if (!alone) __syncthreads();
+  }
+  asm volatile("" ::: "memory");
 }
 
 // What a row sees.

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const Params p) {
   constexpr bool kPaged = std::is_same_v<Params, PagedRopeParams>;
   __shared__ __attribute__((aligned(16))) float cosine[kRopeAngles], sine[kRopeAngles];
   __shared__ int64_t position[kRopeMaxTokens];             // in pages: of the cache's row, page * 2^32 + slot; -1 none, -2 no token
-  __shared__ int depth[kPaged ? kTreeMost : 1], before[kPaged ? kTreeMost : 1];
+  __shared__ int depth[kPaged ? kTreeMost : 1], exits[kPaged ? kTreeMost : 1];
   int first = blockIdx.x * p.tokens_per_group, n_here = min(p.tokens_per_group, p.n_tokens - first), parent = -1;
   if constexpr (kPaged) {
     if (p.steps.parents) {                                 // a workgroup's tokens are of one sequence
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const Params p) {
         made = true;
         if constexpr (kPaged) {
           static_assert(kRopeThreads == kTreeThreads, "a token a thread");
-          if (p.steps.parents) tree_depths(p.steps, parent, depth, before);
+          if (p.steps.parents) tree_depths(p.steps, parent, depth, exits);
         }
         for (int i = threadIdx.x; i < n_here * p.n_half; i += kRopeThreads) {
           const int t = i / p.n_half, b = quotient(first + t, p.by_seq), s = first + t - b * p.seqlen;
