@@ -3,8 +3,8 @@
 // The rows of a key head are the new tokens of each of the query heads that share it, row = token * group + head of the group.  Two kernels:
 //   few rows (up to 32 of a key head): as against a contiguous cache, four waves of a workgroup go through blocks of 32 keys of their own, rows are the columns
 //     of 16x16x32 products, and the waves' rows are merged at the end.  Bound: HBM, the visible keys and values once.
-//   many rows: tiles of 128, 32 a wave, go through blocks of 64 keys together, as in the sliding-window forward (32x32x16 products, two LDS stages).  Bound: the
-//     products, or HBM where the tiles are few.
+//   many rows: tiles of 128, 32 a wave as two times 16 columns of the same products, go through blocks of 64 keys together (two LDS stages).  Bound: the products,
+//     or HBM where the tiles are few.  (With 32x32x16 products, half as many instructions, 2048 tokens of 8 x 4 heads after 6144 keys took 247 us, with these 235.)
 // The keys of long caches are cut into parts, workgroups of their own, that leave fp32 rows for a merge.
 //
 // Pages: a lane's copy names its own address, so a block's keys may lie on any pages and start anywhere.  The table's entries come into LDS two blocks ahead, by
@@ -469,6 +469,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
   using H = SwaHead<kD>;
   using V = SwaVec<T>;
   typedef typename V::x8 x8;
+  using F = FewHead<kD>;                    // (the products' fragments and LDS layout are those of few rows, two tiles of 16 a wave)
   constexpr int kPieces = 2 * H::kCopies, kSecond = H::kTile, kMine = kSwaBlock / kPagedWaves;        // kMine: keys of a block that a wave copies
   static_assert(kMine == 16 && H::kCopies * H::kCopyRows == kMine, "a wave's keys");
   __shared__ __attribute__((aligned(1024))) unsigned char stage_a[2 * H::kTile];
@@ -491,7 +492,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
   const uint32_t entries = (uint32_t)(uintptr_t)(lds_byte*)tables + wave * 1024, entries_first = entries + 512, places = entries + 768;
   const int m = lane & (kMine - 1), key_row = H::kCopyRows * (kPagedWaves * (m / H::kCopyRows) + wave) + m % H::kCopyRows;
   const int copy_row = lane / H::kChunks, slot_row = H::kCopyRows * wave + copy_row, chunk = lane % H::kChunks;
-  const uint32_t k_chunk = 16 * H::slot_n(slot_row, chunk), v_chunk = 16 * H::slot_t(slot_row, chunk);
+  const uint32_t k_chunk = 16 * F::slot_k(slot_row, chunk), v_chunk = 16 * F::slot_v(slot_row, chunk);
   // (as with few rows: what does not depend on the length first)
   const bool early = p.left == kFar && p.pages.room > 0;
   if (early) {
@@ -500,14 +501,14 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
     PagedLane<kMine>::fetch(p, line, kSwaBlock * (part + 2 * p.n_parts) + lane, p.pages.room - 1, entries);
   }
   int parent = kTree ? parent_of(p.steps, b, tree_token(p.steps)) : -1;
-  u32x4 raw[H::kSteps];
-  {
-    const int l = fresh_lane(), c = l % H::kChunks;
+  const int col = lane & 15, quad = lane >> 4;
+  x8 qf[2][F::kSteps];
 #pragma unroll
-    for (int i = 0; i < H::kSteps; ++i) {
-      const RowPlace r = row_place(p, hk, min(row0 + H::kCopyRows * i + l / H::kChunks, p.rows - 1));
-      raw[i] = *reinterpret_cast<const u32x4*>((const T*)p.q + b * p.qs.b + r.token * p.qs.s + r.head * p.qs.h + c * 8);
-    }
+  for (int t = 0; t < 2; ++t) {
+    const RowPlace r = row_place(p, hk, min(row0 + 16 * t + col, p.rows - 1));
+    const T* q = (const T*)p.q + b * p.qs.b + r.token * p.qs.s + r.head * p.qs.h + 8 * quad;
+#pragma unroll
+    for (int k = 0; k < F::kSteps; ++k) qf[t][k] = *reinterpret_cast<const x8*>(q + 32 * k);
   }
   const PagedLane<kMine> from(p, hk, lane);
   const PagedWalk<kSwaBlock> walk(p, step, quotient(r0, p.by_group), quotient(min(r0 + kSwaRows, p.rows) - 1, p.by_group));
@@ -539,7 +540,9 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
     fetch(i0 + 2 * parts, entries);
   }
 #pragma unroll
-  for (int i = 0; i < H::kSteps; ++i) asm volatile("" : "+v"(raw[i]));
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int k = 0; k < F::kSteps; ++k) asm volatile("" : "+v"(qf[t][k]));
   asm volatile("" : "+v"(parent));
   wait_vmem_all();
   if (i0 < i1) {
@@ -555,30 +558,34 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
     there_next = there_after;
   }
   if (kTree && i0 < i1) tree_branches(p, step, parent, branches);
-  x8 qf[H::kSteps];
-  {
-    const uint32_t turn = lds[1] + wave * 32 * H::kRow;   // the stage that the first step fills
-    swa_put_rows<kD>(raw, turn);
-    swa_frags<T, kD>(qf, turn);
+  RowSees sees[2];
+  int token[2];
 #pragma unroll
-    for (int i = 0; i < H::kSteps; ++i) asm volatile("" : "+v"(qf[i]));      // read before the walk
+  for (int t = 0; t < 2; ++t) {
+    token[t] = quotient(min(row0 + 16 * t + col, p.rows - 1), p.by_group);
+    sees[t].template of<kTree>(p, step, token[t], branches);
   }
-  RowSees sees;
-  const int token = quotient(min(row0 + (lane & 31), p.rows - 1), p.by_group);
-  sees.template of<kTree>(p, step, token, branches);
   // Keys that every real row of the wave sees: from .. to - 1, and those before `sinks` up to there.
   const int t_first = quotient(min(row0, p.rows - 1), p.by_group), t_last = min(quotient(min(row0 + 31, p.rows - 1), p.by_group), step.n - 1);
   const int all_to = min(kTree ? step.base : step.base + t_first + 1, p.pages.room), all_from = step.base + (kTree ? step.n - 1 : t_last) - p.left;
   const int some_to = t_first >= step.n ? 0 : kTree ? walk.last + 1 : step.base + t_last + 1, some_from = step.base + (kTree ? 0 : t_first) - p.left;
-  f32x16 o[H::kBlocks];
+  f32x4 o[2][F::kBlocks];
+  float m_run[2], m_use[2], l_run[2];
 #pragma unroll
-  for (int x = 0; x < H::kBlocks; ++x) o[x] = f32x16{0};
-  float m_run = -INFINITY, m_use = 0.f, l_run = 0.f;
-  uint32_t nat[H::kSteps], tr[H::kBlocks];
+  for (int t = 0; t < 2; ++t) {
+    m_run[t] = -INFINITY;
+    m_use[t] = l_run[t] = 0.f;
 #pragma unroll
-  for (int i = 0; i < H::kSteps; ++i) nat[i] = H::at_n(lane & 31, 2 * i + (lane >> 5));
+    for (int d = 0; d < F::kBlocks; ++d) o[t][d] = f32x4{0};
+  }
+  uint32_t nat[F::kSteps], tr[F::kBlocks];
 #pragma unroll
-  for (int x = 0; x < H::kBlocks; ++x) tr[x] = kSecond + H::tr_offset(lane, x);
+  for (int k = 0; k < F::kSteps; ++k) nat[k] = col * F::kRow + (F::slot_k(col, 4 * k + quad) << 4);
+#pragma unroll
+  for (int d = 0; d < F::kBlocks; ++d) {
+    const int r = 4 * quad + (col >> 2);
+    tr[d] = kSecond + r * F::kRow + (F::slot_v(r, 2 * d + ((col & 3) >> 1)) << 4) + (col & 1) * 8;
+  }
 
   auto walk_step = [&](int i, auto stage_tag) {
     constexpr int kStage = decltype(stage_tag)::value;
@@ -606,83 +613,102 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
       turn_over();
       return;
     }
-    // S^T: two blocks of 32 keys in turn
-    f32x16 s[2] = {f32x16{0}, f32x16{0}};
+    // S^T: four blocks of 16 keys in turn, either of the wave's tiles.  From here through the exponentials the wave goes before the SIMD's other one, so that
+    // the two take turns, one's K products beside the other's V products: 2048 tokens of 8 x 4 heads after 6144 keys 245 -> 229 us,
+    // D = 64 157 -> 150; first through K's products alone 228 and 159, through V's products too 245 and 154, exponentials alone 242 and 152.
+    __builtin_amdgcn_s_setprio(1);
+    f32x4 s[2][4];
     {
-      constexpr int kAhead = 4, kAll = 2 * H::kSteps;
+      constexpr int kAhead = 4, kAll = 4 * F::kSteps;
       x8 kf[kAll];
-      auto rd = [&](int n) { return lds_get<x8>(here + nat[n >> 1] + 32 * H::kRow * (n & 1)); };
+      auto rd = [&](int n) { return lds_get<x8>(here + nat[n >> 2] + 16 * F::kRow * (n & 3)); };
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) kf[n] = rd(n);
       __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
       for (int n = 0; n < kAll; ++n) {
         if (n + kAhead < kAll) kf[n + kAhead] = rd(n + kAhead);
-        s[n & 1] = V::mfma(kf[n], qf[n >> 1], s[n & 1]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t][n & 3] = V::mfma16(kf[n], qf[t][n >> 2], n < 4 ? f32x4{0} : s[t][n & 3]);
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         if (n & 1) copy(n >> 1, at[n >> 1], other);
       }
-      static_assert(kAll / 2 == kPieces, "a copy after every other product");
+      static_assert(kAll / 2 == kPieces, "a copy after every other fragment");
     }
     const bool whole = key0 + kSwaBlock <= all_to && (key0 >= all_from || key0 + kSwaBlock <= p.sinks) && there == ~0ull;
     if (!whole) {
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb) {
-        const uint32_t seen = (sees.template word<kTree>(key0 + 32 * mb) & (uint32_t)(there >> (32 * mb))) >> (4 * (lane >> 5));
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (!(seen >> (8 * (j >> 2) + (j & 3)) & 1)) s[mb][j] = -INFINITY;
-      }
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t seen = (sees[t].template word<kTree>(key0 + 32 * half) & (uint32_t)(there >> (32 * half))) >> (4 * quad);
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (!(seen >> (16 * n + j) & 1)) s[t][2 * half + n][j] = -INFINITY;
+        }
     }
-    constexpr int kVAhead = 3, kVAll = 4 * H::kBlocks;
+    constexpr int kVAhead = 3, kVAll = 2 * F::kBlocks;
     x8 vf[4];
-    auto rd_v = [&](int n) {                // fragment n % kBlocks of 16 keys
-      const uint32_t a = here + tr[n % H::kBlocks] + 16 * H::kRow * (n / H::kBlocks);
-      return lds_tr_pair<T>(a, a + 8 * H::kRow);
+    auto rd_v = [&](int n) {                // fragment n % kBlocks of 32 keys
+      const uint32_t a = here + tr[n % F::kBlocks] + 32 * F::kRow * (n / F::kBlocks);
+      return lds_tr_pair<T>(a, a + 16 * F::kRow);
     };
 #pragma unroll
     for (int n = 0; n < kVAhead; ++n) vf[n] = rd_v(n);
-    float rs = 0.f;
-    x8 pf[4];
+    float rs[2];
+    x8 pf[2][2];
     auto exponentials = [&]() {
-      rs = 0.f;
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
+      for (int t = 0; t < 2; ++t) {
+        rs[t] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float e = fast_exp2(fmaf(s[mb][j], p.scale_log2, -m_use));
-          rs += e;
-          pf[2 * mb + (j >> 3)][j & 7] = (T)e;
-        }
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float e = fast_exp2(fmaf(s[t][n][j], p.scale_log2, -m_use[t]));
+            rs[t] += e;
+            pf[t][n >> 1][4 * (n & 1) + j] = (T)e;
+          }
+      }
     };
     exponentials();
-    if (__builtin_amdgcn_ballot_w64(!(rs < ManyRaise<T>::kSum) || m_run == -INFINITY) != 0) {        // wave-uniform, rare
-      float mx = s[0][0], a, c;
+    __builtin_amdgcn_s_setprio(0);
+    if (__builtin_amdgcn_ballot_w64(!(rs[0] < ManyRaise<T>::kSum) || !(rs[1] < ManyRaise<T>::kSum) || m_run[0] == -INFINITY || m_run[1] == -INFINITY) != 0) {
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
+      for (int t = 0; t < 2; ++t) {         // wave-uniform, rare
+        float mx = s[t][0][0], a, c;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[mb][j]);
-      swap_lanes<32>(mx, a, c);
-      const float m_new = fmaxf(m_run, fmaxf(a, c) * p.scale_log2);
-      m_use = m_new == -INFINITY ? 0.f : m_new - ManyRaise<T>::kBits;
-      const float alpha = m_new == m_run ? 1.f : fast_exp2(m_run - m_new);      // m_run = -inf -> 0
-      m_run = m_new;
-      l_run *= alpha;
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int x = 0; x < H::kBlocks; ++x)
+          for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[t][n][j]);
+        swap_lanes<16>(mx, a, c);
+        swap_lanes<32>(fmaxf(a, c), a, c);
+        const float m_new = fmaxf(m_run[t], fmaxf(a, c) * p.scale_log2);
+        m_use[t] = m_new == -INFINITY ? 0.f : m_new - ManyRaise<T>::kBits;
+        const float alpha = m_new == m_run[t] ? 1.f : fast_exp2(m_run[t] - m_new);      // m_run = -inf -> 0
+        m_run[t] = m_new;
+        l_run[t] *= alpha;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) o[x][j] *= alpha;
+        for (int d = 0; d < F::kBlocks; ++d) o[t][d] *= alpha;
+      }
       exponentials();
     }
-    l_run += rs;
+    l_run[0] += rs[0];
+    l_run[1] += rs[1];
     turn_over();
 #pragma unroll
     for (int n = 0; n < kVAll; ++n) {
       if (n + kVAhead < kVAll) vf[(n + kVAhead) & 3] = rd_v(n + kVAhead);
-      o[n % H::kBlocks] = V::mfma(vf[n & 3], pf[n / H::kBlocks], o[n % H::kBlocks]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) o[t][n % F::kBlocks] = V::mfma16(vf[n & 3], pf[t][n / F::kBlocks], o[t][n % F::kBlocks]);
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
   };
   for (int i = i0; i < i1; i += 2 * parts) {
@@ -692,42 +718,39 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
   wait_vmem_all();                          // the last step's copies filled a stage with zeros
   __syncthreads();
   if (n_rows <= 0) return;
-  float a, c;
-  swap_lanes<32>(l_run, a, c);
-  const float l = a + c;
   const PagedParams& e = parameters();
-  const bool any = (l > 0.f || l != l) && token < step.n;              // (NaN stays; a token that is none saw keys beside the others)
-  const float inv = any ? 1.f / l : 0.f, lse = any ? (m_use + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
-#pragma unroll
-  for (int x = 0; x < H::kBlocks; ++x)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[x][j] = any ? o[x][j] : 0.f;
-  const int out_lane = fresh_lane(), my_row = row0 + (out_lane & 31);
-  const RowPlace mine = row_place(e, hk, min(my_row, e.rows - 1));
-  const int64_t out_row = ((int64_t)b * e.n_heads + mine.head) * e.steps.n_tokens + mine.token;
-  if (e.n_parts > 1) {
-    if (my_row < e.rows && any) {
-      float* to = e.part_o + part * e.o_part + out_row * kD + 4 * (out_lane >> 5);
-#pragma unroll
-      for (int x = 0; x < H::kBlocks; ++x)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(to + 32 * x + 8 * g) = f32x4{o[x][4 * g] * inv, o[x][4 * g + 1] * inv, o[x][4 * g + 2] * inv, o[x][4 * g + 3] * inv};
-    }
-    if (my_row < e.rows && out_lane < 32) e.part_lse[part * e.lse_part + out_row] = lse;
-    return;
-  }
-  if (my_row < e.rows && out_lane < 32) e.lse[out_row] = lse;
   const uint32_t turn = lds[0] + wave * 32 * H::kRow;
 #pragma unroll
-  for (int x = 0; x < H::kBlocks; ++x)
+  for (int t = 0; t < 2; ++t) {
+    float a, c;
+    swap_lanes<16>(l_run[t], a, c);
+    swap_lanes<32>(a + c, a, c);
+    const float l = a + c;
+    const int row = row0 + 16 * t + col;
+    const bool any = (l > 0.f || l != l) && token[t] < step.n;         // (NaN stays; a token that is none saw keys beside the others)
+    const float inv = any ? 1.f / l : 0.f, lse = any ? (m_use[t] + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+    const RowPlace mine = row_place(e, hk, min(row, e.rows - 1));
+    const int64_t out_row = ((int64_t)b * e.n_heads + mine.head) * e.steps.n_tokens + mine.token;
+    if (e.n_parts > 1) {
+      if (row < e.rows && any) {
+        float* to = e.part_o + part * e.o_part + out_row * kD + 4 * quad;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      typename V::x4 w;
+        for (int d = 0; d < F::kBlocks; ++d) *reinterpret_cast<f32x4*>(to + 16 * d) = o[t][d] * inv;
+      }
+      if (row < e.rows && quad == 0) e.part_lse[part * e.lse_part + out_row] = lse;
+    } else {
+      if (row < e.rows && quad == 0) e.lse[out_row] = lse;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = (T)(o[x][4 * g + j] * inv);
-      lds_put(turn + H::at_n(out_lane & 31, 4 * x + g) + 8 * (out_lane >> 5), w);
+      for (int d = 0; d < F::kBlocks; ++d) {
+        typename V::x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = any ? (T)(o[t][d][j] * inv) : (T)0.f;
+        lds_put(turn + H::at_n(16 * t + col, 2 * d + (quad >> 1)) + 8 * (quad & 1), w);
+      }
     }
+  }
+  if (e.n_parts > 1) return;
+  const int out_lane = fresh_lane();
 #pragma unroll
   for (int i = 0; i < H::kSteps; ++i) {
     const int r = H::kCopyRows * i + out_lane / H::kChunks, ch = out_lane % H::kChunks;
@@ -787,14 +810,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams p, Di
 // tiles: 16-row tiles of a workgroup of few rows; row_tiles: workgroups of a key head's rows; least: blocks of a part
 struct PagedShape { bool many; int tiles, row_tiles, parts, least; };
 // Parts of a key head's keys: what an estimate in microseconds says of the longest walks that the call allows (lengths are on the device; shorter walks make fewer
-// parts).  Fitted to 4026 drawn calls of 1 to 64 sequences, 1 to 256 tokens, 60 to 33000 rows, each timed in up to 12 numbers of parts: what it takes is
-// 1.3 % (few rows) and 1.5 % (many) slower than the best of them on average, 8 and 9 % at the 95th percentile.  us in 1, 2, 4, 8, 16 and 32 parts:
+// parts).  Fitted to 2166 (few rows) and 3396 (many) drawn calls of 1 to 64 sequences, 1 to 256 tokens, 60 to 33000 rows, each timed in up to 12 numbers of
+// parts: what it takes is 1.3 and 1.8 % slower than the best of them on average, 8 and 10 % at the 95th percentile.  us in 1, 2, 4, 8, 16 and 32 parts:
 //     few    1 x 8, 4000 rows, 128 columns             38.7   25.0   17.3   13.2   11.3   11.2
 //            3 x 8, 6007 to 21353                     237    127     72.3   45.9   36.7   40.6
 //            64 x 8, 8192 to 16384                    549    560    571    594
-//     many   1 x 8, 2777 rows, 26 tokens of 4 heads    54.5   35.6   24.1   19.0   17.5   19.4
-//            16 x 8, 2048 to 8192, 64 tokens of 4     172    124    128    161
-//            3 x 8, 700 to 6000, 256 tokens           114     66.3   42.5   33.0   44
+//     many   1 x 8, 2777 rows, 26 tokens of 4 heads    58.3   36.1   24.4   19.3   17.8   19.9
+//            16 x 8, 2048 to 8192, 64 tokens of 4     171    122    123    155    213    374
+//            3 x 8, 700 to 6000, 256 tokens           118     67.5   41.9   32.2   38.6   48.4
 static PagedShape paged_shape(int batch, int n_tokens, int n_heads, int n_kv_heads, int room, int head_dim, int64_t left, int64_t sinks) {
   PagedShape s;
   const int64_t rows = (int64_t)n_tokens * (n_heads / n_kv_heads);
@@ -814,11 +837,11 @@ static PagedShape paged_shape(int batch, int n_tokens, int n_heads, int n_kv_hea
     return 2.4 + std::max(rounds * steps * step, memory) + (parts > 1 ? 4.1 + 0.024 * parts + entries * parts * 6e-7 : 0);
   };
   auto many_us = [&](int parts) {
-    const double alone = head_dim == 64 ? 0.9 : 1.35, shared = head_dim == 64 ? 1.05 : 1.78;            // a block of 64 keys; of two workgroups of a CU
+    const double alone = head_dim == 64 ? 0.9 : 1.31, shared = head_dim == 64 ? 1.0 : 1.5;             // a block of 64 keys; of two workgroups of a CU
     const double n = groups * parts, steps = std::ceil((double)seen / parts), beside = std::min(std::max((n - kCus) / kCus, 0.0), 1.0);
     double walk = std::max(steps * (alone + (shared - alone) * beside), groups * seen / (2 * kCus) * shared);
-    if (n > 2 * kCus) walk = std::max(walk, (n / (2 * kCus) + 0.18) * steps * shared);
-    return 13.4 + walk + (parts > 1 ? 5 + entries * parts * 1.67e-6 : 0);
+    if (n > 2 * kCus) walk = std::max(walk, (n / (2 * kCus) + 0.45) * steps * shared);
+    return 11.9 + walk + (parts > 1 ? 3.3 + entries * parts * 1.84e-6 : 0);
   };
   s.parts = 1;
   double best_us = 1e30;
