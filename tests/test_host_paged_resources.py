@@ -39,3 +39,11 @@ def test_two_workgroups_share_a_cu(kernels):
         if "paged_many_kernel" in name or ("paged_few_kernel" in name and "Li64E" in name):
             assert k["vgpr_count"] <= 256 and k["group_segment_fixed_size"] <= 80 << 10, (name, k)
         assert k["group_segment_fixed_size"] <= 160 << 10, (name, k)
+
+
+def test_three_workgroups_of_many_rows_of_64_share_a_cu(kernels):
+    """Three waves a SIMD have 168 registers each (of 512 in eights)."""
+    found = [k for name, k in kernels.items() if "paged_many_kernel" in name and "Li64E" in name]
+    assert len(found) == 4
+    for k in found:
+        assert k["vgpr_count"] <= 168 and 3 * k["group_segment_fixed_size"] <= 160 << 10, k

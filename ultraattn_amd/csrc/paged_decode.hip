@@ -464,8 +464,10 @@ __device__ __forceinline__ RowPlace row_place(const PagedParams& p, int hk, int 
   return {token, hk * p.group + row - token * p.group};
 }
 
+// Three workgroups of heads of 64 share a CU (two: 4 prompts of 2048 tokens of 8 x 4 heads 119 us where they take 108; 16 trees of 64 tokens after 2048 to 8192 keys
+// 85 and 77; one prompt of 2048 after 6144, which more parts than two a CU do not help, 152 and 160).
 template <class T, int kD, bool kTree>
-__global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p) {
+__global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void paged_many_kernel(const PagedParams p) {
   using H = SwaHead<kD>;
   using V = SwaVec<T>;
   typedef typename V::x8 x8;
@@ -523,8 +525,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
     if (lane < 2 * kMine) lds_put(places + 8 * lane, a);
     there_after = __builtin_amdgcn_ballot_w64(key0 + lane < end && (uint32_t)entry_lane < (uint32_t)p.pages.n_pages);
   };
-  auto entry_mine = [&](uint32_t at) { return lds_get<int>(at + 4 * key_row); };
-  auto entry_lane = [&](uint32_t at) { return lds_get<int>(at + 4 * lane); };
+  const uint32_t mine_at = entries + 4 * key_row, lane_at = entries + 4 * lane;
   auto place = [&](int n) { return lds_get<uint64_t>(places + 128 * (n & 1) + 8 * (H::kCopyRows * (n >> 1) + copy_row)) + (n & 1 ? v_chunk : k_chunk); };
   auto copy = [&](int n, uint64_t a, uint32_t stage) {
     dma16_at(a, stage + (n & 1 ? kSecond : 0) + (kPagedWaves * (n >> 1) + wave) * 1024);
@@ -546,7 +547,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
   asm volatile("" : "+v"(parent));
   wait_vmem_all();
   if (i0 < i1) {
-    locate(i0, entry_mine(entries_first), entry_lane(entries_first));
+    locate(i0, lds_get<int>(mine_at + 512), lds_get<int>(lane_at + 512));
     there = there_after;
     uint64_t at[kPieces];
 #pragma unroll
@@ -554,17 +555,13 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) copy(n, at[n], lds[0]);
-    locate(i0 + parts, entry_mine(entries + 256), entry_lane(entries + 256));
+    locate(i0 + parts, lds_get<int>(mine_at + 256), lds_get<int>(lane_at + 256));
     there_next = there_after;
   }
   if (kTree && i0 < i1) tree_branches(p, step, parent, branches);
   RowSees sees[2];
-  int token[2];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    token[t] = quotient(min(row0 + 16 * t + col, p.rows - 1), p.by_group);
-    sees[t].template of<kTree>(p, step, token[t], branches);
-  }
+  for (int t = 0; t < 2; ++t) sees[t].template of<kTree>(p, step, quotient(min(row0 + 16 * t + col, p.rows - 1), p.by_group), branches);
   // Keys that every real row of the wave sees: from .. to - 1, and those before `sinks` up to there.
   const int t_first = quotient(min(row0, p.rows - 1), p.by_group), t_last = min(quotient(min(row0 + 31, p.rows - 1), p.by_group), step.n - 1);
   const int all_to = min(kTree ? step.base : step.base + t_first + 1, p.pages.room), all_from = step.base + (kTree ? step.n - 1 : t_last) - p.left;
@@ -598,8 +595,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) at[n] = place(n);
     asm volatile("" ::: "memory");          // (read at once, not one by one before its copy)
-    const uint32_t entries_after = entries + 256 * kStage;
-    const int mine_after = entry_mine(entries_after), lane_after = entry_lane(entries_after);
+    const int mine_after = lds_get<int>(mine_at + 256 * kStage), lane_after = lds_get<int>(lane_at + 256 * kStage);
     fetch(i + 3 * parts, entries + 256 * (kStage ^ 1));
     auto turn_over = [&]() {
       locate(i + 2 * parts, mine_after, lane_after);
@@ -651,7 +647,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
               if (!(seen >> (16 * n + j) & 1)) s[t][2 * half + n][j] = -INFINITY;
         }
     }
-    constexpr int kVAhead = 3, kVAll = 2 * F::kBlocks;
+    constexpr int kVAhead = kD == 64 ? 2 : 3, kVAll = 2 * F::kBlocks;
     x8 vf[4];
     auto rd_v = [&](int n) {                // fragment n % kBlocks of 32 keys
       const uint32_t a = here + tr[n % F::kBlocks] + 32 * F::kRow * (n / F::kBlocks);
@@ -720,37 +716,37 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(const PagedParams p)
   if (n_rows <= 0) return;
   const PagedParams& e = parameters();
   const uint32_t turn = lds[0] + wave * 32 * H::kRow;
+  const int out_lane = fresh_lane(), out_col = out_lane & 15, out_quad = out_lane >> 4;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     float a, c;
     swap_lanes<16>(l_run[t], a, c);
     swap_lanes<32>(a + c, a, c);
     const float l = a + c;
-    const int row = row0 + 16 * t + col;
-    const bool any = (l > 0.f || l != l) && token[t] < step.n;         // (NaN stays; a token that is none saw keys beside the others)
-    const float inv = any ? 1.f / l : 0.f, lse = any ? (m_use[t] + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+    const int row = row0 + 16 * t + out_col;
     const RowPlace mine = row_place(e, hk, min(row, e.rows - 1));
+    const bool any = (l > 0.f || l != l) && mine.token < step.n;         // (NaN stays; a token that is none saw keys beside the others)
+    const float inv = any ? 1.f / l : 0.f, lse = any ? (m_use[t] + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
     const int64_t out_row = ((int64_t)b * e.n_heads + mine.head) * e.steps.n_tokens + mine.token;
     if (e.n_parts > 1) {
       if (row < e.rows && any) {
-        float* to = e.part_o + part * e.o_part + out_row * kD + 4 * quad;
+        float* to = e.part_o + part * e.o_part + out_row * kD + 4 * out_quad;
 #pragma unroll
         for (int d = 0; d < F::kBlocks; ++d) *reinterpret_cast<f32x4*>(to + 16 * d) = o[t][d] * inv;
       }
-      if (row < e.rows && quad == 0) e.part_lse[part * e.lse_part + out_row] = lse;
+      if (row < e.rows && out_quad == 0) e.part_lse[part * e.lse_part + out_row] = lse;
     } else {
-      if (row < e.rows && quad == 0) e.lse[out_row] = lse;
+      if (row < e.rows && out_quad == 0) e.lse[out_row] = lse;
 #pragma unroll
       for (int d = 0; d < F::kBlocks; ++d) {
         typename V::x4 w;
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = any ? (T)(o[t][d][j] * inv) : (T)0.f;
-        lds_put(turn + H::at_n(16 * t + col, 2 * d + (quad >> 1)) + 8 * (quad & 1), w);
+        lds_put(turn + H::at_n(16 * t + out_col, 2 * d + (out_quad >> 1)) + 8 * (out_quad & 1), w);
       }
     }
   }
   if (e.n_parts > 1) return;
-  const int out_lane = fresh_lane();
 #pragma unroll
   for (int i = 0; i < H::kSteps; ++i) {
     const int r = H::kCopyRows * i + out_lane / H::kChunks, ch = out_lane % H::kChunks;
@@ -810,7 +806,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams p, Di
 // tiles: 16-row tiles of a workgroup of few rows; row_tiles: workgroups of a key head's rows; least: blocks of a part
 struct PagedShape { bool many; int tiles, row_tiles, parts, least; };
 // Parts of a key head's keys: what an estimate in microseconds says of the longest walks that the call allows (lengths are on the device; shorter walks make fewer
-// parts).  Fitted to 2166 (few rows) and 3396 (many) drawn calls of 1 to 64 sequences, 1 to 256 tokens, 60 to 33000 rows, each timed in up to 12 numbers of
+// parts).  Fitted to 2166 (few rows) and 4612 (many) drawn calls of 1 to 64 sequences, 1 to 256 tokens, 60 to 33000 rows, each timed in up to 12 numbers of
 // parts: what it takes is 1.3 and 1.8 % slower than the best of them on average, 8 and 10 % at the 95th percentile.  us in 1, 2, 4, 8, 16 and 32 parts:
 //     few    1 x 8, 4000 rows, 128 columns             38.7   25.0   17.3   13.2   11.3   11.2
 //            3 x 8, 6007 to 21353                     237    127     72.3   45.9   36.7   40.6
@@ -837,10 +833,11 @@ static PagedShape paged_shape(int batch, int n_tokens, int n_heads, int n_kv_hea
     return 2.4 + std::max(rounds * steps * step, memory) + (parts > 1 ? 4.1 + 0.024 * parts + entries * parts * 6e-7 : 0);
   };
   auto many_us = [&](int parts) {
-    const double alone = head_dim == 64 ? 0.9 : 1.31, shared = head_dim == 64 ? 1.0 : 1.5;             // a block of 64 keys; of two workgroups of a CU
-    const double n = groups * parts, steps = std::ceil((double)seen / parts), beside = std::min(std::max((n - kCus) / kCus, 0.0), 1.0);
-    double walk = std::max(steps * (alone + (shared - alone) * beside), groups * seen / (2 * kCus) * shared);
-    if (n > 2 * kCus) walk = std::max(walk, (n / (2 * kCus) + 0.45) * steps * shared);
+    // a block of 64 keys by a workgroup that has its CU, and by one of two (heads of 64: three) that fill it
+    const double alone = head_dim == 64 ? 0.98 : 1.31, shared = head_dim == 64 ? 1.3 : 1.5, slots = (head_dim == 64 ? 3 : 2) * kCus;
+    const double n = groups * parts, steps = std::ceil((double)seen / parts), beside = std::min(std::max((n - kCus) / (slots - kCus), 0.0), 1.0);
+    double walk = std::max(steps * (alone + (shared - alone) * beside), groups * seen / slots * shared);
+    if (n > slots) walk = std::max(walk, (n / slots + 0.43) * steps * shared);
     return 11.9 + walk + (parts > 1 ? 3.3 + entries * parts * 1.84e-6 : 0);
   };
   s.parts = 1;
