@@ -124,20 +124,30 @@ struct PagedLane {
 constexpr int kDepth = 9, kExit = 10, kBranchPitch = 11;       // (words; odd, so that 32 tokens' lines meet 32 banks)
 struct Branches { uint32_t line[kTreeMost * kBranchPitch]; };
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
-// (see tree_part.)  A window cuts what is further behind and not among the sinks.
+// (see tree_part.)  A window cuts what is further behind and not among the sinks.  Of up to 64 tokens every wave stores all lines, with no barrier behind: each word
+// once, as it is read, so that no wave puts back what another reads already; what is cut is cut in registers.  kMost: tokens that the kernel takes at the most.
+template <int kMost>
 __device__ __forceinline__ void tree_branches(const PagedParams& p, const StepOf& of, int parent, Branches& out) {
   const int t = tree_token(p.steps), words = 2 * (t >> 6);
-  const bool alone = p.steps.n_tokens <= 64;
+  const bool alone = kMost <= 64 || p.steps.n_tokens <= 64, cut = p.left < p.steps.n_tokens;
   const TreePart x = tree_part(t, parent);
   uint32_t* const line = out.line + t * kBranchPitch;
   int depth = __popc(x.bits[0]) + __popc(x.bits[1]) - 1;
   line[0] = ~0u;
-  line[1 + words] = x.bits[0];
-  line[2 + words] = x.bits[1];
   if (alone) {
+    uint64_t bits = (uint64_t)x.bits[1] << 32 | x.bits[0];
+    if (cut)
+      for (int j = 0; j < p.steps.n_tokens; ++j) {        // (the wave's lanes are the tokens)
+        const int theirs = __builtin_amdgcn_readlane(depth, j);
+        if (depth - theirs > p.left && of.base + theirs >= p.sinks) bits &= ~(1ull << j);
+      }
+    line[1] = (uint32_t)bits;
+    line[2] = (uint32_t)(bits >> 32);
     line[3] = 0u;
     line[kDepth] = depth;
   } else {
+    line[1 + words] = x.bits[0];
+    line[2 + words] = x.bits[1];
     line[kExit] = x.exit;
     for (int w = 0; w < kTreeMost / 32; ++w)
       if (w < words || w > words + 1) line[1 + w] = 0u;
@@ -153,19 +163,19 @@ __device__ __forceinline__ void tree_branches(const PagedParams& p, const StepOf
     }
     line[kDepth] = depth;
     __syncthreads();
-  }
-  if (p.left < p.steps.n_tokens) {
-    asm volatile("" ::: "memory");
-    for (int w = 0; w <= words + 1; ++w) {
-      const uint32_t all = line[1 + w];
-      uint32_t kept = all;
-      for (uint32_t rest = all; rest; rest &= rest - 1) {
-        const int theirs = (int)out.line[(32 * w + __ffs(rest) - 1) * kBranchPitch + kDepth];
-        if (depth - theirs > p.left && of.base + theirs >= p.sinks) kept &= ~(rest & -rest);
+    if (cut) {                                            // (of its own line, by its one thread; of the others only the depths are read)
+      asm volatile("" ::: "memory");
+      for (int w = 0; w <= words + 1; ++w) {
+        const uint32_t all = line[1 + w];
+        uint32_t kept = all;
+        for (uint32_t rest = all; rest; rest &= rest - 1) {
+          const int theirs = (int)out.line[(32 * w + __ffs(rest) - 1) * kBranchPitch + kDepth];
+          if (depth - theirs > p.left && of.base + theirs >= p.sinks) kept &= ~(rest & -rest);
+        }
+        line[1 + w] = kept;
       }
-      line[1 + w] = kept;
+      __syncthreads();
     }
-    if (!alone) __syncthreads();
   }
   asm volatile("" ::: "memory");
 }
@@ -309,7 +319,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_few_kernel(const Pa
       copy_in(mine + H::kStage);
     }
   }
-  if constexpr (kTree) tree_branches(p, step, parent, branches);
+  if constexpr (kTree) tree_branches<kRows>(p, step, parent, branches);
   RowSees sees[kTiles];
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) sees[t].template of<kTree>(p, step, quotient(min(row0 + 16 * t + col, p.rows - 1), p.by_group), branches);
@@ -558,7 +568,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void paged_many_kernel(const
     locate(i0 + parts, lds_get<int>(mine_at + 256), lds_get<int>(lane_at + 256));
     there_next = there_after;
   }
-  if (kTree && i0 < i1) tree_branches(p, step, parent, branches);
+  if (kTree && i0 < i1) tree_branches<kTreeMost>(p, step, parent, branches);
   RowSees sees[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) sees[t].template of<kTree>(p, step, quotient(min(row0 + 16 * t + col, p.rows - 1), p.by_group), branches);
