@@ -436,7 +436,7 @@ int ua_paged_append(const void *q, const void *k, const void *v, void *q_out, vo
 /* Their attention: q, o [batch, n_tokens, n_heads, head_dim], lse [batch, n_heads, n_tokens].  A token sees the rows before base and the tokens of its branch,
  * itself among them; with left >= 0 of both only what is at most `left` positions before its own, and the first `sinks` positions.  Tokens that see nothing, and
  * those that are not real, get o = 0, lse = -inf.  Types, alignment and strides (pools: non-negative multiples of 8 elements) and what may be NaN as in ua_swa_decode; of a
- * tree's tokens NaN in a key or value may reach all of the sequence's new tokens.  o may be q itself.
+ * tree's tokens NaN in a key or value may reach all of the sequence's new tokens.  P is rounded to dtype.  o may be q itself.
  * Long caches are cut into parts if `workspace` (16-byte aligned) holds ua_paged_decode_workspace_bytes(). */
 int64_t ua_paged_decode_workspace_bytes(int batch, int n_tokens, int n_heads, int n_kv_heads, int page, int max_pages, int head_dim, int64_t left, int64_t sinks);
 int ua_paged_decode(const void *q, const void *k_pages, const void *v_pages, void *o, float *lse,

@@ -4,7 +4,8 @@
 //   few rows (up to 32 of a key head): as against a contiguous cache, four waves of a workgroup go through blocks of 32 keys of their own, rows are the columns
 //     of 16x16x32 products, and the waves' rows are merged at the end.  Bound: HBM, the visible keys and values once.
 //   many rows: tiles of 128, 32 a wave as two times 16 columns of the same products, go through blocks of 64 keys together (two LDS stages).  Bound: the products,
-//     or HBM where the tiles are few.  (With 32x32x16 products, half as many instructions, 2048 tokens of 8 x 4 heads after 6144 keys took 247 us, with these 235.)
+//     or HBM where the tiles are few.  (With 32x32x16 products, half as many instructions, 2048 tokens of 8 x 4 heads after 6144 keys took 247 us, with these 235, on one card;
+//     as it is now, 225 to 231 on four.)
 // The keys of long caches are cut into parts, workgroups of their own, that leave fp32 rows for a merge.
 //
 // Pages: a lane's copy names its own address, so a block's keys may lie on any pages and start anywhere.  The table's entries come into LDS two blocks ahead, by
@@ -13,6 +14,10 @@
 //
 // What a row sees of 32 keys is one word: up to its own position, from its window's first key on or among the sinks, on pages that are there, and of
 // the new tokens those of its branch.
+//
+// P is rounded to the operands' type, which the matrix instruction asks for: independent errors of half a step, which the sum over the keys averages, beside the one
+// of O (relative error against 64 bits, bf16 2.3e-3 where O's alone is 1.7e-3).  A second product of what the rounding leaves would double V's.  Sums,
+// statistics and parts' rows stay in 32 bits.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -90,7 +95,8 @@ struct PagedWalk {
     n_sink = (sinks_end + kKeys - 1) / kKeys;
     n = n_sink + (last >= start ? (last - start) / kKeys + 1 : 0);
   }
-  // Parts that the walk is cut into: all of p.n_parts, but none of fewer blocks than p.least.  A part takes every so many-th block.
+  // Parts that the walk is cut into: all of p.n_parts, but no more than its blocks in runs of p.least, a last shorter run included.  A part takes every so many-th
+  // block, so that parts differ by one, and may have fewer than p.least.
   __device__ __forceinline__ int parts(const PagedParams& p) const { return min(p.n_parts, max((n + p.least - 1) / p.least, 1)); }
   __device__ __forceinline__ int at(int i) const { return i < n_sink ? i * kKeys : start + (i - n_sink) * kKeys; }
   __device__ __forceinline__ int end_of(int i) const { return i < n_sink ? sinks_end : last + 1; }
@@ -620,7 +626,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void paged_many_kernel(const
       return;
     }
     // S^T: four blocks of 16 keys in turn, either of the wave's tiles.  From here through the exponentials the wave goes before the SIMD's other one, so that
-    // the two take turns, one's K products beside the other's V products: 2048 tokens of 8 x 4 heads after 6144 keys 245 -> 229 us,
+    // the two take turns, one's K products beside the other's V products: 2048 tokens of 8 x 4 heads after 6144 keys 245 -> 229 us (one card, in turn),
     // D = 64 157 -> 150; first through K's products alone 228 and 159, through V's products too 245 and 154, exponentials alone 242 and 152.
     __builtin_amdgcn_s_setprio(1);
     f32x4 s[2][4];
@@ -817,7 +823,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams p, Di
 struct PagedShape { bool many; int tiles, row_tiles, parts, least; };
 // Parts of a key head's keys: what an estimate in microseconds says of the longest walks that the call allows (lengths are on the device; shorter walks make fewer
 // parts).  Fitted to 2166 (few rows) and 4612 (many) drawn calls of 1 to 64 sequences, 1 to 256 tokens, 60 to 33000 rows, each timed in up to 12 numbers of
-// parts: what it takes is 1.3 and 1.8 % slower than the best of them on average, 8 and 10 % at the 95th percentile.  us in 1, 2, 4, 8, 16 and 32 parts:
+// parts: what it takes is 1.3 and 1.8 % slower than the best of them on average, 8 and 10 % at the 95th percentile.  The tables of all
+// these calls were as wide as their longest sequence.  Wider ones are cut for the walks that they allow: 26 tokens of 8 x 4 heads after 2751 rows 17.7 us in a table of 2784
+// rows, 20.0 of 8192, 23.4 of 32768 and more; 64 x 8 of 8192 to 16384, one token, 555 in 16384 and 584 in 131072.  us in 1, 2, 4, 8, 16 and 32 parts:
 //     few    1 x 8, 4000 rows, 128 columns             38.7   25.0   17.3   13.2   11.3   11.2
 //            3 x 8, 6007 to 21353                     237    127     72.3   45.9   36.7   40.6
 //            64 x 8, 8192 to 16384                    549    560    571    594

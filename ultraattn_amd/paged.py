@@ -7,7 +7,8 @@ state, so every call can be captured into a HIP graph, and one captured call ser
 
 The cache is two pools ``[n_pages, page, Hk, D]`` (any page size and strides, views of one tensor too) and a ``table``, int32 ``[B, max_pages]`` on the device: row r of
 sequence b is slot ``r % page`` of page ``table[b, r // page]``.  An entry outside the pool (-1, say) is a page that is not there: nothing is written to it, and its rows
-are not seen, so that pages behind a window may be given back.  A contiguous cache ``[B, room, Hk, D]`` is one too, with ``table = arange(B)[:, None]``.
+are not seen, so that pages behind a window may be given back.  A contiguous cache ``[B, room, Hk, D]`` is one too, with ``table = arange(B)[:, None]``.  ``paged_decode`` reads caches of bf16 or fp16 with heads of 64 or 128;
+``paged_append`` and ``paged_keep`` also take fp32 and other head sizes, for readers of the caller's own.
 
 A step brings T tokens of every sequence, of which ``n_new`` (int32 ``[B]``; None: all) are real.  ``lens`` (int32 ``[B]``) counts the real ones: token t is row
 ``base + t`` of its sequence, ``base = lens - n_new``.  The tokens are a chain, or with ``parents`` (int32 ``[B, T]``, or ``[T]`` for one tree in all sequences, T up to 256)
@@ -48,7 +49,7 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     A token sees the rows before ``base`` and its own branch, itself included; with ``window >= 0`` of both only what is at most ``window`` positions before it, and the first
     ``sinks`` positions.  One that sees nothing, or is not real, gets ``out = 0``, ``lse = -inf``.  bf16 or fp16, D 64 or 128, Hq a multiple of Hk, strides multiples of 8
     elements.  What lies behind ``lens``, and rows that no token sees, may be anything; NaN in a drafted token's key or value may reach all drafts of its sequence, in
-    another row that is seen also rows beside those that see it."""
+    another row that is seen also rows beside those that see it.  Probabilities are rounded to the type before they meet the values; sums and ``lse`` are 32 bits."""
     return native().paged_decode(q, k_pages, v_pages, table, lens, n_new, parents, window, sinks, softmax_scale, out, lse)
 
 
